@@ -6,8 +6,11 @@ CSRC     := ruvector_amd/csrc
 BUILD    := build
 # -ffp-contract=off: no implicit FMA, so kernels that restate the reference's
 # scalar arithmetic (distances, aggregation) reproduce it bit for bit; FMA is
-# only used where a kernel asks for it (MFMA, fmaf).
+# only used where a kernel asks for it (MFMA, fmaf). -packed-fp32-ops: no packed
+# f32 instructions, some forms of which have given wrong results on this hardware
+# (the host pass warns that it does not know the feature: harmless).
 HIPFLAGS := -O3 -std=c++17 -fPIC --offload-arch=$(ARCH) -ffp-contract=off -Iinclude -I$(CSRC) \
+            -Xclang -target-feature -Xclang -packed-fp32-ops \
             -Wall -Wno-unused-function -Wno-unused-variable -Wno-unused-result -Wno-unused-value
 LDFLAGS  := -shared --offload-arch=$(ARCH) -L/opt/rocm/lib -lamdhip64 -lrccl -Wl,-rpath,/opt/rocm/lib
 

@@ -68,6 +68,12 @@ rvx_status rvx_set_device(int32_t device);
 rvx_status rvx_get_device(int32_t* device);
 /* Wait for all work the library queued on the current device. */
 rvx_status rvx_synchronize(void);
+/* Order the library's work on the current device against another stream's (a hipStream_t of the
+ * same device; NULL = the default stream), without waiting on the host: after
+ * rvx_stream_wait(s) the library's later work waits for what is queued on s; after
+ * rvx_stream_signal(s) later work on s waits for what the library has queued. */
+rvx_status rvx_stream_wait(void* stream);
+rvx_status rvx_stream_signal(void* stream);
 /* Free the per-device scratch pool (pipeline chunk buffers, scan images, ...) that compute
  * calls keep for reuse; the next call re-allocates what it needs. */
 rvx_status rvx_scratch_release(void);
@@ -366,6 +372,56 @@ rvx_status rvx_dual_attention_compute(const rvx_dual_attention* a, const float* 
  * of x [N][dim]); y [N][dim]; isolated rows give zeros. */
 rvx_status rvx_dual_attention_forward_graph_device(const rvx_dual_attention* a, const rvx_graph* g,
                                                    const rvx_buffer* x, rvx_buffer* y);
+
+/* ------------------------------------------------------------------ */
+/* Training and serving the embeddings (rvx extensions)                */
+/* ------------------------------------------------------------------ */
+/* Element types of the entry points below; sums, softmax statistics and norms are kept in 32
+ * bits whatever the type, results are rounded once, to nearest even. */
+enum { RVX_DTYPE_F32 = 0, RVX_DTYPE_F16 = 1, RVX_DTYPE_BF16 = 2 };
+
+/* Rows of a learned table by id: out[i] = scale * table[ids[i]] for i < n, table [rows][dim] and
+ * out [n][dim] of `dtype`, ids int64. An id outside [0, rows) is absent: its row of out is zeros.
+ * rows < 2^31 - 1, n < 2^31, 1 <= dim <= 65536; out must not be the table. */
+rvx_status rvx_embedding_forward_device(const rvx_buffer* table, int32_t dtype, int64_t rows, int32_t dim,
+                                        const rvx_buffer* ids_i64, int64_t n, float scale, rvx_buffer* out);
+/* Its gradient: g[v] = scale * sum of grad_out[i] over the i with ids[i] = v, each sum in 32 bits
+ * and in an order that depends on ids alone (two calls give the same bits). grad_out [n][dim] of
+ * `dtype`. accumulate == 0: grad_table [rows][dim] of `table_dtype` = g, every row written.
+ * accumulate != 0: grad_table += g, rounded once per element and call; rows without an id are
+ * left as they are. Absent ids add to nothing. */
+rvx_status rvx_embedding_backward_device(const rvx_buffer* grad_out, int32_t dtype, const rvx_buffer* ids_i64, int64_t n,
+                                         int64_t rows, int32_t dim, float scale, int32_t accumulate,
+                                         int32_t table_dtype, rvx_buffer* grad_table);
+
+/* Log probabilities of given ids over rows of scores, with entropy and the best alternatives:
+ * scores [n][c] of `dtype`, row i at element i * ld (ld >= c), p = softmax(scores / temperature).
+ * Every output is nullable (= not wanted):
+ *   logp    [n] f32    log p[targets[i]]; 0 where the target is outside [0, c) (no target)
+ *   rank    [n] int64  how many ids are ranked before the target (higher score, or the same score
+ *                      and a lower id); -1 without a target
+ *   entropy [n] f32    -sum p log p
+ *   stats   [n][2] f32 the largest score m of the row and log sum exp((score - m) / temperature):
+ *                      what the backward pass reads
+ *   top_ids [n][k] int64, top_logp [n][k] f32: the k best ids (k <= 64), scores descending, the
+ *                      lowest id first among equals; -1 / -inf past the scores above -inf
+ * logp and rank need targets. Scores of -inf are masked: p = 0. A row with nothing above -inf has
+ * logp -inf, entropy 0, stats (-inf, -inf). A NaN or a +inf makes its row's logp, entropy and log
+ * sum NaN; NaN is never ranked or listed. */
+rvx_status rvx_log_probs_device(const rvx_buffer* scores, int32_t dtype, int64_t n, int64_t c, int64_t ld,
+                                float temperature, const rvx_buffer* targets_i64, int32_t k, rvx_buffer* logp,
+                                rvx_buffer* rank_i64, rvx_buffer* entropy, rvx_buffer* stats, rvx_buffer* top_ids_i64,
+                                rvx_buffer* top_logp);
+/* Its gradient by the scores: grad[i][j] = (grad_logp[i] (1{j = targets[i]} - p_j)
+ *   - grad_entropy[i] p_j (log p_j + entropy[i])) / temperature, [n][c] of `dtype`, row i at element
+ * i * ld_grad; elements c .. ld_grad of a row are left as they are. stats and entropy are the
+ * forward call's (entropy only with grad_entropy); grad_logp needs targets, and either gradient
+ * may be NULL = zeros. Rows with nothing above -inf get zeros (a masked score has p = 0, so it gets
+ * zero unless it is the target). grad may be the scores buffer itself when ld_grad == ld. */
+rvx_status rvx_log_probs_backward_device(const rvx_buffer* scores, int32_t dtype, int64_t n, int64_t c, int64_t ld,
+                                         float temperature, const rvx_buffer* targets_i64, const rvx_buffer* stats,
+                                         const rvx_buffer* grad_logp, const rvx_buffer* entropy,
+                                         const rvx_buffer* grad_entropy, rvx_buffer* grad, int64_t ld_grad);
 
 /* ------------------------------------------------------------------ */
 /* Vector index: VectorIndex (crates/ruvector-core/src/index.rs:11-36) */

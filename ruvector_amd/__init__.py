@@ -9,7 +9,8 @@ from . import _lib
 _lib.load()
 
 from ._lib import RvxError  # noqa: E402
-from .device import Buffer, Profiler, device_count, device_info, release_scratch, set_device, synchronize  # noqa: E402
+from .device import (Buffer, Profiler, device_count, device_info, release_scratch, set_device, stream_signal,  # noqa: E402
+                     stream_wait, synchronize)
 from .graph import Graph  # noqa: E402
 from .core import (DistanceMetric, FlatIndex, HnswConfig, HnswIndex, RuvectorError, SearchResult,  # noqa: E402
                    batch_distances, distance, distance_matrix, hnsw_last_search_stats, scan_last_stats)
@@ -21,6 +22,8 @@ from .attention import DualSpaceAttention, DualSpaceConfig, EdgeFeaturedAttentio
 from .hyperbolic import (DualSpaceIndex, HyperbolicError, HyperbolicHnsw, HyperbolicHnswConfig,  # noqa: E402
                          ShardedHyperbolicHnsw, ShardedHyperbolicSearch)
 
+from .embedding import EmbeddingError, embedding_backward_device, embedding_forward_device  # noqa: E402
+from .logprobs import LogProbsError, log_probs_backward_device, log_probs_device  # noqa: E402
 from .query import NeuralSearch, QueryMode, RuvectorQuery  # noqa: E402
 from .vector_db import DbOptions, SearchQuery, VectorDB, VectorEntry  # noqa: E402
 
@@ -33,6 +36,8 @@ __all__ = [
     "EdgeFeaturedConfig", "HyperbolicError", "HyperbolicHnsw", "HyperbolicHnswConfig", "ShardedHyperbolicHnsw", "ShardedHyperbolicSearch",
     "DualSpaceIndex",
     "NeuralSearch", "QueryMode", "RuvectorQuery", "DbOptions", "SearchQuery", "VectorDB", "VectorEntry", "differentiable_search_device", "hnsw_last_search_stats", "scan_last_stats",
+    "stream_wait", "stream_signal", "EmbeddingError", "embedding_forward_device", "embedding_backward_device",
+    "LogProbsError", "log_probs_device", "log_probs_backward_device",
     "pack_row_image", "row_image", "row_image_bytes",
 ]
 __version__ = "0.1.0"

@@ -27,6 +27,7 @@ STATUS_NAMES = {
 
 METRIC_L2, METRIC_COSINE, METRIC_DOT, METRIC_L1, METRIC_POINCARE, METRIC_HYP_L2 = 0, 1, 2, 3, 4, 5
 INDEX_FLAT, INDEX_HNSW = 0, 1
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 AGG_SUM, AGG_MEAN, AGG_MAX = 0, 1, 2
 SAGE_MEAN, SAGE_MAXPOOL, SAGE_LSTM = 0, 1, 2
 
@@ -91,6 +92,8 @@ SIGNATURES = {
     "rvx_set_device": (None, [I32]),
     "rvx_get_device": (None, [PI32]),
     "rvx_synchronize": (None, []),
+    "rvx_stream_wait": (None, [P]),
+    "rvx_stream_signal": (None, [P]),
     "rvx_scratch_release": (None, []),
     "rvx_device_info": (None, [PI32, PI64, C.c_char_p, SZ]),
     "rvx_buffer_alloc": (None, [I64, PP]),
@@ -153,6 +156,10 @@ SIGNATURES = {
     "rvx_dual_attention_destroy": (None, [P]),
     "rvx_dual_attention_compute": (None, [P, PF32, PF32, PF32, I32, I32, PF32]),
     "rvx_dual_attention_forward_graph_device": (None, [P, P, P, P]),
+    "rvx_embedding_forward_device": (None, [P, I32, I64, I32, P, I64, F32, P]),
+    "rvx_embedding_backward_device": (None, [P, I32, P, I64, I64, I32, F32, I32, I32, P]),
+    "rvx_log_probs_device": (None, [P, I32, I64, I64, I64, F32, P, I32, P, P, P, P, P, P]),
+    "rvx_log_probs_backward_device": (None, [P, I32, I64, I64, I64, F32, P, P, P, P, P, P, I64]),
     "rvx_index_create": (None, [C.POINTER(IndexConfig), PP]),
     "rvx_index_destroy": (None, [P]),
     "rvx_index_add_batch": (None, [P, PF32, PU64, I64]),

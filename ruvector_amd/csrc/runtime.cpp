@@ -246,6 +246,27 @@ rvx_status rvx_synchronize(void) {
     return guard([&] { sync(); });
 }
 
+static void stream_order(hipStream_t first, hipStream_t then) {
+    hipEvent_t e;
+    RVX_HIP(hipEventCreateWithFlags(&e, hipEventDisableTiming));
+    hipError_t st = hipEventRecord(e, first);
+    if (st == hipSuccess) st = hipStreamWaitEvent(then, e, 0);
+    hipEventDestroy(e);  // the queued wait keeps what it needs
+    RVX_HIP(st);
+}
+rvx_status rvx_stream_wait(void* s) {
+    return guard([&] {
+        const hipStream_t mine = stream();
+        stream_order((hipStream_t)s, mine);
+    });
+}
+rvx_status rvx_stream_signal(void* s) {
+    return guard([&] {
+        const hipStream_t mine = stream();
+        stream_order(mine, (hipStream_t)s);
+    });
+}
+
 rvx_status rvx_device_info(int32_t* num_cus, int64_t* hbm_bytes, char* arch, size_t arch_len) {
     return guard([&] {
         Device& d = device();

@@ -34,6 +34,60 @@ def device_info() -> dict:
     return {"num_cus": cus.value, "hbm_bytes": hbm.value, "arch": arch.value.decode()}
 
 
+def stream_wait(stream: int = 0) -> None:
+    """The library's later work on the current device waits for what is queued on `stream` (a
+    hipStream_t as an integer, e.g. torch.cuda.current_stream().cuda_stream), without waiting here."""
+    L.call("rvx_stream_wait", int(stream))
+
+
+def stream_signal(stream: int = 0) -> None:
+    """Later work on `stream` waits for what the library has queued on the current device."""
+    L.call("rvx_stream_signal", int(stream))
+
+
+_DTYPES = {"f32": L.DTYPE_F32, "f16": L.DTYPE_F16, "bf16": L.DTYPE_BF16}
+
+
+def dtype_code(dtype: str) -> int:
+    """The RVX_DTYPE_* of an element type's name."""
+    try:
+        return _DTYPES[dtype]
+    except (KeyError, TypeError):
+        raise L.RvxError(2, f"unknown dtype {dtype!r}: one of {', '.join(_DTYPES)}") from None
+
+
+class _DLTensor(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("device_type", C.c_int32), ("device_id", C.c_int32), ("ndim", C.c_int32),
+                ("code", C.c_uint8), ("bits", C.c_uint8), ("lanes", C.c_uint16), ("shape", C.POINTER(C.c_int64)),
+                ("strides", C.POINTER(C.c_int64)), ("byte_offset", C.c_uint64)]
+
+
+class _DLManaged(C.Structure):
+    pass
+
+
+_DLDeleter = C.CFUNCTYPE(None, C.POINTER(_DLManaged))
+_DLManaged._fields_ = [("tensor", _DLTensor), ("ctx", C.c_void_p), ("deleter", _DLDeleter)]
+_DL_ROCM = 10
+_exported = {}  # address of a _DLManaged -> what it needs alive until its consumer is done
+
+
+@_DLDeleter
+def _dl_release(managed):
+    _exported.pop(C.addressof(managed.contents), None)
+
+
+_capsule_new = C.PYFUNCTYPE(C.py_object, C.c_void_p, C.c_char_p, C.c_void_p)(("PyCapsule_New", C.pythonapi))
+_capsule_valid = C.PYFUNCTYPE(C.c_int, C.c_void_p, C.c_char_p)(("PyCapsule_IsValid", C.pythonapi))
+_capsule_pointer = C.PYFUNCTYPE(C.c_void_p, C.c_void_p, C.c_char_p)(("PyCapsule_GetPointer", C.pythonapi))
+
+
+@C.CFUNCTYPE(None, C.c_void_p)
+def _dl_dropped(capsule):
+    if _capsule_valid(capsule, b"dltensor"):  # no consumer took it
+        _exported.pop(_capsule_pointer(capsule, b"dltensor"), None)
+
+
 class Buffer:
     """A device allocation owned by librvx (row-major f32/i32/i64 data)."""
 
@@ -42,10 +96,30 @@ class Buffer:
         L.call("rvx_buffer_alloc", int(nbytes), C.byref(h))
         self._h = h
         self.nbytes = int(nbytes)
+        dev = C.c_int32(0)
+        L.call("rvx_get_device", C.byref(dev))
+        self._device = dev.value
 
     @property
     def handle(self):
         return self._h
+
+    def __dlpack_device__(self):
+        return (_DL_ROCM, self._device)
+
+    def __dlpack__(self, stream=None, **_):
+        """The allocation as a flat uint8 tensor of another library (DLPack, no copy): what that
+        library queues on `stream` waits for the library's work so far. What it writes is ordered
+        before later rvx calls by stream_wait(stream). The tensor keeps this Buffer alive."""
+        if not self._h:
+            raise L.RvxError(2, "the buffer is freed")
+        if stream != -1:
+            stream_signal(0 if stream in (None, 1) else stream)
+        shape, strides = (C.c_int64 * 1)(self.nbytes), (C.c_int64 * 1)(1)
+        m = _DLManaged(_DLTensor(L.load().rvx_buffer_device_ptr(self._h), _DL_ROCM, self._device, 1, 1, 8, 1, shape,
+                                 strides, 0), None, _dl_release)
+        _exported[C.addressof(m)] = (m, self, shape, strides)
+        return _capsule_new(C.addressof(m), b"dltensor", C.cast(_dl_dropped, C.c_void_p))
 
     @classmethod
     def from_numpy(cls, a: np.ndarray) -> "Buffer":

@@ -1,0 +1,54 @@
+"""Arguments that the typed operators refuse, without a GPU: what is wrong by itself is found
+before any buffer or device is looked at."""
+import pytest
+
+import ruvector_amd as rv
+from ruvector_amd import _lib as L
+
+
+def _status(name, *args):
+    lib = L.load()
+    st = getattr(lib, name)(*args)
+    return st, L.last_error()
+
+
+@pytest.mark.parametrize("dtype,rows,dim,n,word", [
+    (3, 8, 8, 8, "dtype"), (-1, 8, 8, 8, "dtype"), (0, 0, 8, 8, "rows"), (0, 2 ** 31 - 1, 8, 8, "rows"),
+    (0, 8, 0, 8, "dim"), (0, 8, 65537, 8, "dim"), (0, 8, 8, -1, "n must"), (0, 8, 8, 2 ** 31, "n must"), (0, 8, 8, 8, "null")])
+def test_embedding(dtype, rows, dim, n, word):
+    st, msg = _status("rvx_embedding_forward_device", None, dtype, rows, dim, None, n, 1.0, None)
+    assert st == 2 and word in msg
+    st, msg = _status("rvx_embedding_backward_device", None, dtype, None, n, rows, dim, 1.0, 0, 0, None)
+    assert st == 2 and word in msg
+
+
+def test_embedding_table_dtype():
+    st, msg = _status("rvx_embedding_backward_device", None, 0, None, 8, 8, 8, 1.0, 0, 9, None)
+    assert st == 2 and "dtype" in msg
+
+
+@pytest.mark.parametrize("dtype,n,c,ld,temperature,k,word", [
+    (7, 4, 8, 8, 1.0, 0, "dtype"), (0, -1, 8, 8, 1.0, 0, "n must"), (0, 2 ** 31, 8, 8, 1.0, 0, "n must"),
+    (0, 4, 0, 8, 1.0, 0, "c must"), (0, 4, 2 ** 31, 2 ** 32, 1.0, 0, "c must"), (0, 4, 8, 7, 1.0, 0, "stride"),
+    (0, 4, 8, 2 ** 41, 1.0, 0, "stride"), (0, 4, 8, 8, 0.0, 0, "temperature"), (0, 4, 8, 8, -1.0, 0, "temperature"),
+    (0, 4, 8, 8, float("nan"), 0, "temperature"), (0, 4, 8, 8, float("inf"), 0, "temperature"),
+    (0, 4, 8, 8, 1e-45, 0, "temperature"), (0, 4, 8, 8, 1.0, 0, "null")])
+def test_log_probs(dtype, n, c, ld, temperature, k, word):
+    st, msg = _status("rvx_log_probs_device", None, dtype, n, c, ld, temperature, None, k, *[None] * 6)
+    assert st == 2 and word in msg
+    st, msg = _status("rvx_log_probs_backward_device", None, dtype, n, c, ld, temperature, None, None, None, None, None, None, ld)
+    assert st == 2 and word in msg
+
+
+@pytest.mark.parametrize("k", [-1, 65])
+def test_log_probs_k(k):
+    st, msg = _status("rvx_log_probs_device", None, 0, 4, 8, 8, 1.0, None, k, *[None] * 6)
+    assert st == 2 and "k must" in msg
+
+
+def test_dtype_names():
+    from ruvector_amd.device import dtype_code
+    assert [dtype_code(d) for d in ("f32", "f16", "bf16")] == [0, 1, 2]
+    for bad in ("f64", None, 2, []):
+        with pytest.raises(rv.RvxError):
+            dtype_code(bad)
