@@ -423,6 +423,31 @@ rvx_status rvx_log_probs_backward_device(const rvx_buffer* scores, int32_t dtype
                                          const rvx_buffer* grad_logp, const rvx_buffer* entropy,
                                          const rvx_buffer* grad_entropy, rvx_buffer* grad, int64_t ld_grad);
 
+/* AdapterLinear: a shared projection with one low-rank adapter per row, for batches whose rows
+ * belong to different tenants or requests:
+ *   y[i] = W x[i] + bias + scale_r B_r (A_r x[i]),  r = adapter_ids[i],
+ * W [out][in], bias [out], A_r [rank_r][in], B_r [out][rank_r], x [n][in], y [n][out], all row-major
+ * of the layer's dtype; A_r x is kept in 32 bits. The layer copies weights and adapters into its
+ * own layout, so their buffers may be freed after the call. A row whose id is outside
+ * [0, max_adapters), or names a slot never set or set with rank 0, has no adapter. */
+typedef struct rvx_adapter_linear rvx_adapter_linear;
+typedef struct {
+    int32_t in_features, out_features;  /* 1 .. 65536 */
+    int32_t dtype;                      /* RVX_DTYPE_* */
+    int32_t max_rank;                   /* 1 .. 128 */
+    int32_t max_adapters;               /* slots, 0 .. 65536 */
+} rvx_adapter_linear_config;
+rvx_status rvx_adapter_linear_create(const rvx_adapter_linear_config* cfg, const rvx_buffer* weight,
+                                     const rvx_buffer* bias /*nullable*/, rvx_adapter_linear** out);
+rvx_status rvx_adapter_linear_destroy(rvx_adapter_linear* l);
+/* Set (or replace) the adapter of a slot; rank 0 removes it (a and b are then ignored). Forward
+ * calls made before keep the adapter they had. */
+rvx_status rvx_adapter_linear_set(rvx_adapter_linear* l, int32_t slot, int32_t rank, const rvx_buffer* a,
+                                  const rvx_buffer* b, float scale);
+/* n <= 2^24 rows; adapter_ids int32 [n], NULL = no adapters. y must not be x. */
+rvx_status rvx_adapter_linear_forward_device(const rvx_adapter_linear* l, const rvx_buffer* x, int64_t n,
+                                             const rvx_buffer* adapter_ids_i32, rvx_buffer* y);
+
 /* ------------------------------------------------------------------ */
 /* Vector index: VectorIndex (crates/ruvector-core/src/index.rs:11-36) */
 /*   FlatIndex (index/flat.rs) and HnswIndex (index/hnsw.rs)           */

@@ -22,6 +22,7 @@ from .attention import DualSpaceAttention, DualSpaceConfig, EdgeFeaturedAttentio
 from .hyperbolic import (DualSpaceIndex, HyperbolicError, HyperbolicHnsw, HyperbolicHnswConfig,  # noqa: E402
                          ShardedHyperbolicHnsw, ShardedHyperbolicSearch)
 
+from .adapters import AdapterError, AdapterLinear  # noqa: E402
 from .embedding import EmbeddingError, embedding_backward_device, embedding_forward_device  # noqa: E402
 from .logprobs import LogProbsError, log_probs_backward_device, log_probs_device  # noqa: E402
 from .query import NeuralSearch, QueryMode, RuvectorQuery  # noqa: E402
@@ -37,7 +38,7 @@ __all__ = [
     "DualSpaceIndex",
     "NeuralSearch", "QueryMode", "RuvectorQuery", "DbOptions", "SearchQuery", "VectorDB", "VectorEntry", "differentiable_search_device", "hnsw_last_search_stats", "scan_last_stats",
     "stream_wait", "stream_signal", "EmbeddingError", "embedding_forward_device", "embedding_backward_device",
-    "LogProbsError", "log_probs_device", "log_probs_backward_device",
+    "AdapterError", "AdapterLinear", "LogProbsError", "log_probs_device", "log_probs_backward_device",
     "pack_row_image", "row_image", "row_image_bytes",
 ]
 __version__ = "0.1.0"

@@ -57,6 +57,11 @@ class DualAttentionConfig(C.Structure):
                 ("hyperbolic_weight", C.c_float), ("temperature", C.c_float)]
 
 
+class AdapterLinearConfig(C.Structure):
+    _fields_ = [("in_features", C.c_int32), ("out_features", C.c_int32), ("dtype", C.c_int32),
+                ("max_rank", C.c_int32), ("max_adapters", C.c_int32)]
+
+
 class HyperbolicConfig(C.Structure):
     _fields_ = [("dim", C.c_int32), ("max_connections", C.c_int32), ("max_connections_0", C.c_int32),
                 ("ef_construction", C.c_int32), ("ef_search", C.c_int32), ("level_mult", C.c_float),
@@ -160,6 +165,10 @@ SIGNATURES = {
     "rvx_embedding_backward_device": (None, [P, I32, P, I64, I64, I32, F32, I32, I32, P]),
     "rvx_log_probs_device": (None, [P, I32, I64, I64, I64, F32, P, I32, P, P, P, P, P, P]),
     "rvx_log_probs_backward_device": (None, [P, I32, I64, I64, I64, F32, P, P, P, P, P, P, I64]),
+    "rvx_adapter_linear_create": (None, [C.POINTER(AdapterLinearConfig), P, P, PP]),
+    "rvx_adapter_linear_destroy": (None, [P]),
+    "rvx_adapter_linear_set": (None, [P, I32, I32, P, P, F32]),
+    "rvx_adapter_linear_forward_device": (None, [P, P, I64, P, P]),
     "rvx_index_create": (None, [C.POINTER(IndexConfig), PP]),
     "rvx_index_destroy": (None, [P]),
     "rvx_index_add_batch": (None, [P, PF32, PU64, I64]),

@@ -52,3 +52,17 @@ def test_dtype_names():
     for bad in ("f64", None, 2, []):
         with pytest.raises(rv.RvxError):
             dtype_code(bad)
+
+
+@pytest.mark.parametrize("inp,out,dtype,rank,slots,word", [
+    (0, 8, 0, 8, 1, "features"), (8, 0, 0, 8, 1, "features"), (65537, 8, 0, 8, 1, "features"), (8, 8, 3, 8, 1, "dtype"),
+    (8, 8, 0, 0, 1, "max_rank"), (8, 8, 0, 129, 1, "max_rank"), (8, 8, 0, 8, -1, "max_adapters"), (8, 8, 0, 8, 65537, "max_adapters"),
+    (8, 8, 0, 8, 1, "null weight")])
+def test_adapter_linear(inp, out, dtype, rank, slots, word):
+    import ctypes as C
+    cfg, h = L.AdapterLinearConfig(inp, out, dtype, rank, slots), C.c_void_p()
+    st, msg = _status("rvx_adapter_linear_create", C.byref(cfg), None, None, C.byref(h))
+    assert st in (2, 4) and word in msg and not h.value
+    assert _status("rvx_adapter_linear_set", None, 0, 4, None, None, 1.0)[0] == 2
+    assert _status("rvx_adapter_linear_forward_device", None, None, 1, None, None)[0] == 2
+    assert _status("rvx_adapter_linear_destroy", None)[0] == 0
