@@ -58,11 +58,10 @@ __global__ __launch_bounds__(256) void embed_forward_kernel(const T* __restrict_
 
 // ---------------------------------------------------------------- grouping positions by id
 // Stable LSD radix sort of (key, position), key = id, or `rows` for an absent id. The n positions
-// are cut into at most SORT_TILES tiles, one block each, so that a block can sum the digit counts
-// of the tiles before it by itself: a pass is one launch. The pass that moves an element also
-// counts its next digit for the tile it lands in (integer atomics: the counts do not depend on
-// their order).
-constexpr int SORT_TILES = 32, SORT_THREADS = 512, SORT_WAVES = SORT_THREADS / 64, SORT_STEP = SORT_THREADS * 4;
+// are cut into at most SORT_TILES tiles, one block each. A pass is two launches: every tile counts
+// its digits in LDS, then moves its elements; for that each block sums the counts of the tiles
+// before it by itself, which costs less than a launch for a scan.
+constexpr int SORT_TILES = 64, SORT_THREADS = 512, SORT_WAVES = SORT_THREADS / 64, SORT_STEP = SORT_THREADS * 4;
 constexpr int SORT_MAX_BITS = 11, SORT_BINS = 1 << SORT_MAX_BITS;
 
 __device__ __forceinline__ uint32_t sort_key(const int64_t* ids, int64_t i, uint32_t rows) {
@@ -70,18 +69,23 @@ __device__ __forceinline__ uint32_t sort_key(const int64_t* ids, int64_t i, uint
     return id >= 0 && id < (int64_t)rows ? (uint32_t)id : rows;
 }
 
-__global__ __launch_bounds__(256) void fill_words_kernel(uint32_t* p, int64_t words) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (int64_t)gridDim.x * 256) p[i] = 0;
-}
-
-// counts of digit 0 by tile, and a bit for each row that is looked up (present: nullable)
-__global__ __launch_bounds__(256) void sort_count_kernel(const int64_t* __restrict__ ids, int64_t n, uint32_t rows,
-                                                        int64_t tile, int bits, uint32_t* counts, uint32_t* present) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const uint32_t key = sort_key(ids, i, rows);
-        atomicAdd(&counts[(i / tile) << bits | (key & ((1u << bits) - 1))], 1u);
-        if (present && key < rows) atomicOr(&present[key >> 5], 1u << (key & 31));
+template <bool FIRST>
+__global__ __launch_bounds__(SORT_THREADS) void sort_count_kernel(const int64_t* __restrict__ ids,
+                                                                 const uint32_t* __restrict__ key_in, int64_t n,
+                                                                 uint32_t rows, int64_t tile, int bits, int shift,
+                                                                 uint32_t* __restrict__ counts) {
+    __shared__ uint32_t hist[SORT_BINS];
+    const int bins = 1 << bits;
+    for (int d = threadIdx.x; d < bins; d += SORT_THREADS) hist[d] = 0;
+    __syncthreads();
+    const int64_t lo = blockIdx.x * tile, hi = min(n, lo + tile);
+#pragma unroll 4
+    for (int64_t i = lo + threadIdx.x; i < hi; i += SORT_THREADS) {
+        const uint32_t key = FIRST ? sort_key(ids, i, rows) : key_in[i];
+        atomicAdd(&hist[(key >> shift) & (bins - 1)], 1u);
     }
+    __syncthreads();
+    for (int d = threadIdx.x; d < bins; d += SORT_THREADS) counts[((int64_t)blockIdx.x << bits) | d] = hist[d];
 }
 
 // FIRST: the elements are ids in their own order; else (key, pos) of the pass before.
@@ -92,7 +96,7 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_move_kernel(const int64_t* 
                                                                 uint32_t rows, int64_t tile, int tiles, int bits,
                                                                 int shift, const uint32_t* __restrict__ counts,
                                                                 uint32_t* __restrict__ key_out,
-                                                                uint32_t* __restrict__ pos_out, uint32_t* next_counts) {
+                                                                uint32_t* __restrict__ pos_out) {
     __shared__ uint32_t base[SORT_BINS];               // where this block's next element of a digit goes
     __shared__ uint32_t mine[SORT_WAVES][SORT_BINS];   // per wave: its count of a digit, then its next place
     __shared__ uint32_t sums[SORT_THREADS];
@@ -106,6 +110,7 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_move_kernel(const int64_t* 
         const int d = t * PER + j;
         total[j] = ahead[j] = 0;
         if (d < bins)
+#pragma unroll 8
             for (int b = 0; b < tiles; ++b) {
                 const uint32_t v = counts[(int64_t)b << bits | d];
                 total[j] += v;
@@ -130,7 +135,8 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_move_kernel(const int64_t* 
     const int64_t lo = me * tile, hi = min(n, lo + tile);
     for (int64_t at = lo; at < hi; at += SORT_STEP) {
         __syncthreads();
-        for (int i = t; i < SORT_WAVES * SORT_BINS; i += SORT_THREADS) (&mine[0][0])[i] = 0;
+        for (int d = t; d < bins; d += SORT_THREADS)
+            for (int w = 0; w < SORT_WAVES; ++w) mine[w][d] = 0;
         __syncthreads();
         // a wave has 4 x 64 elements in order
         uint32_t key[4], pos[4];
@@ -174,8 +180,6 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_move_kernel(const int64_t* 
             if (there) {
                 key_out[to] = key[u];
                 pos_out[to] = pos[u];
-                if (next_counts)
-                    atomicAdd(&next_counts[(int64_t)(to / tile) << bits | ((key[u] >> (shift + bits)) & (bins - 1))], 1u);
             }
         }
     }
@@ -193,21 +197,23 @@ struct Slab {  // a wave's columns of a row: N a lane
     static constexpr int N = Vec16<T>::N, COLS = 64 * N;
 };
 
-// acc += columns [col, col + N) of `count` (<= 64) rows; row j's start is rows_of(j), wave-uniform
+// acc += columns [col, col + N) of `count` (<= 64) rows; row j's start is row_of(j), wave-uniform
 template <class S, int N, class F>
 __device__ __forceinline__ void add_rows(float (&acc)[N], int count, int col, int dim, F&& row_of) {
-    constexpr int U = 8;
+    constexpr int U = 4;
     static_assert(N % Vec16<S>::N == 0, "a lane's columns are whole vectors");
     for (int j = 0; j < count; j += U) {
         S v[U][N];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const S* p = row_of(min(j + u, count - 1)) + col;
-            if (col + N <= dim) {
-                __builtin_memcpy(v[u], p, sizeof(S) * N);
-            } else {
+            if (j + u < count) {
+                const S* p = row_of(j + u) + col;
+                if (col + N <= dim) {
+                    __builtin_memcpy(v[u], p, sizeof(S) * N);
+                } else {
 #pragma unroll
-                for (int i = 0; i < N; ++i) v[u][i] = col + i < dim ? p[i] : (S)0.0f;
+                    for (int i = 0; i < N; ++i) v[u][i] = col + i < dim ? p[i] : (S)0.0f;
+                }
             }
         }
 #pragma unroll
@@ -247,19 +253,19 @@ __global__ __launch_bounds__(256) void embed_partial_kernel(const T* __restrict_
         if (col + i < dim) o[i] = acc[i];
 }
 
-template <class S, int N, bool ADD>
-__device__ __forceinline__ void put_row(S* o, const float (&acc)[N], int col, int dim, float scale) {
-    S v[N];
-    const bool whole = col + N <= dim;
-    if constexpr (ADD) {
-        if (whole) __builtin_memcpy(v, o, sizeof(v));
-        else
+// columns [col, col + N) of a row that is added to (read early: the load does not wait for the sum)
+template <class S, int N>
+__device__ __forceinline__ void get_row(const S* o, S (&v)[N], int col, int dim) {
+    if (col + N <= dim) __builtin_memcpy(v, o, sizeof(v));
+    else
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = col + i < dim ? o[i] : (S)0.0f;
-    }
+        for (int i = 0; i < N; ++i) v[i] = col + i < dim ? o[i] : (S)0.0f;
+}
+template <class S, int N, bool ADD>
+__device__ __forceinline__ void put_row(S* o, const float (&acc)[N], S (&v)[N], int col, int dim, float scale) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = (S)(ADD ? fmaf(acc[i], scale, (float)v[i]) : acc[i] * scale);
-    if (whole) __builtin_memcpy(o, v, sizeof(v));
+    if (col + N <= dim) __builtin_memcpy(o, v, sizeof(v));
     else
 #pragma unroll
         for (int i = 0; i < N; ++i)
@@ -277,10 +283,25 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const T* __restrict__ g
     const int lane = threadIdx.x & 63;
     const int64_t i0 = begin + (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (i0 >= n) return;
-    const uint32_t k = key[i0];
-    if (k >= rows || (i0 > 0 && key[i0 - 1] == k)) return;
+    // one load gives the entry before, this one and the 62 after it
+    const int64_t near_i = i0 + lane - 1;
+    const uint32_t near_key = near_i >= 0 && near_i < n ? key[near_i] : 0xffffffffu;  // no key is that large
+    const uint32_t near_pos = near_i >= 0 && near_i < n ? pos[near_i] : 0;
+    const uint32_t k = __builtin_amdgcn_readlane(near_key, 1);
+    if (k >= rows || (uint32_t)__builtin_amdgcn_readlane(near_key, 0) == k) return;
     const int col = blockIdx.y * Slab<T>::COLS + lane * N;
+    S* const row = grad_table + (int64_t)k * dim + col;
+    S old[N];
+    if constexpr (ADD)
+        if (col < dim) get_row<S, N>(row, old, col, dim);
     float acc[N] = {};
+    const int run = __ffsll(__ballot(lane > 0 && near_key != k) | 1ull << 63) - 2;  // entries of the id, if below 62
+    if (run < 62) {
+        add_rows<T>(acc, run, min(col, dim), dim,
+                    [&](int j) { return grad_out + (int64_t)(uint32_t)__builtin_amdgcn_readlane(near_pos, j + 1) * dim; });
+        if (col < dim) put_row<S, N, ADD>(row, acc, old, col, dim, scale);
+        return;
+    }
     int64_t at = i0;
     while (at < n) {
         if ((at & (GROUP * GROUP - 1)) == 0 && at + GROUP * GROUP <= n && key[at + GROUP * GROUP - 1] == k) {
@@ -315,7 +336,7 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const T* __restrict__ g
         }
         if (at < n && key[at] != k) break;
     }
-    if (col < dim) put_row<S, N, ADD>(grad_table + (int64_t)k * dim + col, acc, col, dim, scale);
+    if (col < dim) put_row<S, N, ADD>(row, acc, old, col, dim, scale);
 }
 
 // Few positions: no sort. The wave of position i looks for its id among the positions before it
@@ -349,7 +370,24 @@ __global__ __launch_bounds__(256) void embed_scan_kernel(const T* __restrict__ g
         add_rows<T>(acc, count, min(col, dim), dim,
                     [&](int r) { return grad_out + (int64_t)__builtin_amdgcn_readlane(mine, r) * dim; });
     }
-    if (col < dim) put_row<S, N, ADD>(grad_table + id * dim + col, acc, col, dim, scale);
+    if (col < dim) {
+        S* const row = grad_table + id * dim + col;
+        S old[N];
+        if constexpr (ADD) get_row<S, N>(row, old, col, dim);
+        put_row<S, N, ADD>(row, acc, old, col, dim, scale);
+    }
+}
+
+__global__ __launch_bounds__(256) void clear_bits_kernel(uint32_t* p, int64_t words) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (int64_t)gridDim.x * 256) p[i] = 0;
+}
+// a bit for each row that is looked up, from the first entry of each id in the sorted order
+__global__ __launch_bounds__(256) void mark_rows_kernel(const uint32_t* __restrict__ key, int64_t n, uint32_t rows,
+                                                       uint32_t* present) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const uint32_t k = key[i];
+        if (k < rows && (i == 0 || key[i - 1] != k)) atomicOr(&present[k >> 5], 1u << (k & 31));
+    }
 }
 
 // Rows without an id are zeros: present == null, every row; else the rows whose bit is not set.
@@ -423,44 +461,49 @@ void embedding_backward(int32_t dtype, const void* grad_out, const int64_t* ids,
     int64_t tile = (n + SORT_TILES - 1) / SORT_TILES;
     tile = (tile + SORT_STEP - 1) / SORT_STEP * SORT_STEP;
     const int tiles = (int)((n + tile - 1) / tile);
-    const int64_t count_words = (int64_t)SORT_TILES << bits, bit_words = accumulate ? 0 : (rows + 31) / 32;
-    const int64_t zero_words = count_words * passes + bit_words;
-    auto* counts = (uint32_t*)scratch_bytes("embed_counts", zero_words * 4);
-    auto* present = accumulate ? nullptr : counts + count_words * passes;
+    auto* counts = (uint32_t*)scratch_bytes("embed_counts", ((int64_t)SORT_TILES << bits) * 4);
     auto* sorted = (uint32_t*)scratch_bytes("embed_sorted", n * 16);  // key, pos and their other halves
     uint32_t *key[2] = {sorted, sorted + 2 * n}, *pos[2] = {sorted + n, sorted + 3 * n};
     const int64_t groups = n / GROUP, groups2 = groups / GROUP;
     float* first = scratch_f32("embed_partial", std::max<int64_t>(1, (groups + groups2) * dim));
     float* second = first + groups * dim;
-
-    RVX_LAUNCH("embedding_sort", fill_words_kernel,
-               dim3((unsigned)std::min<int64_t>((zero_words + 255) / 256, 4LL * device().num_cus)), dim3(256), 0, counts,
-               zero_words);
-    RVX_LAUNCH("embedding_sort", sort_count_kernel,
-               dim3((unsigned)std::min<int64_t>((n + 255) / 256, 4LL * device().num_cus)), dim3(256), 0, ids, n,
-               (uint32_t)rows, tile, bits, counts, present);
     for (int p = 0; p < passes; ++p) {
-        uint32_t* next = p + 1 < passes ? counts + (p + 1) * count_words : nullptr;
-        if (p == 0)
-            RVX_LAUNCH("embedding_sort", sort_move_kernel<true>, dim3(tiles), dim3(SORT_THREADS), 0, ids, nullptr, nullptr,
-                       n, (uint32_t)rows, tile, tiles, bits, 0, counts, key[0], pos[0], next);
-        else
-            RVX_LAUNCH("embedding_sort", sort_move_kernel<false>, dim3(tiles), dim3(SORT_THREADS), 0, nullptr,
-                       key[(p + 1) & 1], pos[(p + 1) & 1], n, (uint32_t)rows, tile, tiles, bits, p * bits,
-                       counts + p * count_words, key[p & 1], pos[p & 1], next);
+        const int in = (p + 1) & 1, out = p & 1, shift = p * bits;
+        if (p == 0) {
+            RVX_LAUNCH("embedding_sort", sort_count_kernel<true>, dim3(tiles), dim3(SORT_THREADS), 0, ids,
+                       (const uint32_t*)nullptr, n, (uint32_t)rows, tile, bits, shift, counts);
+            RVX_LAUNCH("embedding_sort", sort_move_kernel<true>, dim3(tiles), dim3(SORT_THREADS), 0, ids,
+                       (const uint32_t*)nullptr, (const uint32_t*)nullptr, n, (uint32_t)rows, tile, tiles, bits, shift,
+                       (const uint32_t*)counts, key[out], pos[out]);
+        } else {
+            RVX_LAUNCH("embedding_sort", sort_count_kernel<false>, dim3(tiles), dim3(SORT_THREADS), 0,
+                       (const int64_t*)nullptr, (const uint32_t*)key[in], n, (uint32_t)rows, tile, bits, shift, counts);
+            RVX_LAUNCH("embedding_sort", sort_move_kernel<false>, dim3(tiles), dim3(SORT_THREADS), 0,
+                       (const int64_t*)nullptr, (const uint32_t*)key[in], (const uint32_t*)pos[in], n, (uint32_t)rows, tile,
+                       tiles, bits, shift, (const uint32_t*)counts, key[out], pos[out]);
+        }
     }
     const uint32_t *sk = key[(passes + 1) & 1], *sp = pos[(passes + 1) & 1];
-    if (!accumulate) zero_rows(present);
+    if (!accumulate) {
+        const int64_t words = (rows + 31) / 32;
+        auto* present = (uint32_t*)scratch_bytes("embed_present", words * 4);
+        RVX_LAUNCH("embedding_zero", clear_bits_kernel,
+                   dim3((unsigned)std::min<int64_t>((words + 255) / 256, 4LL * device().num_cus)), dim3(256), 0, present, words);
+        RVX_LAUNCH("embedding_zero", mark_rows_kernel,
+                   dim3((unsigned)std::min<int64_t>((n + 255) / 256, 4LL * device().num_cus)), dim3(256), 0, sk, n,
+                   (uint32_t)rows, present);
+        zero_rows(present);
+    }
     typed([&](auto t, auto s, auto add) {
         using T = decltype(t);
         using S = decltype(s);
         const int slabs = (dim + Slab<T>::COLS - 1) / Slab<T>::COLS;
         auto blocks = [&](int64_t items) { return dim3((unsigned)((items + 3) / 4), slabs); };
         if (groups)
-            RVX_LAUNCH("embedding_backward", (embed_partial_kernel<T, false>), blocks(groups), dim3(256), 0,
+            RVX_LAUNCH("embedding_partial", (embed_partial_kernel<T, false>), blocks(groups), dim3(256), 0,
                        (const T*)grad_out, (const float*)nullptr, dim, sk, sp, groups, (uint32_t)rows, first);
         if (groups2)
-            RVX_LAUNCH("embedding_backward", (embed_partial_kernel<T, true>), blocks(groups2), dim3(256), 0,
+            RVX_LAUNCH("embedding_partial", (embed_partial_kernel<T, true>), blocks(groups2), dim3(256), 0,
                        (const T*)grad_out, (const float*)first, dim, sk, sp, groups2, (uint32_t)rows, second);
         constexpr int64_t SLICE = (int64_t)1 << 24;  // entries of one launch: at most 2^30 threads
         for (int64_t i = 0; i < n; i += SLICE)

@@ -12,7 +12,8 @@ namespace rvx {
 namespace {
 
 constexpr float LN2 = 0.69314718055994530942f, LOG2E = 1.44269504088896340736f;
-constexpr float FLOOR_U = -1e30f;  // e^u is 0 long before; keeps 0 * u finite for masked scores
+constexpr float FLOOR_U = -1e4f;   // 2^u is 0 long before; keeps 0 * u finite for masked scores
+constexpr float FAR_SCORE = 1e30f; // past it the one-fma form of u could overflow
 using u64 = unsigned long long;
 
 struct Stat {
@@ -28,6 +29,81 @@ __device__ __forceinline__ Stat join(const Stat& a, const Stat& b, float c1) {
     return o;
 }
 
+// ---------------------------------------------------------------- values of other lanes
+// x of lane (l ^ ST), without a trip through LDS: rows of 16 lanes are permuted by DPP, rows and
+// halves exchanged by the permlane swaps.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true);
+}
+template <int ST>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t x) {
+    const int lane = threadIdx.x & 63;
+    if constexpr (ST == 1) return dpp<0xB1>(x);             // quad_perm [1,0,3,2]
+    else if constexpr (ST == 2) return dpp<0x4E>(x);        // quad_perm [2,3,0,1]
+    else if constexpr (ST == 4) return dpp<0x1B>(dpp<0x141>(x));  // mirror of 8 lanes, then of 4: l ^ 7 ^ 3
+    else if constexpr (ST == 8) return dpp<0x128>(x);       // rotation of a row by 8
+    else if constexpr (ST == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+        return lane & 16 ? r[0] : r[1];
+    } else {
+        const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+        return lane & 32 ? r[0] : r[1];
+    }
+}
+template <int ST>
+__device__ __forceinline__ float lane_xor(float x) {
+    return __uint_as_float(lane_xor<ST>(__float_as_uint(x)));
+}
+template <int ST>
+__device__ __forceinline__ u64 lane_xor(u64 x) {
+    return (u64)lane_xor<ST>((uint32_t)(x >> 32)) << 32 | lane_xor<ST>((uint32_t)x);
+}
+// One exchange of a bitonic network: the smaller value goes to the lower lane where `up`.
+template <int ST, class K>
+__device__ __forceinline__ K exchange(K x, bool up) {
+    const K y = lane_xor<ST>(x);
+    const bool low = ((threadIdx.x & 63) & ST) == 0;
+    return (low == up) == (x < y) ? x : y;
+}
+template <int SIZE, int ST, class K>
+__device__ __forceinline__ K sort_stage(K x) {  // the stage of SIZE: strides ST, ST / 2 .. 1
+    x = exchange<ST>(x, ((threadIdx.x & 63) & SIZE) == 0);
+    if constexpr (ST > 1) x = sort_stage<SIZE, ST / 2>(x);
+    return x;
+}
+template <class K>
+__device__ __forceinline__ K sort_up(K x) {  // ascending over the 64 lanes
+    x = sort_stage<2, 1>(x);
+    x = sort_stage<4, 2>(x);
+    x = sort_stage<8, 4>(x);
+    x = sort_stage<16, 8>(x);
+    x = sort_stage<32, 16>(x);
+    return sort_stage<64, 32>(x);
+}
+template <int ST = 32>
+__device__ __forceinline__ u64 bitonic_down(u64 x) {  // a bitonic row to descending order
+    x = exchange<ST>(x, false);
+    if constexpr (ST > 1) x = bitonic_down<ST / 2>(x);
+    return x;
+}
+__device__ __forceinline__ Stat join_lanes(Stat st, float c1) {
+    auto step = [&](auto o) {
+        constexpr int ST = decltype(o)::value;
+        Stat b;
+        b.m = lane_xor<ST>(st.m), b.s = lane_xor<ST>(st.s), b.e = lane_xor<ST>(st.e);
+        st = join(st, b, c1);
+    };
+    step(std::integral_constant<int, 32>{});
+    step(std::integral_constant<int, 16>{});
+    step(std::integral_constant<int, 8>{});
+    step(std::integral_constant<int, 4>{});
+    step(std::integral_constant<int, 2>{});
+    step(std::integral_constant<int, 1>{});
+    return st;
+}
+
+// ---------------------------------------------------------------- the best scores
 // Scores in the order "higher first, then lower id first", as 64-bit keys (0 = none).
 __device__ __forceinline__ u64 key_of(float x, uint32_t id) {
     int b = __float_as_int(x + 0.0f);  // -0 and +0 are the same score
@@ -39,44 +115,43 @@ __device__ __forceinline__ float key_score(u64 k) {
     b ^= (b >> 31) & 0x7fffffff;
     return __int_as_float(b);
 }
+__device__ __forceinline__ u64 lane_value(u64 x, int lane) {  // lane: the same in all lanes
+    return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)x, lane);
+}
 
 // The 64 best keys a wave has seen, one a lane, best first. Keys above the k-th best wait in LDS;
-// 64 of them at a time are sorted (bitonic, ascending) and merged: max(best, new) of a descending and
-// an ascending row holds the 64 largest as a bitonic row.
+// 64 of them at a time are sorted (bitonic, ascending) and merged: max(best, new) of a descending
+// and an ascending row holds the 64 largest as a bitonic row.
 struct Best {
-    u64 list = 0, tau = 0;  // tau: the k-th best key
+    u64 list = 0, tau = 0;  // tau: no key up to it can be among the k best
     float tau_score = -INFINITY;
     int waiting = 0, k;
     u64* pend;  // this wave's waiting keys: room for 64 and for what is offered between two flushes
     __device__ Best(u64* p, int kk) : k(kk), pend(p) {}
 
-    __device__ void merge(u64 x) {
-        const int lane = threadIdx.x & 63;
-#pragma unroll
-        for (int size = 2; size <= 64; size <<= 1)
-#pragma unroll
-            for (int st = size >> 1; st > 0; st >>= 1) {
-                const u64 y = __shfl_xor(x, st);
-                const bool up = (lane & size) == 0, low = (lane & st) == 0;
-                x = (low == up) == (x < y) ? x : y;
-            }
-        u64 z = list > x ? list : x;
-#pragma unroll
-        for (int st = 32; st > 0; st >>= 1) {
-            const u64 y = __shfl_xor(z, st);
-            z = ((lane & st) == 0) == (z > y) ? z : y;
+    __device__ __forceinline__ void take(u64 ascending) {
+        list = bitonic_down(list > ascending ? list : ascending);
+        const u64 kth = lane_value(list, k - 1);
+        if (kth > tau) {
+            tau = kth;
+            tau_score = key_score(tau);
         }
-        list = z;
-        tau = __shfl(list, k - 1);
-        tau_score = tau ? key_score(tau) : -INFINITY;
     }
-    __device__ void flush() {  // the last 64 waiting keys
+    // At least k scores are known to be `bound` or above (-inf: nothing is known).
+    __device__ __forceinline__ void bound(float score) {
+        if (score > -INFINITY) {
+            tau = key_of(score, 0xffffffffu);
+            tau_score = score;
+        }
+    }
+    __device__ __forceinline__ void flush() {  // the last 64 waiting keys
         const int lane = threadIdx.x & 63;
         __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");
         const int from = max(0, waiting - 64);
         const u64 x = from + lane < waiting ? pend[from + lane] : 0;
         waiting = from;
-        if (__any(x > tau)) merge(x);
+        if (__any(x > tau)) take(sort_up(x));
     }
     __device__ __forceinline__ void offer(u64 key, bool there) {
         const bool in = there && key > tau;
@@ -88,7 +163,7 @@ struct Best {
     }
 };
 
-struct Part {  // what one wave found of one row
+struct Part {  // what one block found of one row
     float m, s, e;
     int before;
 };
@@ -116,71 +191,112 @@ __device__ __forceinline__ void write_top(u64 list, int k, int64_t row, const St
         out.top_logp[row * k + lane] = none ? -INFINITY : (key_score(list) - st.m) * inv_t - logf(st.s);
 }
 
+// ---------------------------------------------------------------- one pass
 constexpr int LP_U = 2, LP_WAVES = 4;  // 16-byte loads per lane and step; waves per block
 
-// One wave: elements [seg * seg_len, ..) of one row. parts == null: the wave has the whole row.
-template <class T, bool ENT, bool RANK, bool TOP>
-__global__ __launch_bounds__(64 * LP_WAVES) void logprobs_kernel(const T* __restrict__ scores, int64_t n, int64_t c,
-                                                                int64_t ld, float c1, float inv_t,
-                                                                const int64_t* __restrict__ targets, int k,
-                                                                int splits, int64_t seg_len, Part* parts, u64* keys,
-                                                                LogProbsOut out) {
-    constexpr int N = Vec16<T>::N, STEP = 64 * N * LP_U;
-    constexpr int ROOM = 64 + 64 * N;
-    __shared__ u64 pend[TOP ? LP_WAVES * ROOM : 1];
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t w = (int64_t)blockIdx.x * LP_WAVES + wave;
-    if (w >= n * splits) return;
-    const int64_t row = w / splits;
-    const int64_t lo = (w - row * splits) * seg_len, hi = min(c, lo + seg_len);
-    const T* x = scores + row * ld;
-    int64_t target = targets ? targets[row] : -1;
-    const bool has_target = target >= 0 && target < c;
-    const float st_score = has_target ? (float)x[target] : NAN;
-    if (!has_target) target = -1;
-
-    Stat st;
-    int before = 0;
-    Best best(TOP ? pend + wave * ROOM : nullptr, k);
-    for (int64_t at = lo; at < hi; at += STEP) {
-        float v[LP_U][N];
-        const bool whole = at + STEP <= hi;
+template <class T>
+struct Step {  // a wave's elements of one step, lane by lane 16 bytes
+    static constexpr int N = Vec16<T>::N, SIZE = 64 * N * LP_U;
+    Vec16<T> v[LP_U];
+    __device__ __forceinline__ void load(const T* x, int64_t at, int64_t hi) {  // past hi: masked
+        const int lane = threadIdx.x & 63;
+        if (at + SIZE <= hi) {
 #pragma unroll
-        for (int u = 0; u < LP_U; ++u) {
-            const int64_t p = at + (u * 64 + lane) * N;
-            if (whole || p + N <= hi) {
-                const Vec16<T> r = load16(x + p);
+            for (int u = 0; u < LP_U; ++u) v[u] = load16(x + at + (u * 64 + lane) * N);
+        } else {
 #pragma unroll
-                for (int j = 0; j < N; ++j) v[u][j] = (float)r.v[j];
-            } else {
+            for (int u = 0; u < LP_U; ++u) {
+                const int64_t p = at + (u * 64 + lane) * N;
+                if (p + N <= hi) v[u] = load16(x + p);
+                else
 #pragma unroll
-                for (int j = 0; j < N; ++j) v[u][j] = p + j < hi ? (float)x[p + j] : -INFINITY;
+                    for (int j = 0; j < N; ++j) v[u].v[j] = p + j < hi ? x[p + j] : (T)-INFINITY;
             }
         }
+    }
+};
+
+// S and E by subtraction of the running maximum itself: right for scores of any size. Only for
+// rows whose largest score is past FAR_SCORE, and for temperatures outside [1e-6, 1e6].
+template <class T>
+__device__ __attribute__((noinline)) Stat far_stats(const T* x, int64_t lo, int64_t hi, float c1) {
+    constexpr int N = Step<T>::N;
+    Stat st;
+    for (int64_t at = lo; at < hi; at += Step<T>::SIZE) {
+        Step<T> cur;
+        cur.load(x, at, hi);
+#pragma unroll
+        for (int u = 0; u < LP_U; ++u)
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const float v = (float)cur.v[u].v[j], mn = fmaxf(st.m, v);
+                const float d = fmaxf((st.m - mn) * c1, FLOOR_U), r = __builtin_amdgcn_exp2f(d);
+                const float y = (v - mn) * c1, ex = __builtin_amdgcn_exp2f(y);
+                st.e = fmaf(r, fmaf(st.s, d, st.e), ex * fmaxf(y, FLOOR_U));
+                st.s = fmaf(st.s, r, ex);
+                st.m = mn;
+            }
+    }
+    return st;
+}
+
+// A wave goes over elements [lo, hi) of a row. Bound by reading them: per score one unpack, half a
+// max, one fma, one exp (4 cycles), two additions and one comparison.
+template <class T, bool ENT, bool RANK, bool TOP>
+__device__ __forceinline__ Stat walk(const T* __restrict__ x, int64_t lo, int64_t hi, float c1, bool near, int64_t target,
+                                     float st_score, int& before, Best& best) {
+    constexpr int N = Step<T>::N, SIZE = Step<T>::SIZE;
+    const int lane = threadIdx.x & 63;
+    // 2^u is taken against b = fl(m c1), the lane's largest score in log2 units: u = fma(x, c1, -b) is
+    // rounded once, and what b is off from m c1 is put right at the end.
+    float m = -INFINITY, b = -FAR_SCORE * c1, s = 0.f, e = 0.f;
+    Step<T> nxt;
+    if (lo < hi) nxt.load(x, lo, hi);
+    for (int64_t at = lo; at < hi; at += SIZE) {
+        float v[LP_U][N];
+#pragma unroll
+        for (int u = 0; u < LP_U; ++u)
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[u][j] = (float)nxt.v[u].v[j];
+        if (at + SIZE < hi) nxt.load(x, at + SIZE, hi);  // on its way while this step is worked on
         float cm = -INFINITY;
 #pragma unroll
         for (int u = 0; u < LP_U; ++u)
 #pragma unroll
             for (int j = 0; j < N; ++j) cm = fmaxf(cm, v[u][j]);
-        {
-            const float mn = fmaxf(st.m, cm);
-            const float d = fmaxf((st.m - mn) * c1, FLOOR_U), r = __builtin_amdgcn_exp2f(d);
-            float s = 0.f, e = 0.f;
-#pragma unroll
-            for (int u = 0; u < LP_U; ++u)
-#pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    const float y = (v[u][j] - mn) * c1, ex = __builtin_amdgcn_exp2f(y);
-                    s += ex;
-                    if constexpr (ENT) e = fmaf(ex, fmaxf(y, FLOOR_U), e);
-                }
-            if constexpr (ENT) st.e = fmaf(r, fmaf(st.s, d, st.e), e);
-            st.s = fmaf(st.s, r, s);
-            st.m = mn;
+        if (__any(cm > m)) {
+            m = fmaxf(m, cm);
+            const float bn = fminf(fmaxf(m, -FAR_SCORE), FAR_SCORE) * c1;
+            const float d = fmaxf(b - bn, FLOOR_U), r = __builtin_amdgcn_exp2f(d);
+            if constexpr (ENT) e = r * fmaf(s, d, e);
+            s *= r;
+            b = bn;
         }
+        float ds = 0.f, de = 0.f;
+#pragma unroll
+        for (int u = 0; u < LP_U; ++u)
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const float y = fmaf(v[u][j], c1, -b), ex = __builtin_amdgcn_exp2f(y);
+                ds += ex;
+                if constexpr (ENT) de = fmaf(ex, y, de);
+            }
+        if constexpr (ENT) {
+            if (__any(de != de)) {  // a masked score (0 * -inf) or a NaN
+                de = 0.f;
+#pragma unroll
+                for (int u = 0; u < LP_U; ++u)
+#pragma unroll
+                    for (int j = 0; j < N; ++j) {
+                        const float y = fmaf(v[u][j], c1, -b);
+                        de = fmaf(__builtin_amdgcn_exp2f(y), fmaxf(y, FLOOR_U), de);
+                    }
+            }
+            e += de;
+        }
+        s += ds;
         if constexpr (RANK) {
-            if (at + STEP <= target) {
+            if (at + SIZE <= target) {
 #pragma unroll
                 for (int u = 0; u < LP_U; ++u)
 #pragma unroll
@@ -191,16 +307,19 @@ __global__ __launch_bounds__(64 * LP_WAVES) void logprobs_kernel(const T* __rest
 #pragma unroll
                     for (int j = 0; j < N; ++j) before += __popcll(__ballot(v[u][j] > st_score));
             } else {
+                const int t = (int)(target - at);
 #pragma unroll
                 for (int u = 0; u < LP_U; ++u)
 #pragma unroll
                     for (int j = 0; j < N; ++j)
-                        before += __popcll(__ballot(
-                            v[u][j] > st_score || (v[u][j] == st_score && at + (u * 64 + lane) * N + j < target)));
+                        before += __popcll(__ballot(v[u][j] > st_score ||
+                                                    (v[u][j] == st_score && (u * 64 + lane) * N + j < t)));
             }
         }
         if constexpr (TOP) {
-            if (__any(cm > best.tau_score)) {
+            // the k-th best of the lanes' largest scores of the first step bounds the k-th best score
+            if (at == lo) best.bound(__uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(sort_up(cm)), 64 - best.k)));
+            if (at == lo || __any(cm > best.tau_score)) {
 #pragma unroll
                 for (int u = 0; u < LP_U; ++u) {
 #pragma unroll
@@ -211,36 +330,111 @@ __global__ __launch_bounds__(64 * LP_WAVES) void logprobs_kernel(const T* __rest
             }
         }
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        Stat b;
-        b.m = __shfl_xor(st.m, o), b.s = __shfl_xor(st.s, o), b.e = __shfl_xor(st.e, o);
-        st = join(st, b, c1);
-    }
     if constexpr (TOP)
         if (best.waiting) best.flush();
+    Stat st;
+    if (s != 0.f) {  // to the reference m itself
+        const float d = fmaf(-m, c1, b), r = __builtin_amdgcn_exp2f(d);
+        st.m = m;
+        st.e = r * fmaf(s, d, e);
+        st.s = s * r;
+    }
+    const bool far = fabsf(m) > FAR_SCORE && m != -INFINITY;
+    if (!near || __any(far)) {
+        // lanes past FAR_SCORE count only where the row's largest score is there too
+        float mw = m;
+        mw = fmaxf(mw, lane_xor<32>(mw)), mw = fmaxf(mw, lane_xor<16>(mw)), mw = fmaxf(mw, lane_xor<8>(mw));
+        mw = fmaxf(mw, lane_xor<4>(mw)), mw = fmaxf(mw, lane_xor<2>(mw)), mw = fmaxf(mw, lane_xor<1>(mw));
+        if (!near || (fabsf(mw) > FAR_SCORE && mw != -INFINITY)) st = far_stats(x, lo, hi, c1);
+    }
+    return join_lanes(st, c1);
+}
+
+struct Row {  // a row's target
+    int64_t target;
+    bool there;
+    float score;
+    template <class T>
+    __device__ __forceinline__ Row(const T* x, const int64_t* targets, int64_t row, int64_t c) {
+        target = targets ? targets[row] : -1;
+        there = target >= 0 && target < c;
+        if (!there) target = -1;
+        score = there ? (float)x[target] : NAN;
+    }
+};
+
+// A wave a row (many rows).
+template <class T, bool ENT, bool RANK, bool TOP>
+__global__ __launch_bounds__(64 * LP_WAVES) void logprobs_wave_kernel(const T* __restrict__ scores, int64_t n, int64_t c,
+                                                                     int64_t ld, float c1, float inv_t, bool near,
+                                                                     const int64_t* __restrict__ targets, int k,
+                                                                     LogProbsOut out) {
+    constexpr int ROOM = 64 + 64 * Vec16<T>::N;
+    __shared__ u64 pend[TOP ? LP_WAVES * ROOM : 1];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t row = (int64_t)blockIdx.x * LP_WAVES + wave;
+    if (row >= n) return;
+    const T* x = scores + row * ld;
+    const Row r(x, targets, row, c);
+    int before = 0;
+    Best best(TOP ? pend + wave * ROOM : nullptr, k);
+    const Stat st = walk<T, ENT, RANK, TOP>(x, 0, c, c1, near, r.target, r.score, before, best);
+    if ((threadIdx.x & 63) == 0) write_row(st, before, row, r.score, r.there, inv_t, out);
+    if constexpr (TOP) write_top(best.list, k, row, st, inv_t, out);
+}
+
+// A block a row, or one of `splits` parts of a row: its waves take a quarter each and join in LDS.
+// parts == null: the block has the whole row.
+template <class T, bool ENT, bool RANK, bool TOP>
+__global__ __launch_bounds__(64 * LP_WAVES) void logprobs_block_kernel(const T* __restrict__ scores, int64_t c, int64_t ld,
+                                                                      float c1, float inv_t, bool near,
+                                                                      const int64_t* __restrict__ targets, int k,
+                                                                      int splits, int64_t seg_len, Part* parts, u64* keys,
+                                                                      LogProbsOut out) {
+    constexpr int ROOM = 64 + 64 * Vec16<T>::N;
+    __shared__ u64 pend[TOP ? LP_WAVES * ROOM : 1];
+    __shared__ Part found[LP_WAVES];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t row = blockIdx.x / splits;
+    const int64_t lo = min(c, ((int64_t)(blockIdx.x - row * splits) * LP_WAVES + wave) * seg_len), hi = min(c, lo + seg_len);
+    const T* x = scores + row * ld;
+    const Row r(x, targets, row, c);
+    int before = 0;
+    Best best(TOP ? pend + wave * ROOM : nullptr, k);
+    Stat st = walk<T, ENT, RANK, TOP>(x, lo, hi, c1, near, r.target, r.score, before, best);
+    if (lane == 0) found[wave] = Part{st.m, st.s, st.e, before};
+    if constexpr (TOP) pend[wave * ROOM + lane] = best.list;
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int w = 1; w < LP_WAVES; ++w) {
+        Stat b;
+        b.m = found[w].m, b.s = found[w].s, b.e = found[w].e;
+        st = join(st, b, c1);
+        before += found[w].before;
+        if constexpr (TOP) best.take(pend[w * ROOM + 63 - lane]);
+    }
     if (!parts) {
-        if (lane == 0) write_row(st, before, row, st_score, has_target, inv_t, out);
+        if (lane == 0) write_row(st, before, row, r.score, r.there, inv_t, out);
         if constexpr (TOP) write_top(best.list, k, row, st, inv_t, out);
     } else {
-        if (lane == 0) parts[w] = Part{st.m, st.s, st.e, before};
+        if (lane == 0) parts[blockIdx.x] = Part{st.m, st.s, st.e, before};
         if constexpr (TOP)
-            if (lane < k) keys[w * k + lane] = best.list;
+            if (lane < k) keys[(int64_t)blockIdx.x * k + lane] = best.list;
     }
 }
 
-// One wave a row: joins the parts of its splits in their order.
+// One wave a row: joins the parts of its blocks in their order.
 template <class T>
 __global__ __launch_bounds__(64) void logprobs_join_kernel(const T* __restrict__ scores, int64_t c, int64_t ld, float c1,
                                                            float inv_t, const int64_t* __restrict__ targets, int k,
                                                            int splits, const Part* __restrict__ parts,
                                                            const u64* __restrict__ keys, LogProbsOut out) {
-    __shared__ u64 pend[128];
+    __shared__ u64 pend[64 + 8 * 64];
     const int lane = threadIdx.x;
     const int64_t row = blockIdx.x;
-    int64_t target = targets ? targets[row] : -1;
-    const bool has_target = target >= 0 && target < c;
-    const float st_score = has_target ? (float)scores[row * ld + target] : NAN;
+    const Row r(scores + row * ld, targets, row, c);
     Stat st;
     int before = 0;
     for (int i = lane; i < splits; i += 64) {
@@ -250,19 +444,24 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(const T* __restrict__
         st = join(st, b, c1);
         before += p.before;
     }
+    st = join_lanes(st, c1);
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        Stat b;
-        b.m = __shfl_xor(st.m, o), b.s = __shfl_xor(st.s, o), b.e = __shfl_xor(st.e, o);
-        st = join(st, b, c1);
-        before += __shfl_xor(before, o);
-    }
-    if (lane == 0) write_row(st, before, row, st_score, has_target, inv_t, out);
+    for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o);
+    if (lane == 0) write_row(st, before, row, r.score, r.there, inv_t, out);
     if (k) {
         Best best(pend, k);
-        for (int i = 0; i < splits * k; i += 64) {
-            const u64 key = i + lane < splits * k ? keys[row * splits * k + i + lane] : 0;
-            best.offer(key, key != 0);
+        const u64* list = keys + row * splits * k;
+        const int total = splits * k;
+        // the k-th best of the first 64 parts' best keys bounds the k-th best score
+        const u64 first = lane < splits ? list[lane * k] : 0;
+        const u64 kth = lane_value(sort_up(first), 64 - k);
+        if (kth) best.bound(key_score(kth));
+        for (int i = 0; i < total; i += 8 * 64) {
+            u64 x[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) x[u] = i + u * 64 + lane < total ? list[i + u * 64 + lane] : 0;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) best.offer(x[u], x[u] != 0);
             while (best.waiting >= 64) best.flush();
         }
         if (best.waiting) best.flush();
@@ -270,47 +469,61 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(const T* __restrict__
     }
 }
 
-constexpr int LB_U = 2;  // 16-byte loads per lane
-
-template <class T, bool ENT>
+// ---------------------------------------------------------------- gradient
+// A wave: U * 64 * N neighbouring elements of one row. All loads go out before the first use.
+template <class T, bool ENT, int U>
 __global__ __launch_bounds__(256) void logprobs_backward_kernel(
-    const T* scores, int64_t c, int64_t ld, float c1, float inv_t, const int64_t* __restrict__ targets,
+    const T* scores, int64_t n, int64_t c, int64_t ld, float c1, float inv_t, const int64_t* __restrict__ targets,
     const float* __restrict__ stats, const float* __restrict__ grad_logp, const float* __restrict__ entropy,
-    const float* __restrict__ grad_entropy, T* grad, int64_t ld_grad, int blocks_per_row) {
+    const float* __restrict__ grad_entropy, T* grad, int64_t ld_grad, uint32_t per_row) {
     constexpr int N = Vec16<T>::N;
-    const int64_t row = blockIdx.x / blocks_per_row;
-    const int64_t at = (int64_t)(blockIdx.x - row * blocks_per_row) * (256 * N * LB_U);
-    int64_t target = targets ? targets[row] : -1;
-    const bool has_target = target >= 0 && target < c;
-    const float m = stats[2 * row], log_sum = stats[2 * row + 1], log_sum2 = log_sum * LOG2E;
-    const bool empty = log_sum == -INFINITY;
-    const float gl = has_target && grad_logp && !empty ? grad_logp[row] * inv_t : 0.0f;
-    const float gh = ENT ? grad_entropy[row] * inv_t : 0.0f, h = ENT ? entropy[row] : 0.0f;
-    if (!has_target) target = -1;
+    const int lane = threadIdx.x & 63;
+    const uint32_t w = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t row = w / per_row;
+    if (row >= n) return;
+    const int64_t at = (int64_t)(w - row * per_row) * (64 * N * U);
+    const T* x = scores + row * ld;
+    T* g = grad + row * ld_grad;
+    Vec16<T> v[U];
 #pragma unroll
-    for (int u = 0; u < LB_U; ++u) {
-        const int64_t p = at + (u * 256 + threadIdx.x) * N;
-        if (p >= c) return;
-        const T* x = scores + row * ld + p;
-        T* g = grad + row * ld_grad + p;
-        const bool whole = p + N <= c;
-        Vec16<T> v;
-        if (whole) v = load16(x);
+    for (int u = 0; u < U; ++u) {
+        const int64_t p = at + (u * 64 + lane) * N;
+        if (p + N <= c) v[u] = load16(x + p);
         else
-            for (int j = 0; j < N; ++j) v.v[j] = p + j < c ? x[j] : (T)0.0f;
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[u].v[j] = p + j < c ? x[p + j] : (T)0.0f;
+    }
+    int64_t target = targets ? targets[row] : -1;
+    if (target >= c) target = -1;
+    float m = stats[2 * (int64_t)row], log_sum2 = stats[2 * (int64_t)row + 1] * LOG2E;
+    const bool empty = log_sum2 == -INFINITY;
+    const float gl = target >= 0 && grad_logp && !empty ? grad_logp[row] * inv_t : 0.0f;
+    const float gh = ENT && !empty ? grad_entropy[row] * inv_t : 0.0f, h = ENT ? entropy[row] : 0.0f;
+    if (empty) m = 0.0f, log_sum2 = INFINITY;  // p = 0 everywhere
+    const bool has = target >= at && target < at + 64 * N * U;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int64_t p = at + (u * 64 + lane) * N;
+        float d[N];
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            const float lp = fmaf((float)v.v[j] - m, c1, -log_sum2), pr = __builtin_amdgcn_exp2f(lp);
-            float d = -gl * pr;
-            if constexpr (ENT) d = fmaf(-gh * pr, fmaf(fmaxf(lp, FLOOR_U), LN2, h), d);
-            if (empty) d = 0.0f;
-            if (p + j == target) d += gl;
-            v.v[j] = (T)d;
+            const float lp = fmaf((float)v[u].v[j] - m, c1, -log_sum2), pr = __builtin_amdgcn_exp2f(lp);
+            if constexpr (ENT) d[j] = pr * fmaf(-gh, fmaf(fmaxf(lp, FLOOR_U), LN2, h), -gl);
+            else d[j] = pr * -gl;
         }
-        if (whole) store16(g, v);
+        if (has) {
+            const int t = (int)(target - at) - (u * 64 + lane) * N;
+#pragma unroll
+            for (int j = 0; j < N; ++j) d[j] += j == t ? gl : 0.0f;
+        }
+        Vec16<T> o;
+#pragma unroll
+        for (int j = 0; j < N; ++j) o.v[j] = (T)d[j];
+        if (p + N <= c) store16(g + p, o);
         else
+#pragma unroll
             for (int j = 0; j < N; ++j)
-                if (p + j < c) g[j] = v.v[j];
+                if (p + j < c) g[p + j] = o.v[j];
     }
 }
 
@@ -319,49 +532,56 @@ __global__ __launch_bounds__(256) void logprobs_backward_kernel(
 void log_probs(int32_t dtype, const void* scores, int64_t n, int64_t c, int64_t ld, float temperature,
                const int64_t* targets, int k, const LogProbsOut& out) {
     const float inv_t = (float)(1.0 / (double)temperature), c1 = (float)(1.44269504088896340736 / (double)temperature);
+    const bool near = temperature >= 1e-6f && temperature <= 1e6f;
     with_dtype(dtype, [&](auto zero) {
         using T = decltype(zero);
-        constexpr int64_t STEP = 64 * Vec16<T>::N * LP_U;
-        // A row goes to one wave unless that leaves CUs without work: 16 waves a CU hide the loads.
-        const int64_t want = (16LL * device().num_cus + n - 1) / n, most = (c + STEP - 1) / STEP;
-        int64_t splits = std::max<int64_t>(1, std::min(want, most));
-        const int64_t seg = ((most + splits - 1) / splits) * STEP;
-        splits = (c + seg - 1) / seg;
+        constexpr int64_t STEP = Step<T>::SIZE;
+        // A row goes to one wave where that gives every CU 16 waves, else to a block, else to as many
+        // blocks as give every CU 4: the loads of fewer waves do not hide each other.
+        const int cus = device().num_cus;
+        const int64_t steps = (c + STEP - 1) / STEP;
+        const bool by_wave = n >= 16LL * cus || steps == 1;
+        int64_t splits = std::max<int64_t>(1, std::min<int64_t>((4LL * cus + n - 1) / n, (steps + LP_WAVES - 1) / LP_WAVES));
+        const int64_t seg = (steps + splits * LP_WAVES - 1) / (splits * LP_WAVES) * STEP;
+        splits = by_wave ? 1 : (c + seg * LP_WAVES - 1) / (seg * LP_WAVES);
         Part* parts = nullptr;
         u64* keys = nullptr;
         if (splits > 1) {
             parts = (Part*)scratch_bytes("lp_parts", n * splits * (int64_t)sizeof(Part));
             keys = (u64*)scratch_bytes("lp_keys", std::max<int64_t>(1, n * splits * k) * 8);
         }
-        const bool ent = out.entropy != nullptr, rank = out.rank != nullptr, top = k > 0;
-        const int64_t slice = ((int64_t)1 << 25) / splits;  // rows of one launch: at most 2^31 threads
+        const int64_t slice = ((int64_t)1 << 23) / splits;  // rows of one launch: at most 2^31 threads
         for (int64_t r = 0; r < n; r += slice) {
-        const int64_t rows = std::min(slice, n - r);
-        const T* x = (const T*)scores + r * ld;
-        const int64_t* t = targets ? targets + r : nullptr;
-        LogProbsOut o = out;
-        if (o.logp) o.logp += r;
-        if (o.rank) o.rank += r;
-        if (o.entropy) o.entropy += r;
-        if (o.stats) o.stats += 2 * r;
-        if (o.top_ids) o.top_ids += r * k;
-        if (o.top_logp) o.top_logp += r * k;
-        const dim3 grid((unsigned)((rows * splits + LP_WAVES - 1) / LP_WAVES));
-        auto go = [&](auto kernel) {
-            RVX_LAUNCH("log_probs", kernel, grid, dim3(64 * LP_WAVES), 0, x, rows, c, ld, c1, inv_t, t, k, (int)splits,
-                       seg, parts, keys, o);
-        };
-        if (ent && rank && top) go(logprobs_kernel<T, true, true, true>);
-        else if (ent && rank) go(logprobs_kernel<T, true, true, false>);
-        else if (ent && top) go(logprobs_kernel<T, true, false, true>);
-        else if (ent) go(logprobs_kernel<T, true, false, false>);
-        else if (rank && top) go(logprobs_kernel<T, false, true, true>);
-        else if (rank) go(logprobs_kernel<T, false, true, false>);
-        else if (top) go(logprobs_kernel<T, false, false, true>);
-        else go(logprobs_kernel<T, false, false, false>);
-        if (splits > 1)
-            RVX_LAUNCH("log_probs_join", logprobs_join_kernel<T>, dim3((unsigned)rows), dim3(64), 0, x, c, ld, c1, inv_t, t,
-                       k, (int)splits, (const Part*)parts, (const u64*)keys, o);
+            const int64_t rows = std::min(slice, n - r);
+            const T* x = (const T*)scores + r * ld;
+            const int64_t* t = targets ? targets + r : nullptr;
+            LogProbsOut o = out;
+            if (o.logp) o.logp += r;
+            if (o.rank) o.rank += r;
+            if (o.entropy) o.entropy += r;
+            if (o.stats) o.stats += 2 * r;
+            if (o.top_ids) o.top_ids += r * k;
+            if (o.top_logp) o.top_logp += r * k;
+            auto go = [&](auto ent, auto rank, auto top) {
+                constexpr bool E = decltype(ent)::value, R = decltype(rank)::value, K = decltype(top)::value;
+                if (by_wave)
+                    RVX_LAUNCH("log_probs", (logprobs_wave_kernel<T, E, R, K>),
+                               dim3((unsigned)((rows + LP_WAVES - 1) / LP_WAVES)), dim3(64 * LP_WAVES), 0, x, rows, c, ld, c1,
+                               inv_t, near, t, k, o);
+                else
+                    RVX_LAUNCH("log_probs", (logprobs_block_kernel<T, E, R, K>), dim3((unsigned)(rows * splits)),
+                               dim3(64 * LP_WAVES), 0, x, c, ld, c1, inv_t, near, t, k, (int)splits, seg, parts, keys, o);
+            };
+            auto flag = [](bool on, auto&& f) {
+                if (on) f(std::true_type{});
+                else f(std::false_type{});
+            };
+            flag(out.entropy != nullptr, [&](auto e) {
+                flag(out.rank != nullptr, [&](auto q) { flag(k > 0, [&](auto p) { go(e, q, p); }); });
+            });
+            if (splits > 1)
+                RVX_LAUNCH("log_probs_join", logprobs_join_kernel<T>, dim3((unsigned)rows), dim3(64), 0, x, c, ld, c1, inv_t, t,
+                           k, (int)splits, (const Part*)parts, (const u64*)keys, o);
         }
     });
 }
@@ -372,21 +592,26 @@ void log_probs_backward(int32_t dtype, const void* scores, int64_t n, int64_t c,
     const float inv_t = (float)(1.0 / (double)temperature), c1 = (float)(1.44269504088896340736 / (double)temperature);
     with_dtype(dtype, [&](auto zero) {
         using T = decltype(zero);
-        constexpr int64_t BLOCK = 256 * Vec16<T>::N * LB_U;
-        const int64_t per_row = (c + BLOCK - 1) / BLOCK;
-        // rows go in slices of at most 2^31 threads
-        const int64_t slice = std::max<int64_t>(1, ((int64_t)1 << 23) / per_row);
-        for (int64_t r = 0; r < n; r += slice) {
-            const dim3 grid((unsigned)(std::min(slice, n - r) * per_row));
-            auto go = [&](auto kernel) {
-                RVX_LAUNCH("log_probs_backward", kernel, grid, dim3(256), 0, (const T*)scores + r * ld, c, ld, c1, inv_t,
-                           targets ? targets + r : nullptr, stats + 2 * r, grad_logp ? grad_logp + r : nullptr,
+        auto go = [&](auto unroll, auto ent) {
+            constexpr int U = decltype(unroll)::value;
+            constexpr int64_t CHUNK = 64 * Vec16<T>::N * U;
+            const int64_t per_row = (c + CHUNK - 1) / CHUNK;
+            const int64_t slice = std::max<int64_t>(1, ((int64_t)1 << 25) / per_row);  // at most 2^31 threads
+            for (int64_t r = 0; r < n; r += slice) {
+                const int64_t rows = std::min(slice, n - r);
+                RVX_LAUNCH("log_probs_backward", (logprobs_backward_kernel<T, decltype(ent)::value, U>),
+                           dim3((unsigned)((rows * per_row + 3) / 4)), dim3(256), 0, (const T*)scores + r * ld, rows, c, ld, c1,
+                           inv_t, targets ? targets + r : nullptr, stats + 2 * r, grad_logp ? grad_logp + r : nullptr,
                            entropy ? entropy + r : nullptr, grad_entropy ? grad_entropy + r : nullptr,
-                           (T*)grad + r * ld_grad, ld_grad, (int)per_row);
-            };
-            if (grad_entropy) go(logprobs_backward_kernel<T, true>);
-            else go(logprobs_backward_kernel<T, false>);
-        }
+                           (T*)grad + r * ld_grad, ld_grad, (uint32_t)per_row);
+            }
+        };
+        auto by_width = [&](auto ent) {
+            if (c > 64 * Vec16<T>::N * 2) go(std::integral_constant<int, 4>{}, ent);
+            else go(std::integral_constant<int, 1>{}, ent);
+        };
+        if (grad_entropy) by_width(std::true_type{});
+        else by_width(std::false_type{});
     });
 }
 
