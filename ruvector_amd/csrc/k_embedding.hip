@@ -186,100 +186,126 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_move_kernel(const int64_t* 
 }
 
 // ---------------------------------------------------------------- sums over groups
-// A long group is summed in two steps: GROUP neighbouring entries of the sorted order that share
-// one id are first summed to a partial row (level 1), GROUP such partial rows to another (level
-// 2), each by a wave of its own; the row's wave then adds partial rows. What is a group depends
-// on the sorted ids alone, and so does the order of the additions.
-constexpr int GROUP = 64;
+// An id's entries are a run of the sorted order. A run of fewer than LONG entries is summed by one
+// wave per slab of columns, in order. A longer run is cut where the order is, into groups of GROUP
+// entries: each group's part is summed by a wave of its own (`tails`: the part of a run that
+// began in an earlier group; `heads`: of one that begins in the group and leaves it),
+// GROUP whole tails are summed once more (`spans`), and the run's wave adds these. Groups and
+// order depend on the sorted ids alone.
+constexpr int GROUP = 64, LONG = 62;
 
-template <class T>
-struct Slab {  // a wave's columns of a row: N a lane
-    static constexpr int N = Vec16<T>::N, COLS = 64 * N;
-};
-
-// acc += columns [col, col + N) of `count` (<= 64) rows; row j's start is row_of(j), wave-uniform
-template <class S, int N, class F>
-__device__ __forceinline__ void add_rows(float (&acc)[N], int count, int col, int dim, F&& row_of) {
-    constexpr int U = 4;
-    static_assert(N % Vec16<S>::N == 0, "a lane's columns are whole vectors");
+// A wave's columns of a row: V vectors of N columns a lane, vector q at (q * 64 + lane) * N.
+template <class S, int N, int V>
+__device__ __forceinline__ void get_cols(const S* row, S (&v)[V][N], int col, int dim) {
+#pragma unroll
+    for (int q = 0; q < V; ++q) {
+        const int c = col + q * 64 * N;
+        if (c + N <= dim) __builtin_memcpy(v[q], row + c, sizeof(S) * N);
+        else
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[q][i] = c + i < dim ? row[c + i] : (S)0.0f;
+    }
+}
+template <class S, int N, int V>
+__device__ __forceinline__ void put_cols(S* row, const S (&v)[V][N], int col, int dim) {
+#pragma unroll
+    for (int q = 0; q < V; ++q) {
+        const int c = col + q * 64 * N;
+        if (c + N <= dim) __builtin_memcpy(row + c, v[q], sizeof(S) * N);
+        else
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (c + i < dim) row[c + i] = v[q][i];
+    }
+}
+// acc += the wave's columns of `count` rows, row_of(j) in turn (the same in all lanes), U in flight
+template <int U, class S, int N, int V, class F>
+__device__ __forceinline__ void add_rows(float (&acc)[V][N], int count, int col, int dim, F&& row_of) {
     for (int j = 0; j < count; j += U) {
-        S v[U][N];
+        S v[U][V][N];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (j + u < count) {
-                const S* p = row_of(j + u) + col;
-                if (col + N <= dim) {
-                    __builtin_memcpy(v[u], p, sizeof(S) * N);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < N; ++i) v[u][i] = col + i < dim ? p[i] : (S)0.0f;
-                }
-            }
-        }
+        for (int u = 0; u < U; ++u)
+            if (j + u < count) get_cols<S, N, V>(row_of(j + u), v[u], col, dim);
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (j + u < count)
 #pragma unroll
-                for (int i = 0; i < N; ++i) acc[i] += (float)v[u][i];
+                for (int q = 0; q < V; ++q)
+#pragma unroll
+                    for (int i = 0; i < N; ++i) acc[q][i] += (float)v[u][q][i];
     }
 }
+// how many lanes from lane 0 on hold `on`
+__device__ __forceinline__ int leading(bool on) {
+    const int first = __ffsll(~__ballot(on)) - 1;
+    return first < 0 ? 64 : first;
+}
 
-// level 1 (SRC = T, rows by position) and level 2 (SRC = float, rows in their order): partial rows
-template <class T, bool SECOND>
-__global__ __launch_bounds__(256) void embed_partial_kernel(const T* __restrict__ grad_out,
-                                                           const float* __restrict__ first, int dim,
-                                                           const uint32_t* __restrict__ key,
-                                                           const uint32_t* __restrict__ pos, int64_t groups,
-                                                           uint32_t rows, float* __restrict__ out) {
-    constexpr int N = Slab<T>::N;
+// One wave per (group, slab): the group's parts of long runs.
+template <class T>
+__global__ __launch_bounds__(256) void embed_groups_kernel(const T* __restrict__ grad_out, int dim,
+                                                          const uint32_t* __restrict__ key,
+                                                          const uint32_t* __restrict__ pos, int64_t n, int64_t groups,
+                                                          uint32_t rows, float* __restrict__ heads,
+                                                          float* __restrict__ tails) {
+    constexpr int N = Vec16<T>::N;
     const int lane = threadIdx.x & 63;
     const int64_t g = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (g >= groups) return;
-    constexpr int64_t SPAN = SECOND ? GROUP * GROUP : GROUP;
-    const uint32_t k = key[g * SPAN];
-    if (k >= rows || key[g * SPAN + SPAN - 1] != k) return;
-    const int col = blockIdx.y * Slab<T>::COLS + lane * N;
-    if (col >= dim) return;
-    float acc[N] = {};
-    if constexpr (SECOND) {
-        add_rows<float>(acc, GROUP, col, dim, [&](int j) { return first + (g * GROUP + j) * dim; });
-    } else {
-        const uint32_t* p = pos + g * SPAN;
-        add_rows<T>(acc, GROUP, col, dim, [&](int j) { return grad_out + (int64_t)p[j] * dim; });
+    const int64_t i = g * GROUP + lane;
+    const uint32_t none = 0xffffffffu;  // no key is that large
+    const uint32_t mine = i < n ? key[i] : none;
+    const uint32_t before = i >= GROUP ? key[i - GROUP] : none;
+    const uint32_t after = i + GROUP < n ? key[i + GROUP] : none;
+    const uint32_t my_pos = i < n ? pos[i] : 0;
+    const uint32_t first = __builtin_amdgcn_readlane(mine, 0), last = __builtin_amdgcn_readlane(mine, 63);
+    const int lead = leading(mine == first);                                 // entries of the first key here
+    const int trail = __clzll(~__ballot(mine == last) | 1);                  // of the last key, below 64 unless all
+    const unsigned long long back = ~__ballot(before == first), ahead = ~__ballot(after == last);
+    const int came = back ? __clzll(back) : 64, goes = ahead ? __ffsll(ahead) - 1 : 64;  // neighbours in the next groups
+    const int col = blockIdx.y * 64 * N + lane * N;
+    auto sum = [&](int from, int count, float* out) {
+        float acc[1][N] = {};
+        add_rows<8, T>(acc, count, col, dim, [&](int j) {
+            return grad_out + (int64_t)(uint32_t)__builtin_amdgcn_readlane(my_pos, from + j) * dim;
+        });
+        put_cols<float, N, 1>(out + g * dim, acc, col, dim);
+    };
+    if (first < rows && came > 0) {  // began before
+        if (came + lead >= LONG) sum(0, lead, tails);
+        if (lead == 64) return;
     }
-    float* o = out + g * dim + col;
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-        if (col + i < dim) o[i] = acc[i];
+    // begins here (a run that fills the group and began before has returned) and goes on
+    const int count = lead == 64 ? 64 : trail;
+    if (last < rows && goes > 0 && count + goes >= LONG) sum(64 - count, count, heads);
 }
 
-// columns [col, col + N) of a row that is added to (read early: the load does not wait for the sum)
-template <class S, int N>
-__device__ __forceinline__ void get_row(const S* o, S (&v)[N], int col, int dim) {
-    if (col + N <= dim) __builtin_memcpy(v, o, sizeof(v));
-    else
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = col + i < dim ? o[i] : (S)0.0f;
-}
-template <class S, int N, bool ADD>
-__device__ __forceinline__ void put_row(S* o, const float (&acc)[N], S (&v)[N], int col, int dim, float scale) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = (S)(ADD ? fmaf(acc[i], scale, (float)v[i]) : acc[i] * scale);
-    if (col + N <= dim) __builtin_memcpy(o, v, sizeof(v));
-    else
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (col + i < dim) o[i] = v[i];
+// One wave per (GROUP groups, slab) that one run fills and began before: the sum of their tails.
+__global__ __launch_bounds__(256) void embed_spans_kernel(const float* __restrict__ tails, int dim,
+                                                         const uint32_t* __restrict__ key, int64_t spans, uint32_t rows,
+                                                         float* __restrict__ out) {
+    const int lane = threadIdx.x & 63;
+    const int64_t s = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (s >= spans || s == 0) return;
+    const int64_t at = s * GROUP * GROUP;
+    const uint32_t k = key[at];
+    if (k >= rows || key[at - 1] != k || key[at + GROUP * GROUP - 1] != k) return;
+    const int col = blockIdx.y * 64 * 4 + lane * 4;
+    float acc[1][4] = {};
+    add_rows<8, float>(acc, GROUP, col, dim, [&](int j) { return tails + (s * GROUP + j) * dim; });
+    put_cols<float, 4, 1>(out + s * dim, acc, col, dim);
 }
 
-// One wave per (sorted entry, slab): the first entry of an id sums the id's rows.
-template <class T, class S, bool ADD>
+// One wave per (sorted entry, slab): the first entry of an id sums the id's run into its row. Bound
+// by HBM: a wave takes up to 4 vectors a lane, so that a row's bytes are all in flight at once.
+template <class T, class S, int V>
 __global__ __launch_bounds__(256) void embed_rows_kernel(const T* __restrict__ grad_out, int dim, int64_t begin,
                                                         const uint32_t* __restrict__ key,
                                                         const uint32_t* __restrict__ pos, int64_t n, uint32_t rows,
-                                                        const float* __restrict__ first,
-                                                        const float* __restrict__ second, float scale, S* grad_table) {
-    constexpr int N = Slab<T>::N;
+                                                        const float* __restrict__ heads,
+                                                        const float* __restrict__ tails,
+                                                        const float* __restrict__ spans, float scale, bool add, S* grad_table) {
+    constexpr int N = Vec16<T>::N;
     const int lane = threadIdx.x & 63;
     const int64_t i0 = begin + (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (i0 >= n) return;
@@ -289,65 +315,64 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const T* __restrict__ g
     const uint32_t near_pos = near_i >= 0 && near_i < n ? pos[near_i] : 0;
     const uint32_t k = __builtin_amdgcn_readlane(near_key, 1);
     if (k >= rows || (uint32_t)__builtin_amdgcn_readlane(near_key, 0) == k) return;
-    const int col = blockIdx.y * Slab<T>::COLS + lane * N;
-    S* const row = grad_table + (int64_t)k * dim + col;
-    S old[N];
-    if constexpr (ADD)
-        if (col < dim) get_row<S, N>(row, old, col, dim);
-    float acc[N] = {};
-    const int run = __ffsll(__ballot(lane > 0 && near_key != k) | 1ull << 63) - 2;  // entries of the id, if below 62
-    if (run < 62) {
-        add_rows<T>(acc, run, min(col, dim), dim,
-                    [&](int j) { return grad_out + (int64_t)(uint32_t)__builtin_amdgcn_readlane(near_pos, j + 1) * dim; });
-        if (col < dim) put_row<S, N, ADD>(row, acc, old, col, dim, scale);
-        return;
-    }
-    int64_t at = i0;
-    while (at < n) {
-        if ((at & (GROUP * GROUP - 1)) == 0 && at + GROUP * GROUP <= n && key[at + GROUP * GROUP - 1] == k) {
-            const int64_t g = at / (GROUP * GROUP);
-            const int64_t left = (n - at) / (GROUP * GROUP);
-            const bool same = lane < left && key[at + (int64_t)(lane + 1) * GROUP * GROUP - 1] == k;
-            const int count = __ffsll(~__ballot(same)) - 1;
-            const int c = count < 0 ? 64 : count;
-            if (col < dim) add_rows<float>(acc, c, col, dim, [&](int j) { return second + (g + j) * dim; });
-            at += (int64_t)c * GROUP * GROUP;
-        } else if ((at & (GROUP - 1)) == 0 && at + GROUP <= n && key[at + GROUP - 1] == k) {
-            // partial rows up to the next whole second-level group
-            const int64_t g = at / GROUP;
-            const int64_t left = min((n - at) / GROUP, (int64_t)GROUP - (g & (GROUP - 1)));
-            const bool same = lane < left && key[at + (int64_t)(lane + 1) * GROUP - 1] == k;
-            const int count = __ffsll(~__ballot(same)) - 1;
-            const int c = count < 0 ? 64 : count;
-            if (col < dim) add_rows<float>(acc, c, col, dim, [&](int j) { return first + (g + j) * dim; });
-            at += (int64_t)c * GROUP;
-        } else {
-            // single rows up to the next whole group
-            const int left = (int)min(n - at, (int64_t)GROUP - (at & (GROUP - 1)));
-            const bool same = lane < left && key[at + lane] == k;
-            const int count = __ffsll(~__ballot(same)) - 1;
-            const int c = count < 0 ? 64 : count;
-            const uint32_t p = same ? pos[at + lane] : 0;
-            add_rows<T>(acc, c, min(col, dim), dim,
-                        [&](int j) { return grad_out + (int64_t)(uint32_t)__builtin_amdgcn_readlane(p, j) * dim; });
-            at += c;
-            if (c < left) break;
-            continue;
+    const int col = blockIdx.y * 64 * N * V + lane * N;
+    S* const row = grad_table + (int64_t)k * dim;
+    S old[V][N] = {};
+    if (add) get_cols<S, N, V>(row, old, col, dim);  // does not wait for the sum
+    float acc[V][N] = {};
+    const int run = __ffsll(__ballot(lane > 0 && near_key != k) | 1ull << 63) - 2;  // LONG: that many or more
+    if (run < LONG) {
+        add_rows<2, T>(acc, run, col, dim, [&](int j) {
+            return grad_out + (int64_t)(uint32_t)__builtin_amdgcn_readlane(near_pos, j + 1) * dim;
+        });
+    } else if (const int64_t end = (i0 / GROUP + 1) * GROUP; end >= n || key[end] != k) {  // stays in its group
+        const bool mine = i0 + lane < n && key[i0 + lane] == k;
+        const uint32_t p = mine ? pos[i0 + lane] : 0;
+        add_rows<2, T>(acc, leading(mine), col, dim, [&](int j) {
+            return grad_out + (int64_t)(uint32_t)__builtin_amdgcn_readlane(p, j) * dim;
+        });
+    } else {
+        // the head's group, then whole spans where there are, then tails
+        int64_t g = i0 / GROUP;
+        add_rows<1, float>(acc, 1, col, dim, [&](int) { return heads + g * dim; });
+        ++g;
+        const int64_t whole_spans = n / (GROUP * GROUP);
+        while (g * GROUP < n) {
+            if ((g & (GROUP - 1)) == 0 && g / GROUP < whole_spans) {
+                const int64_t s = g / GROUP;
+                const int count = leading(s + lane < whole_spans && key[(s + lane + 1) * GROUP * GROUP - 1] == k);
+                if (count) {
+                    add_rows<8, float>(acc, count, col, dim, [&](int j) { return spans + (s + j) * dim; });
+                    g += (int64_t)count * GROUP;
+                    continue;
+                }
+            }
+            // tails up to the next span's begin: a group has one if its first entry is the id's
+            const int most = GROUP - (int)(g & (GROUP - 1));
+            const int count = leading(lane < most && (g + lane) * GROUP < n && key[(g + lane) * GROUP] == k);
+            add_rows<8, float>(acc, count, col, dim, [&](int j) { return tails + (g + j) * dim; });
+            g += count;
+            if (count < most) break;
         }
-        if (at < n && key[at] != k) break;
     }
-    if (col < dim) put_row<S, N, ADD>(row, acc, old, col, dim, scale);
+    S v[V][N];
+#pragma unroll
+    for (int q = 0; q < V; ++q)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            v[q][i] = (S)fmaf(acc[q][i], scale, (float)old[q][i]);
+    put_cols<S, N, V>(row, v, col, dim);
 }
 
 // Few positions: no sort. The wave of position i looks for its id among the positions before it
 // (then another wave has the row) and adds the rows of the positions after it, in order.
 constexpr int SCAN_MAX = 1024;
 
-template <class T, class S, bool ADD>
+template <class T, class S>
 __global__ __launch_bounds__(256) void embed_scan_kernel(const T* __restrict__ grad_out, int dim,
                                                         const int64_t* __restrict__ ids, int n, int64_t rows,
-                                                        float scale, S* grad_table) {
-    constexpr int N = Slab<T>::N;
+                                                        float scale, bool add, S* grad_table) {
+    constexpr int N = Vec16<T>::N;
     const int lane = threadIdx.x & 63;
     const int i0 = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (i0 >= n) return;
@@ -355,27 +380,26 @@ __global__ __launch_bounds__(256) void embed_scan_kernel(const T* __restrict__ g
     if (id < 0 || id >= rows) return;
     for (int j = 0; j < i0; j += 64)
         if (__any(j + lane < i0 && ids[j + lane] == id)) return;
-    const int col = blockIdx.y * Slab<T>::COLS + lane * N;
-    float acc[N] = {};
+    const int col = blockIdx.y * 64 * N + lane * N;
+    S* const row = grad_table + id * dim;
+    S v[1][N] = {};
+    if (add) get_cols<S, N, 1>(row, v, col, dim);
+    float acc[1][N] = {};
     for (int j = i0; j < n; j += 64) {
         unsigned long long m = __ballot(j + lane < n && ids[j + lane] == id);
         const int count = __popcll(m);
-        // lane r holds the r-th position of the group's rows
-        int mine = 0;
+        int mine = 0;  // lane r: the r-th position of the 64 with the id
         for (int r = 0; r < count; ++r) {
             const int b = __ffsll(m) - 1;
             m &= m - 1;
             if (lane == r) mine = j + b;
         }
-        add_rows<T>(acc, count, min(col, dim), dim,
-                    [&](int r) { return grad_out + (int64_t)__builtin_amdgcn_readlane(mine, r) * dim; });
+        add_rows<4, T>(acc, count, col, dim,
+                       [&](int r) { return grad_out + (int64_t)__builtin_amdgcn_readlane(mine, r) * dim; });
     }
-    if (col < dim) {
-        S* const row = grad_table + id * dim + col;
-        S old[N];
-        if constexpr (ADD) get_row<S, N>(row, old, col, dim);
-        put_row<S, N, ADD>(row, acc, old, col, dim, scale);
-    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[0][i] = (S)fmaf(acc[0][i], scale, (float)v[0][i]);
+    put_cols<S, N, 1>(row, v, col, dim);
 }
 
 __global__ __launch_bounds__(256) void clear_bits_kernel(uint32_t* p, int64_t words) {
@@ -433,24 +457,19 @@ void embedding_backward(int32_t dtype, const void* grad_out, const int64_t* ids,
         RVX_LAUNCH("embedding_zero", embed_zero_kernel, dim3((unsigned)blocks), dim3(256), 0, (unsigned char*)grad_table,
                    rows, row_bytes, present);
     };
-    auto typed = [&](auto&& f) {  // f(T, S, ADD) of the gradient's, the table's type and the mode
-        with_dtype(dtype, [&](auto t) {
-            with_dtype(table_dtype, [&](auto s) {
-                if (accumulate) f(t, s, std::true_type{});
-                else f(t, s, std::false_type{});
-            });
-        });
+    auto typed = [&](auto&& f) {  // f(T, S) of the gradient's and the table's type
+        with_dtype(dtype, [&](auto t) { with_dtype(table_dtype, [&](auto s) { f(t, s); }); });
     };
     if (n <= SCAN_MAX) {
         if (!accumulate) zero_rows(nullptr);
         if (n == 0) return;
-        typed([&](auto t, auto s, auto add) {
+        typed([&](auto t, auto s) {
             using T = decltype(t);
             using S = decltype(s);
-            const int slabs = (dim + Slab<T>::COLS - 1) / Slab<T>::COLS;
-            RVX_LAUNCH("embedding_backward", (embed_scan_kernel<T, S, decltype(add)::value>),
+            const int slabs = (dim + 64 * Vec16<T>::N - 1) / (64 * Vec16<T>::N);
+            RVX_LAUNCH("embedding_backward", (embed_scan_kernel<T, S>),
                        dim3((unsigned)((n + 3) / 4), slabs), dim3(256), 0, (const T*)grad_out, dim, ids, (int)n,
-                       rows, scale, (S*)grad_table);
+                       rows, scale, accumulate, (S*)grad_table);
         });
         return;
     }
@@ -464,9 +483,9 @@ void embedding_backward(int32_t dtype, const void* grad_out, const int64_t* ids,
     auto* counts = (uint32_t*)scratch_bytes("embed_counts", ((int64_t)SORT_TILES << bits) * 4);
     auto* sorted = (uint32_t*)scratch_bytes("embed_sorted", n * 16);  // key, pos and their other halves
     uint32_t *key[2] = {sorted, sorted + 2 * n}, *pos[2] = {sorted + n, sorted + 3 * n};
-    const int64_t groups = n / GROUP, groups2 = groups / GROUP;
-    float* first = scratch_f32("embed_partial", std::max<int64_t>(1, (groups + groups2) * dim));
-    float* second = first + groups * dim;
+    const int64_t groups = (n + GROUP - 1) / GROUP, span_count = n / (GROUP * GROUP);
+    float* heads = scratch_f32("embed_partial", (2 * groups + span_count) * dim);
+    float *tails = heads + groups * dim, *spans = tails + groups * dim;
     for (int p = 0; p < passes; ++p) {
         const int in = (p + 1) & 1, out = p & 1, shift = p * bits;
         if (p == 0) {
@@ -494,22 +513,29 @@ void embedding_backward(int32_t dtype, const void* grad_out, const int64_t* ids,
                    (uint32_t)rows, present);
         zero_rows(present);
     }
-    typed([&](auto t, auto s, auto add) {
+    typed([&](auto t, auto s) {
         using T = decltype(t);
         using S = decltype(s);
-        const int slabs = (dim + Slab<T>::COLS - 1) / Slab<T>::COLS;
-        auto blocks = [&](int64_t items) { return dim3((unsigned)((items + 3) / 4), slabs); };
-        if (groups)
-            RVX_LAUNCH("embedding_partial", (embed_partial_kernel<T, false>), blocks(groups), dim3(256), 0,
-                       (const T*)grad_out, (const float*)nullptr, dim, sk, sp, groups, (uint32_t)rows, first);
-        if (groups2)
-            RVX_LAUNCH("embedding_partial", (embed_partial_kernel<T, true>), blocks(groups2), dim3(256), 0,
-                       (const T*)grad_out, (const float*)first, dim, sk, sp, groups2, (uint32_t)rows, second);
-        constexpr int64_t SLICE = (int64_t)1 << 24;  // entries of one launch: at most 2^30 threads
-        for (int64_t i = 0; i < n; i += SLICE)
-        RVX_LAUNCH("embedding_backward", (embed_rows_kernel<T, S, decltype(add)::value>), blocks(std::min(SLICE, n - i)),
-                   dim3(256), 0, (const T*)grad_out, dim, i, sk, sp, n, (uint32_t)rows, (const float*)first,
-                   (const float*)second, scale, (S*)grad_table);
+        constexpr int N = Vec16<T>::N;
+        const int vecs = (dim + 64 * N - 1) / (64 * N);  // vectors a lane for a whole row
+        RVX_LAUNCH("embedding_groups", embed_groups_kernel<T>, dim3((unsigned)((groups + 3) / 4), vecs), dim3(256), 0,
+                   (const T*)grad_out, dim, sk, sp, n, groups, (uint32_t)rows, heads, tails);
+        if (span_count > 1)
+            RVX_LAUNCH("embedding_groups", embed_spans_kernel, dim3((unsigned)((span_count + 3) / 4), (dim + 255) / 256),
+                       dim3(256), 0, (const float*)tails, dim, sk, span_count, (uint32_t)rows, spans);
+        const int slabs = (vecs + 3) / 4, per = (vecs + slabs - 1) / slabs;
+        auto go = [&](auto v) {
+            constexpr int64_t SLICE = (int64_t)1 << 24;  // entries of one launch: at most 2^30 threads
+            for (int64_t i = 0; i < n; i += SLICE)
+                RVX_LAUNCH("embedding_backward", (embed_rows_kernel<T, S, decltype(v)::value>),
+                           dim3((unsigned)((std::min(SLICE, n - i) + 3) / 4), slabs), dim3(256), 0, (const T*)grad_out, dim, i,
+                           sk, sp, n, (uint32_t)rows, (const float*)heads, (const float*)tails, (const float*)spans, scale,
+                           accumulate, (S*)grad_table);
+        };
+        if (per == 1) go(std::integral_constant<int, 1>{});
+        else if (per == 2) go(std::integral_constant<int, 2>{});
+        else if (per == 3) go(std::integral_constant<int, 3>{});
+        else go(std::integral_constant<int, 4>{});
     });
 }
 

@@ -90,6 +90,22 @@ def test_gradient(dtype, table_dtype, rows, dim, n, kind, accumulate):
     assert torch.equal(got.view(torch.uint8), again.view(torch.uint8))
 
 
+@pytest.mark.parametrize("length", [1, 2, 61, 62, 63, 64, 65, 126, 127, 128, 129, 4096, 4097, 8500])
+@pytest.mark.parametrize("before", [0, 1, 2, 62, 63, 64])
+def test_gradient_runs_at_every_edge(length, before):
+    """A run of one id that starts `before` entries into the sorted order, between runs of others."""
+    rows, dim = 9, 5
+    ids = torch.cat([torch.zeros(before, dtype=torch.int64), torch.full((length,), 3), torch.full((70,), 4),
+                     torch.full((63,), 5), torch.arange(900) % 3 + 6])
+    g = torch.Generator().manual_seed(length)
+    ids = torch.cat([ids, torch.full((max(0, 1100 - len(ids)),), 8)])[torch.randperm(max(1100, len(ids)), generator=g)]
+    # whole numbers: every sum is exact in 32 bits
+    dy = torch.randint(-8, 9, (len(ids), dim), generator=g).float()
+    want = torch.zeros(rows, dim).index_add_(0, ids, dy)
+    assert torch.equal(_grad(dy, ids, torch.zeros(rows, dim), "f32", "f32", False, scale=1.0), want)
+    assert torch.equal(_grad(dy, ids, torch.ones(rows, dim), "f32", "f32", True, scale=1.0), want + 1)
+
+
 def test_gradient_without_positions():
     start = torch.randn(5, 6)
     assert torch.equal(_grad(torch.empty(0, 6), torch.empty(0, dtype=torch.int64), start, "f32", "f32", True), start)
