@@ -69,11 +69,15 @@ __device__ __forceinline__ uint32_t sort_key(const int64_t* ids, int64_t i, uint
     return id >= 0 && id < (int64_t)rows ? (uint32_t)id : rows;
 }
 
+// counts[tile][digit]; clear: nullable, words to set to 0
 template <bool FIRST>
 __global__ __launch_bounds__(SORT_THREADS) void sort_count_kernel(const int64_t* __restrict__ ids,
                                                                  const uint32_t* __restrict__ key_in, int64_t n,
                                                                  uint32_t rows, int64_t tile, int bits, int shift,
-                                                                 uint32_t* __restrict__ counts) {
+                                                                 uint32_t* __restrict__ counts, uint32_t* clear,
+                                                                 int64_t words) {
+    for (int64_t i = (int64_t)blockIdx.x * SORT_THREADS + threadIdx.x; clear && i < words; i += gridDim.x * SORT_THREADS)
+        clear[i] = 0;
     __shared__ uint32_t hist[SORT_BINS];
     const int bins = 1 << bits;
     for (int d = threadIdx.x; d < bins; d += SORT_THREADS) hist[d] = 0;
@@ -99,34 +103,37 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_move_kernel(const int64_t* 
                                                                 uint32_t* __restrict__ pos_out) {
     __shared__ uint32_t base[SORT_BINS];               // where this block's next element of a digit goes
     __shared__ uint32_t mine[SORT_WAVES][SORT_BINS];   // per wave: its count of a digit, then its next place
-    __shared__ uint32_t sums[SORT_THREADS];
+    __shared__ uint32_t sums[SORT_WAVES];
     const int bins = 1 << bits, t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int me = blockIdx.x;
     // base[d] = elements of smaller digits anywhere + of digit d in the tiles before
     constexpr int PER = SORT_BINS / SORT_THREADS;
-    uint32_t total[PER], ahead[PER], sum = 0;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        const int d = t * PER + j;
-        total[j] = ahead[j] = 0;
-        if (d < bins)
+    uint32_t total[PER] = {}, ahead[PER] = {}, sum = 0;
+    if (t * PER < bins) {  // bins are a multiple of PER
+        const uint32_t* c = counts + t * PER;
 #pragma unroll 8
-            for (int b = 0; b < tiles; ++b) {
-                const uint32_t v = counts[(int64_t)b << bits | d];
-                total[j] += v;
-                ahead[j] += b < me ? v : 0;
+        for (int b = 0; b < tiles; ++b) {
+            uint32_t v[PER];
+            __builtin_memcpy(v, c + ((int64_t)b << bits), sizeof(v));
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                total[j] += v[j];
+                ahead[j] += b < me ? v[j] : 0;
             }
-        sum += total[j];
+        }
+#pragma unroll
+        for (int j = 0; j < PER; ++j) sum += total[j];
     }
-    sums[t] = sum;
+    uint32_t scan = sum;  // over the wave's lanes, then over the waves
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t v = __shfl_up(scan, o);
+        scan += lane >= o ? v : 0;
+    }
+    if (lane == 63) sums[wave] = scan;
     __syncthreads();
-    for (int o = 1; o < SORT_THREADS; o <<= 1) {
-        const uint32_t v = t >= o ? sums[t - o] : 0;
-        __syncthreads();
-        sums[t] += v;
-        __syncthreads();
-    }
-    uint32_t run = t ? sums[t - 1] : 0;
+    uint32_t run = scan - sum;
+    for (int w = 0; w < wave; ++w) run += sums[w];
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
         base[t * PER + j] = run + ahead[j];
@@ -187,53 +194,61 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_move_kernel(const int64_t* 
 
 // ---------------------------------------------------------------- sums over groups
 // An id's entries are a run of the sorted order. A run of fewer than LONG entries is summed by one
-// wave per slab of columns, in order. A longer run is cut where the order is, into groups of GROUP
-// entries: each group's part is summed by a wave of its own (`tails`: the part of a run that
-// began in an earlier group; `heads`: of one that begins in the group and leaves it),
-// GROUP whole tails are summed once more (`spans`), and the run's wave adds these. Groups and
-// order depend on the sorted ids alone.
-constexpr int GROUP = 64, LONG = 62;
+// wave per slab of columns, in order. A longer one is cut where the order is, into groups of GROUP
+// entries: a group's part of its first key's run (`tails`) and of its last key's (`heads`, where
+// that is another key) are summed by a wave of their own, GROUP whole tails of one run once more
+// (`spans`), and the wave of the run's first group adds these. (A run of LONG entries touches an end
+// of its group.) Groups and order depend on the sorted ids alone.
+constexpr int GROUP = 64, LONG = 63;
+
+// N values of S as one vector (kept packed: arrays of 16-bit values are spread over registers)
+template <class S, int N>
+struct Pack {
+    typedef S V __attribute__((ext_vector_type(N)));
+};
+template <class S, int N>
+using PackOf = typename Pack<S, N>::V;
 
 // A wave's columns of a row: V vectors of N columns a lane, vector q at (q * 64 + lane) * N.
 template <class S, int N, int V>
-__device__ __forceinline__ void get_cols(const S* row, S (&v)[V][N], int col, int dim) {
+__device__ __forceinline__ void get_cols(const S* row, PackOf<S, N> (&v)[V], int col, int dim) {
 #pragma unroll
     for (int q = 0; q < V; ++q) {
         const int c = col + q * 64 * N;
-        if (c + N <= dim) __builtin_memcpy(v[q], row + c, sizeof(S) * N);
+        if (c + N <= dim) __builtin_memcpy(&v[q], row + c, sizeof(S) * N);
         else
 #pragma unroll
             for (int i = 0; i < N; ++i) v[q][i] = c + i < dim ? row[c + i] : (S)0.0f;
     }
 }
 template <class S, int N, int V>
-__device__ __forceinline__ void put_cols(S* row, const S (&v)[V][N], int col, int dim) {
+__device__ __forceinline__ void put_cols(S* row, const PackOf<S, N> (&v)[V], int col, int dim) {
 #pragma unroll
     for (int q = 0; q < V; ++q) {
         const int c = col + q * 64 * N;
-        if (c + N <= dim) __builtin_memcpy(row + c, v[q], sizeof(S) * N);
+        if (c + N <= dim) __builtin_memcpy(row + c, &v[q], sizeof(S) * N);
         else
 #pragma unroll
             for (int i = 0; i < N; ++i)
                 if (c + i < dim) row[c + i] = v[q][i];
     }
 }
-// acc += the wave's columns of `count` rows, row_of(j) in turn (the same in all lanes), U in flight
+// acc += the wave's columns of rows [j, count), row_of(j) in turn (the same in all lanes): U rows in
+// flight while there are U, then U / 2 ..
 template <int U, class S, int N, int V, class F>
-__device__ __forceinline__ void add_rows(float (&acc)[V][N], int count, int col, int dim, F&& row_of) {
-    for (int j = 0; j < count; j += U) {
-        S v[U][V][N];
+__device__ __forceinline__ void add_rows(PackOf<float, N> (&acc)[V], int count, int col, int dim, F&& row_of, int j = 0) {
+    for (; j + U <= count; j += U) {
+        PackOf<S, N> v[U][V];
+#pragma unroll
+        for (int u = 0; u < U; ++u) get_cols<S, N, V>(row_of(j + u), v[u], col, dim);
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (j + u < count) get_cols<S, N, V>(row_of(j + u), v[u], col, dim);
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (j + u < count)
+            for (int q = 0; q < V; ++q)
 #pragma unroll
-                for (int q = 0; q < V; ++q)
-#pragma unroll
-                    for (int i = 0; i < N; ++i) acc[q][i] += (float)v[u][q][i];
+                for (int i = 0; i < N; ++i) acc[q][i] += (float)v[u][q][i];
     }
+    if constexpr (U > 1) add_rows<U / 2, S, N, V>(acc, count, col, dim, row_of, j);
 }
 // how many lanes from lane 0 on hold `on`
 __device__ __forceinline__ int leading(bool on) {
@@ -241,43 +256,63 @@ __device__ __forceinline__ int leading(bool on) {
     return first < 0 ? 64 : first;
 }
 
+// What a wave sees of group g and of the groups beside it.
+struct Group {
+    uint32_t first, last;      // its first and last key
+    int lead, trail;           // entries of either in it; trail counts the last key only where it is another
+    int came, goes;            // entries of the first key just before it, of the last just after it, up to 64
+    uint32_t key, pos;         // this lane's entry
+    __device__ __forceinline__ Group(const uint32_t* __restrict__ keys, const uint32_t* __restrict__ poss, int64_t n,
+                                     int64_t g) {
+        const int lane = threadIdx.x & 63;
+        const int64_t i = g * GROUP + lane;
+        const uint32_t none = 0xffffffffu;  // no key is that large
+        key = i < n ? keys[i] : none;
+        pos = i < n ? poss[i] : 0;
+        const uint32_t before = i >= GROUP ? keys[i - GROUP] : none;
+        const uint32_t after = i + GROUP < n ? keys[i + GROUP] : none;
+        first = __builtin_amdgcn_readlane(key, 0), last = __builtin_amdgcn_readlane(key, 63);
+        lead = leading(key == first);
+        trail = lead == 64 ? 0 : __clzll(~__ballot(key == last));
+        const unsigned long long back = ~__ballot(before == first);
+        came = back ? __clzll(back) : 64;
+        goes = leading(after == last);
+    }
+    __device__ __forceinline__ bool long_first(uint32_t rows) const {
+        return first < rows && came + lead + (lead == 64 ? goes : 0) >= LONG;
+    }
+    __device__ __forceinline__ bool long_last(uint32_t rows) const { return last < rows && trail > 0 && trail + goes >= LONG; }
+};
+
+// A 1 for every row that is looked up, from the first entry of each id's run.
+__global__ __launch_bounds__(256) void embed_mark_kernel(const uint32_t* __restrict__ key, int64_t n, uint32_t rows,
+                                                        unsigned char* __restrict__ present) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const uint32_t k = key[i];
+        if (k < rows && (i == 0 || key[i - 1] != k)) present[k] = 1;
+    }
+}
+
 // One wave per (group, slab): the group's parts of long runs.
 template <class T>
-__global__ __launch_bounds__(256) void embed_groups_kernel(const T* __restrict__ grad_out, int dim,
-                                                          const uint32_t* __restrict__ key,
-                                                          const uint32_t* __restrict__ pos, int64_t n, int64_t groups,
-                                                          uint32_t rows, float* __restrict__ heads,
-                                                          float* __restrict__ tails) {
+__global__ __launch_bounds__(64) void embed_groups_kernel(const T* __restrict__ grad_out, int dim,
+                                                         const uint32_t* __restrict__ key,
+                                                         const uint32_t* __restrict__ pos, int64_t n, uint32_t rows,
+                                                         float* __restrict__ heads, float* __restrict__ tails) {
     constexpr int N = Vec16<T>::N;
-    const int lane = threadIdx.x & 63;
-    const int64_t g = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (g >= groups) return;
-    const int64_t i = g * GROUP + lane;
-    const uint32_t none = 0xffffffffu;  // no key is that large
-    const uint32_t mine = i < n ? key[i] : none;
-    const uint32_t before = i >= GROUP ? key[i - GROUP] : none;
-    const uint32_t after = i + GROUP < n ? key[i + GROUP] : none;
-    const uint32_t my_pos = i < n ? pos[i] : 0;
-    const uint32_t first = __builtin_amdgcn_readlane(mine, 0), last = __builtin_amdgcn_readlane(mine, 63);
-    const int lead = leading(mine == first);                                 // entries of the first key here
-    const int trail = __clzll(~__ballot(mine == last) | 1);                  // of the last key, below 64 unless all
-    const unsigned long long back = ~__ballot(before == first), ahead = ~__ballot(after == last);
-    const int came = back ? __clzll(back) : 64, goes = ahead ? __ffsll(ahead) - 1 : 64;  // neighbours in the next groups
+    const int64_t g = blockIdx.x;
+    const int lane = threadIdx.x;
+    const Group at(key, pos, n, g);
     const int col = blockIdx.y * 64 * N + lane * N;
     auto sum = [&](int from, int count, float* out) {
-        float acc[1][N] = {};
-        add_rows<8, T>(acc, count, col, dim, [&](int j) {
-            return grad_out + (int64_t)(uint32_t)__builtin_amdgcn_readlane(my_pos, from + j) * dim;
+        PackOf<float, N> acc[1] = {};
+        add_rows<16, T, N, 1>(acc, count, col, dim, [&](int j) {
+            return grad_out + (int64_t)(uint32_t)__builtin_amdgcn_readlane(at.pos, from + j) * dim;
         });
         put_cols<float, N, 1>(out + g * dim, acc, col, dim);
     };
-    if (first < rows && came > 0) {  // began before
-        if (came + lead >= LONG) sum(0, lead, tails);
-        if (lead == 64) return;
-    }
-    // begins here (a run that fills the group and began before has returned) and goes on
-    const int count = lead == 64 ? 64 : trail;
-    if (last < rows && goes > 0 && count + goes >= LONG) sum(64 - count, count, heads);
+    if (at.long_first(rows)) sum(0, at.lead, tails);
+    if (at.long_last(rows)) sum(64 - at.trail, at.trail, heads);
 }
 
 // One wave per (GROUP groups, slab) that one run fills and began before: the sum of their tails.
@@ -291,9 +326,62 @@ __global__ __launch_bounds__(256) void embed_spans_kernel(const float* __restric
     const uint32_t k = key[at];
     if (k >= rows || key[at - 1] != k || key[at + GROUP * GROUP - 1] != k) return;
     const int col = blockIdx.y * 64 * 4 + lane * 4;
-    float acc[1][4] = {};
-    add_rows<8, float>(acc, GROUP, col, dim, [&](int j) { return tails + (s * GROUP + j) * dim; });
+    PackOf<float, 4> acc[1] = {};
+    add_rows<8, float, 4, 1>(acc, GROUP, col, dim, [&](int j) { return tails + (s * GROUP + j) * dim; });
     put_cols<float, 4, 1>(out + s * dim, acc, col, dim);
+}
+
+// row = scale * acc (+ row)
+template <class S, int N, int V>
+__device__ __forceinline__ void finish_row(S* row, const PackOf<float, N> (&acc)[V], const PackOf<S, N> (&old)[V], int col, int dim,
+                                           float scale) {
+    PackOf<S, N> v[V];
+#pragma unroll
+    for (int q = 0; q < V; ++q)
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[q][i] = (S)fmaf(acc[q][i], scale, (float)old[q][i]);
+    put_cols<S, N, V>(row, v, col, dim);
+}
+
+// One wave per (group, slab): the rows of the long runs that begin in the group.
+template <class T, class S>
+__global__ __launch_bounds__(64) void embed_long_kernel(int dim, const uint32_t* __restrict__ key,
+                                                       const uint32_t* __restrict__ pos, int64_t n, uint32_t rows,
+                                                       const float* __restrict__ heads, const float* __restrict__ tails,
+                                                       const float* __restrict__ spans, float scale, bool add,
+                                                       S* grad_table) {
+    constexpr int N = Vec16<T>::N;
+    const int lane = threadIdx.x;
+    const Group here(key, pos, n, blockIdx.x);
+    const int col = blockIdx.y * 64 * N + lane * N;
+    const int64_t whole_spans = n / (GROUP * GROUP);
+    auto run = [&](uint32_t k, const float* part, bool on) {  // on: the run leaves the group
+        S* const row = grad_table + (int64_t)k * dim;
+        PackOf<S, N> old[1] = {};
+        if (add) get_cols<S, N, 1>(row, old, col, dim);
+        PackOf<float, N> acc[1] = {};
+        add_rows<1, float, N, 1>(acc, 1, col, dim, [&](int) { return part + (int64_t)blockIdx.x * dim; });
+        for (int64_t g = blockIdx.x + 1; on && g * GROUP < n;) {
+            if ((g & (GROUP - 1)) == 0 && g / GROUP < whole_spans) {
+                const int64_t s = g / GROUP;
+                const int count = leading(s + lane < whole_spans && key[(s + lane + 1) * GROUP * GROUP - 1] == k);
+                if (count) {
+                    add_rows<8, float, N, 1>(acc, count, col, dim, [&](int j) { return spans + (s + j) * dim; });
+                    g += (int64_t)count * GROUP;
+                    continue;
+                }
+            }
+            // tails up to the next span's begin: a group has one if its first entry is the id's
+            const int most = GROUP - (int)(g & (GROUP - 1));
+            const int count = leading(lane < most && (g + lane) * GROUP < n && key[(g + lane) * GROUP] == k);
+            add_rows<8, float, N, 1>(acc, count, col, dim, [&](int j) { return tails + (g + j) * dim; });
+            g += count;
+            on = count == most;
+        }
+        finish_row<S, N, 1>(row, acc, old, col, dim, scale);
+    };
+    if (here.came == 0 && here.long_first(rows)) run(here.first, tails, here.lead == 64 && here.goes > 0);
+    if (here.long_last(rows)) run(here.last, heads, here.goes > 0);
 }
 
 // One wave per (sorted entry, slab): the first entry of an id sums the id's run into its row. Bound
@@ -302,9 +390,7 @@ template <class T, class S, int V>
 __global__ __launch_bounds__(256) void embed_rows_kernel(const T* __restrict__ grad_out, int dim, int64_t begin,
                                                         const uint32_t* __restrict__ key,
                                                         const uint32_t* __restrict__ pos, int64_t n, uint32_t rows,
-                                                        const float* __restrict__ heads,
-                                                        const float* __restrict__ tails,
-                                                        const float* __restrict__ spans, float scale, bool add, S* grad_table) {
+                                                        float scale, bool add, S* grad_table) {
     constexpr int N = Vec16<T>::N;
     const int lane = threadIdx.x & 63;
     const int64_t i0 = begin + (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -315,53 +401,18 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const T* __restrict__ g
     const uint32_t near_pos = near_i >= 0 && near_i < n ? pos[near_i] : 0;
     const uint32_t k = __builtin_amdgcn_readlane(near_key, 1);
     if (k >= rows || (uint32_t)__builtin_amdgcn_readlane(near_key, 0) == k) return;
+    const unsigned long long others = __ballot(lane > 0 && near_key != k);
+    if (!others) return;  // LONG entries or more
+    const int run = __ffsll(others) - 2;
     const int col = blockIdx.y * 64 * N * V + lane * N;
     S* const row = grad_table + (int64_t)k * dim;
-    S old[V][N] = {};
+    PackOf<S, N> old[V] = {};
     if (add) get_cols<S, N, V>(row, old, col, dim);  // does not wait for the sum
-    float acc[V][N] = {};
-    const int run = __ffsll(__ballot(lane > 0 && near_key != k) | 1ull << 63) - 2;  // LONG: that many or more
-    if (run < LONG) {
-        add_rows<2, T>(acc, run, col, dim, [&](int j) {
-            return grad_out + (int64_t)(uint32_t)__builtin_amdgcn_readlane(near_pos, j + 1) * dim;
-        });
-    } else if (const int64_t end = (i0 / GROUP + 1) * GROUP; end >= n || key[end] != k) {  // stays in its group
-        const bool mine = i0 + lane < n && key[i0 + lane] == k;
-        const uint32_t p = mine ? pos[i0 + lane] : 0;
-        add_rows<2, T>(acc, leading(mine), col, dim, [&](int j) {
-            return grad_out + (int64_t)(uint32_t)__builtin_amdgcn_readlane(p, j) * dim;
-        });
-    } else {
-        // the head's group, then whole spans where there are, then tails
-        int64_t g = i0 / GROUP;
-        add_rows<1, float>(acc, 1, col, dim, [&](int) { return heads + g * dim; });
-        ++g;
-        const int64_t whole_spans = n / (GROUP * GROUP);
-        while (g * GROUP < n) {
-            if ((g & (GROUP - 1)) == 0 && g / GROUP < whole_spans) {
-                const int64_t s = g / GROUP;
-                const int count = leading(s + lane < whole_spans && key[(s + lane + 1) * GROUP * GROUP - 1] == k);
-                if (count) {
-                    add_rows<8, float>(acc, count, col, dim, [&](int j) { return spans + (s + j) * dim; });
-                    g += (int64_t)count * GROUP;
-                    continue;
-                }
-            }
-            // tails up to the next span's begin: a group has one if its first entry is the id's
-            const int most = GROUP - (int)(g & (GROUP - 1));
-            const int count = leading(lane < most && (g + lane) * GROUP < n && key[(g + lane) * GROUP] == k);
-            add_rows<8, float>(acc, count, col, dim, [&](int j) { return tails + (g + j) * dim; });
-            g += count;
-            if (count < most) break;
-        }
-    }
-    S v[V][N];
-#pragma unroll
-    for (int q = 0; q < V; ++q)
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            v[q][i] = (S)fmaf(acc[q][i], scale, (float)old[q][i]);
-    put_cols<S, N, V>(row, v, col, dim);
+    PackOf<float, N> acc[V] = {};
+    add_rows<V == 1 ? 8 : V == 2 ? 4 : 2, T, N, V>(acc, run, col, dim, [&](int j) {
+        return grad_out + (int64_t)(uint32_t)__builtin_amdgcn_readlane(near_pos, j + 1) * dim;
+    });
+    finish_row<S, N, V>(row, acc, old, col, dim, scale);
 }
 
 // Few positions: no sort. The wave of position i looks for its id among the positions before it
@@ -382,9 +433,9 @@ __global__ __launch_bounds__(256) void embed_scan_kernel(const T* __restrict__ g
         if (__any(j + lane < i0 && ids[j + lane] == id)) return;
     const int col = blockIdx.y * 64 * N + lane * N;
     S* const row = grad_table + id * dim;
-    S v[1][N] = {};
+    PackOf<S, N> v[1] = {};
     if (add) get_cols<S, N, 1>(row, v, col, dim);
-    float acc[1][N] = {};
+    PackOf<float, N> acc[1] = {};
     for (int j = i0; j < n; j += 64) {
         unsigned long long m = __ballot(j + lane < n && ids[j + lane] == id);
         const int count = __popcll(m);
@@ -394,7 +445,7 @@ __global__ __launch_bounds__(256) void embed_scan_kernel(const T* __restrict__ g
             m &= m - 1;
             if (lane == r) mine = j + b;
         }
-        add_rows<4, T>(acc, count, col, dim,
+        add_rows<4, T, N, 1>(acc, count, col, dim,
                        [&](int r) { return grad_out + (int64_t)__builtin_amdgcn_readlane(mine, r) * dim; });
     }
 #pragma unroll
@@ -402,35 +453,41 @@ __global__ __launch_bounds__(256) void embed_scan_kernel(const T* __restrict__ g
     put_cols<S, N, 1>(row, v, col, dim);
 }
 
-__global__ __launch_bounds__(256) void clear_bits_kernel(uint32_t* p, int64_t words) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (int64_t)gridDim.x * 256) p[i] = 0;
-}
-// a bit for each row that is looked up, from the first entry of each id in the sorted order
-__global__ __launch_bounds__(256) void mark_rows_kernel(const uint32_t* __restrict__ key, int64_t n, uint32_t rows,
-                                                       uint32_t* present) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const uint32_t k = key[i];
-        if (k < rows && (i == 0 || key[i - 1] != k)) atomicOr(&present[k >> 5], 1u << (k & 31));
-    }
-}
-
-// Rows without an id are zeros: present == null, every row; else the rows whose bit is not set.
-__global__ __launch_bounds__(256) void embed_zero_kernel(unsigned char* table, int64_t rows, int64_t row_bytes,
-                                                        const uint32_t* __restrict__ present) {
+// Every row that is not marked: zeros.
+__global__ __launch_bounds__(256) void embed_zero_rows_kernel(unsigned char* table, int64_t rows, int64_t row_bytes,
+                                                             const unsigned char* __restrict__ present) {
     const int lane = threadIdx.x & 63;
     const int64_t waves = (int64_t)gridDim.x * 4;
-    for (int64_t v = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); v < rows; v += waves) {
-        if (present && (present[v >> 5] >> (v & 31) & 1)) continue;
-        unsigned char* p = table + v * row_bytes;
-        const uint4 z = {0, 0, 0, 0};
-        int64_t b = (int64_t)lane * 16;
-        for (; b + 16 <= row_bytes; b += 64 * 16) __builtin_memcpy(p + b, &z, 16);
-        if (b < row_bytes)
-            for (; b < row_bytes; b += 2) *(uint16_t*)(p + b) = 0;
+    const uint4 z = {0, 0, 0, 0};
+    for (int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); w * 64 < rows; w += waves) {  // 64 rows a turn
+        unsigned long long absent = __ballot(w * 64 + lane < rows && !present[w * 64 + lane]);
+        while (absent) {
+            unsigned char* p = table + (w * 64 + __ffsll(absent) - 1) * row_bytes;
+            absent &= absent - 1;
+            int64_t b = (int64_t)lane * 16;
+            for (; b + 16 <= row_bytes; b += 64 * 16) __builtin_memcpy(p + b, &z, 16);
+            if (b < row_bytes)
+                for (; b < row_bytes; b += 2) *(uint16_t*)(p + b) = 0;
+        }
     }
+}
+// The whole table: zeros.
+__global__ __launch_bounds__(256) void embed_zero_kernel(unsigned char* table, int64_t bytes) {
+    const int64_t step = (int64_t)gridDim.x * 256 * 16;
+    const uint4 z = {0, 0, 0, 0};
+    int64_t b = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 16;
+    for (; b + 3 * step + 16 <= bytes; b += 4 * step)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) __builtin_memcpy(table + b + u * step, &z, 16);
+    for (; b + 16 <= bytes; b += step) __builtin_memcpy(table + b, &z, 16);
+    if (b < bytes)
+        for (; b < bytes; b += 2) *(uint16_t*)(table + b) = 0;
 }
 
 }  // namespace
+
+constexpr int64_t ZERO_BESIDE_BYTES = (int64_t)32 << 20;
+constexpr int ZERO_BESIDE_BLOCKS = 2;
 
 void embedding_forward(int32_t dtype, const void* table, int64_t rows, int dim, const int64_t* ids, int64_t n,
                        float scale, void* out) {
@@ -451,17 +508,17 @@ void embedding_forward(int32_t dtype, const void* table, int64_t rows, int dim, 
 
 void embedding_backward(int32_t dtype, const void* grad_out, const int64_t* ids, int64_t n, int64_t rows, int dim,
                         float scale, bool accumulate, int32_t table_dtype, void* grad_table) {
-    const int64_t row_bytes = (int64_t)dim * dtype_size(table_dtype);
-    auto zero_rows = [&](const uint32_t* present) {
-        const int64_t blocks = std::min<int64_t>((rows + 3) / 4, 16LL * device().num_cus);
+    const int64_t table_bytes = rows * dim * dtype_size(table_dtype);
+    auto zero_table = [&](int per_cu) {
+        const int64_t blocks = std::min<int64_t>((table_bytes + 4095) / 4096, (int64_t)per_cu * device().num_cus);
         RVX_LAUNCH("embedding_zero", embed_zero_kernel, dim3((unsigned)blocks), dim3(256), 0, (unsigned char*)grad_table,
-                   rows, row_bytes, present);
+                   table_bytes);
     };
     auto typed = [&](auto&& f) {  // f(T, S) of the gradient's and the table's type
         with_dtype(dtype, [&](auto t) { with_dtype(table_dtype, [&](auto s) { f(t, s); }); });
     };
     if (n <= SCAN_MAX) {
-        if (!accumulate) zero_rows(nullptr);
+        if (!accumulate) zero_table(8);
         if (n == 0) return;
         typed([&](auto t, auto s) {
             using T = decltype(t);
@@ -476,7 +533,8 @@ void embedding_backward(int32_t dtype, const void* grad_out, const int64_t* ids,
     // digits of equal width, as few as SORT_MAX_BITS allows; the key `rows` stands for absent ids
     int key_bits = 1;
     while (((int64_t)1 << key_bits) <= rows) ++key_bits;
-    const int passes = (key_bits + SORT_MAX_BITS - 1) / SORT_MAX_BITS, bits = (key_bits + passes - 1) / passes;
+    const int passes = (key_bits + SORT_MAX_BITS - 1) / SORT_MAX_BITS;
+    const int bits = std::max(2, (key_bits + passes - 1) / passes);  // at least the 4 digits of a thread
     int64_t tile = (n + SORT_TILES - 1) / SORT_TILES;
     tile = (tile + SORT_STEP - 1) / SORT_STEP * SORT_STEP;
     const int tiles = (int)((n + tile - 1) / tile);
@@ -486,57 +544,76 @@ void embedding_backward(int32_t dtype, const void* grad_out, const int64_t* ids,
     const int64_t groups = (n + GROUP - 1) / GROUP, span_count = n / (GROUP * GROUP);
     float* heads = scratch_f32("embed_partial", (2 * groups + span_count) * dim);
     float *tails = heads + groups * dim, *spans = tails + groups * dim;
+    const int64_t words = (rows + 3) / 4;
+    auto* present = accumulate ? nullptr : (uint32_t*)scratch_bytes("embed_present", words * 4);  // a byte a row
     for (int p = 0; p < passes; ++p) {
         const int in = (p + 1) & 1, out = p & 1, shift = p * bits;
         if (p == 0) {
-            RVX_LAUNCH("embedding_sort", sort_count_kernel<true>, dim3(tiles), dim3(SORT_THREADS), 0, ids,
-                       (const uint32_t*)nullptr, n, (uint32_t)rows, tile, bits, shift, counts);
+            RVX_LAUNCH("embedding_count", sort_count_kernel<true>, dim3(tiles), dim3(SORT_THREADS), 0, ids,
+                       (const uint32_t*)nullptr, n, (uint32_t)rows, tile, bits, shift, counts, present, words);
             RVX_LAUNCH("embedding_sort", sort_move_kernel<true>, dim3(tiles), dim3(SORT_THREADS), 0, ids,
                        (const uint32_t*)nullptr, (const uint32_t*)nullptr, n, (uint32_t)rows, tile, tiles, bits, shift,
                        (const uint32_t*)counts, key[out], pos[out]);
         } else {
-            RVX_LAUNCH("embedding_sort", sort_count_kernel<false>, dim3(tiles), dim3(SORT_THREADS), 0,
-                       (const int64_t*)nullptr, (const uint32_t*)key[in], n, (uint32_t)rows, tile, bits, shift, counts);
+            RVX_LAUNCH("embedding_count", sort_count_kernel<false>, dim3(tiles), dim3(SORT_THREADS), 0,
+                       (const int64_t*)nullptr, (const uint32_t*)key[in], n, (uint32_t)rows, tile, bits, shift, counts, nullptr, (int64_t)0);
             RVX_LAUNCH("embedding_sort", sort_move_kernel<false>, dim3(tiles), dim3(SORT_THREADS), 0,
                        (const int64_t*)nullptr, (const uint32_t*)key[in], (const uint32_t*)pos[in], n, (uint32_t)rows, tile,
                        tiles, bits, shift, (const uint32_t*)counts, key[out], pos[out]);
         }
     }
     const uint32_t *sk = key[(passes + 1) & 1], *sp = pos[(passes + 1) & 1];
+    // The dense gradient's zeros are written on a second stream beside the sums: the two write
+    // different rows. Small tables are not worth the events.
+    hipEvent_t zeroed = nullptr;
     if (!accumulate) {
-        const int64_t words = (rows + 31) / 32;
-        auto* present = (uint32_t*)scratch_bytes("embed_present", words * 4);
-        RVX_LAUNCH("embedding_zero", clear_bits_kernel,
-                   dim3((unsigned)std::min<int64_t>((words + 255) / 256, 4LL * device().num_cus)), dim3(256), 0, present, words);
-        RVX_LAUNCH("embedding_zero", mark_rows_kernel,
+        auto zero_rows = [&](int per_cu) {
+            const int64_t blocks = std::min<int64_t>((rows + 255) / 256, (int64_t)per_cu * device().num_cus);
+            RVX_LAUNCH("embedding_zero", embed_zero_rows_kernel, dim3((unsigned)blocks), dim3(256), 0,
+                       (unsigned char*)grad_table, rows, table_bytes / rows, (const unsigned char*)present);
+        };
+        RVX_LAUNCH("embedding_mark", embed_mark_kernel,
                    dim3((unsigned)std::min<int64_t>((n + 255) / 256, 4LL * device().num_cus)), dim3(256), 0, sk, n,
-                   (uint32_t)rows, present);
-        zero_rows(present);
+                   (uint32_t)rows, (unsigned char*)present);
+        if (table_bytes >= ZERO_BESIDE_BYTES) {
+            hipEvent_t* ev = pipeline_events(2);
+            RVX_HIP(hipEventRecord(ev[0], stream()));
+            RVX_HIP(hipStreamWaitEvent(device().aux, ev[0], 0));
+            StreamScope on(device().aux);
+            zero_rows(ZERO_BESIDE_BLOCKS);
+            zeroed = ev[1];
+            RVX_HIP(hipEventRecord(zeroed, device().aux));
+        } else {
+            zero_rows(8);
+        }
     }
     typed([&](auto t, auto s) {
         using T = decltype(t);
         using S = decltype(s);
         constexpr int N = Vec16<T>::N;
         const int vecs = (dim + 64 * N - 1) / (64 * N);  // vectors a lane for a whole row
-        RVX_LAUNCH("embedding_groups", embed_groups_kernel<T>, dim3((unsigned)((groups + 3) / 4), vecs), dim3(256), 0,
-                   (const T*)grad_out, dim, sk, sp, n, groups, (uint32_t)rows, heads, tails);
+        RVX_LAUNCH("embedding_groups", embed_groups_kernel<T>, dim3((unsigned)groups, vecs), dim3(64), 0, (const T*)grad_out,
+                   dim, sk, sp, n, (uint32_t)rows, heads, tails);
         if (span_count > 1)
-            RVX_LAUNCH("embedding_groups", embed_spans_kernel, dim3((unsigned)((span_count + 3) / 4), (dim + 255) / 256),
+            RVX_LAUNCH("embedding_long", embed_spans_kernel, dim3((unsigned)((span_count + 3) / 4), (dim + 255) / 256),
                        dim3(256), 0, (const float*)tails, dim, sk, span_count, (uint32_t)rows, spans);
+        RVX_LAUNCH("embedding_long", (embed_long_kernel<T, S>), dim3((unsigned)groups, vecs), dim3(64), 0, dim, sk, sp, n,
+                   (uint32_t)rows, (const float*)heads, (const float*)tails, (const float*)spans, scale, accumulate,
+                   (S*)grad_table);
         const int slabs = (vecs + 3) / 4, per = (vecs + slabs - 1) / slabs;
         auto go = [&](auto v) {
             constexpr int64_t SLICE = (int64_t)1 << 24;  // entries of one launch: at most 2^30 threads
             for (int64_t i = 0; i < n; i += SLICE)
                 RVX_LAUNCH("embedding_backward", (embed_rows_kernel<T, S, decltype(v)::value>),
                            dim3((unsigned)((std::min(SLICE, n - i) + 3) / 4), slabs), dim3(256), 0, (const T*)grad_out, dim, i,
-                           sk, sp, n, (uint32_t)rows, (const float*)heads, (const float*)tails, (const float*)spans, scale,
-                           accumulate, (S*)grad_table);
+                           sk, sp, n, (uint32_t)rows, scale, accumulate, (S*)grad_table);
         };
         if (per == 1) go(std::integral_constant<int, 1>{});
         else if (per == 2) go(std::integral_constant<int, 2>{});
         else if (per == 3) go(std::integral_constant<int, 3>{});
         else go(std::integral_constant<int, 4>{});
     });
+    if (zeroed) RVX_HIP(hipStreamWaitEvent(stream(), zeroed, 0));
 }
 
 }  // namespace rvx

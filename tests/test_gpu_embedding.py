@@ -90,7 +90,7 @@ def test_gradient(dtype, table_dtype, rows, dim, n, kind, accumulate):
     assert torch.equal(got.view(torch.uint8), again.view(torch.uint8))
 
 
-@pytest.mark.parametrize("length", [1, 2, 61, 62, 63, 64, 65, 126, 127, 128, 129, 4096, 4097, 8500])
+@pytest.mark.parametrize("length", [1, 2, 57, 58, 59, 61, 62, 63, 64, 65, 126, 127, 128, 129, 4096, 4097, 8500])
 @pytest.mark.parametrize("before", [0, 1, 2, 62, 63, 64])
 def test_gradient_runs_at_every_edge(length, before):
     """A run of one id that starts `before` entries into the sorted order, between runs of others."""
