@@ -17,19 +17,25 @@ struct AdapterSlot {  // one entry of the device table; rank 0 = no adapter
 struct AdapterShape {
     int32_t dtype, in, out, slots;
     int32_t kt;   // fragments along in, an even number
-    int32_t nt;   // 16-row tiles along out
+    int32_t nt;   // 16-row tiles along out, an even number
     int32_t rt;   // 16-row tiles along the rank (rows of A)
     int32_t rk;   // fragments along the rank (columns of B)
     int64_t a_slot, b_slot;  // elements of one adapter's A and B
 };
 AdapterShape adapter_shape(int32_t dtype, int32_t in, int32_t out, int32_t max_rank, int32_t slots);
 
-// src [rows][cols] row-major to fragments [ceil(rows / 16) = tiles][frags][64 lanes][16 bytes], zero padded
-void adapter_pack(int32_t dtype, const void* src, int rows, int cols, int tiles, int frags, void* dst);
+// src [rows][cols] row-major to fragments [tiles][frags][64 lanes][16 bytes], zero padded; outputs: the
+// rows are outputs (W, B), interleaved over pairs of tiles
+void adapter_pack(int32_t dtype, const void* src, int rows, int cols, int tiles, int frags, bool outputs, void* dst);
+// f32 layers: W as the split-f16 planes of the framework's GEMM (bytes; planes and column scales from w)
+int64_t adapter_split_bytes(const AdapterShape& s);
+void adapter_split(const AdapterShape& s, const float* w, void* planes, float* inv);
 
 struct AdapterArgs {
     AdapterShape s;
     const void *w, *bias, *a, *b;  // bias nullable
+    const void* w_split;           // f32: split-f16 planes of W and their scales (nullable)
+    const float* w_inv;
     const AdapterSlot* slot;
     const void* x;
     const int32_t* ids;  // nullable: no adapters
@@ -44,6 +50,6 @@ struct rvx_adapter_linear {
     rvx::AdapterShape s;
     int32_t max_rank = 0;
     int device = 0;
-    rvx::DevMem w, bias, a, b, slot;
+    rvx::DevMem w, bias, a, b, slot, split, split_inv;
     std::vector<rvx::AdapterSlot> host_slot;
 };

@@ -40,7 +40,12 @@ rvx_status rvx_adapter_linear_create(const rvx_adapter_linear_config* cfg, const
         l->device = device().id;
         const AdapterShape& s = l->s;
         l->w.reset((int64_t)s.nt * s.kt * 1024);
-        adapter_pack(s.dtype, weight->mem.p, s.out, s.in, s.nt, s.kt, l->w.p);
+        adapter_pack(s.dtype, weight->mem.p, s.out, s.in, s.nt, s.kt, true, l->w.p);
+        if (const int64_t bytes = adapter_split_bytes(s)) {
+            l->split.reset(bytes);
+            l->split_inv.reset((int64_t)s.out * 4);
+            adapter_split(s, weight->mem.as<float>(), l->split.p, l->split_inv.as<float>());
+        }
         if (bias) {
             l->bias.reset((int64_t)s.out * size);
             RVX_HIP(hipMemcpyAsync(l->bias.p, bias->mem.p, (size_t)s.out * size, hipMemcpyDeviceToDevice, stream()));
@@ -78,8 +83,8 @@ rvx_status rvx_adapter_linear_set(rvx_adapter_linear* l, int32_t slot, int32_t r
         }
         ComputeLock cl;
         if (rank) {
-            adapter_pack(s.dtype, a->mem.p, rank, s.in, s.rt, s.kt, (char*)l->a.p + slot * s.a_slot * size);
-            adapter_pack(s.dtype, b->mem.p, s.out, rank, s.nt, s.rk, (char*)l->b.p + slot * s.b_slot * size);
+            adapter_pack(s.dtype, a->mem.p, rank, s.in, s.rt, s.kt, false, (char*)l->a.p + slot * s.a_slot * size);
+            adapter_pack(s.dtype, b->mem.p, s.out, rank, s.nt, s.rk, true, (char*)l->b.p + slot * s.b_slot * size);
         }
         l->host_slot[slot] = AdapterSlot{scale, rank};
         l->slot.upload(&l->host_slot[slot], sizeof(AdapterSlot), (int64_t)slot * sizeof(AdapterSlot));  // waits
@@ -100,7 +105,7 @@ rvx_status rvx_adapter_linear_forward_device(const rvx_adapter_linear* l, const 
         check_apart(adapter_ids, y, "adapter_ids and y");
         if (n == 0) return;
         ComputeLock cl;
-        AdapterArgs g{s, l->w.p, l->bias.p, l->a.p, l->b.p, l->slot.as<AdapterSlot>(), x->mem.p,
+        AdapterArgs g{s, l->w.p, l->bias.p, l->a.p, l->b.p, l->split.p, l->split_inv.as<float>(), l->slot.as<AdapterSlot>(), x->mem.p,
                       adapter_ids && s.slots ? adapter_ids->mem.as<int32_t>() : nullptr, y->mem.p, n};
         adapter_forward(g);
     });

@@ -1,15 +1,18 @@
 // k_adapter.hip — y_i = W x_i + bias + s_r B_r (A_r x_i) with r = ids[i], the adapter of row i.
 //
-// Two launches: t_i = s_r A_r x_i for every row (f32, n x rank), then the projection whose
-// epilogue adds B_r t_i. Rows may come in any order of adapters: each 16-row tile goes over the
-// different adapters among its rows, so rows of one request cost one turn and a tile of 16
-// requests reads 16 adapters, which are all needed.
+// t_i = s_r A_r x_i for every row is a launch of its own; the projection adds B_r t_i behind its
+// sum. Rows may come in any order of adapters. For more than a few rows they are first grouped: the
+// kernels then go through a permutation of the rows, in which a 16-row tile holds one adapter or
+// two, and take one turn for each. The products of a row do not depend on its place.
 //
 // Weights lie in fragment order: the 16 rows x 64 bytes that one matrix instruction takes from
 // one operand are 1 KiB, lane l's 16 bytes at l * 16 (row l % 16, elements (l / 16) * N ..). A
 // wave loads a fragment with one coalesced instruction, copies it to LDS as it is, and reads it
-// back without bank conflicts.
+// back without bank conflicts. W and B are the first operand, x and t the second, so that a lane
+// holds 4 outputs of one row; the 32 outputs of two neighbouring fragments are interleaved by 4
+// (`out_of`), so that the two give it 8 neighbouring outputs.
 #include "adapter.hpp"
+#include "kernels.hpp"
 
 namespace rvx {
 namespace {
@@ -54,15 +57,20 @@ __device__ __forceinline__ typename Mma<T>::V load_piece(const T* p) {
 }
 
 // ---------------------------------------------------------------- layout
+// the output in row m of fragment tile nt
+__host__ __device__ __forceinline__ int out_of(int nt, int m) {
+    return (nt >> 1) * 32 + (m >> 2) * 8 + (nt & 1) * 4 + (m & 3);
+}
+
 template <class T>
 __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ src, int rows, int cols, int64_t pieces,
-                                                  int frags, T* __restrict__ dst) {
+                                                  int frags, bool outputs, T* __restrict__ dst) {
     constexpr int N = PIECE<T>;
     const int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (p >= pieces) return;
     const int lane = (int)(p & 63);
     const int64_t f = p >> 6;
-    const int row = (int)(f / frags) * 16 + (lane & 15);
+    const int tile = (int)(f / frags), row = outputs ? out_of(tile, lane & 15) : tile * 16 + (lane & 15);
     const int col = (int)(f % frags) * DEPTH<T> + (lane >> 4) * N;
     T v[N];
 #pragma unroll
@@ -87,29 +95,95 @@ __device__ __forceinline__ int adapter_of(const int32_t* ids, const AdapterSlot*
     return id >= 0 && id < slots && slot[id].rank > 0 ? id : -1;
 }
 
-// ---------------------------------------------------------------- t = s A x
-constexpr int SH_WAVES = 8;
+// ---------------------------------------------------------------- grouping rows
+// perm: the rows in the order of their adapters (adapters that agree modulo GROUP_BINS - 1 may mix:
+// the order is for speed alone). One block: it is a small part of what follows.
+constexpr int GROUP_THREADS = 1024, GROUP_BITS = 9, GROUP_BINS = 1 << GROUP_BITS;
 
-// A block: 16 * SM rows, the waves split the sum over `in`. The block's y-th, (y + gridDim.y)-th
-// .. different adapter is its work.
-template <class T, int SM, int RT>
-__global__ __launch_bounds__(64 * SH_WAVES) void shrink_kernel(const T* __restrict__ x, int ldx, int64_t n,
-                                                              const T* __restrict__ a, int64_t a_slot, int kt,
-                                                              const int32_t* __restrict__ ids,
-                                                              const AdapterSlot* __restrict__ slot, int slots,
-                                                              float* __restrict__ t, int ldt) {
+__global__ __launch_bounds__(GROUP_THREADS) void group_rows_kernel(const int32_t* __restrict__ ids, int64_t n,
+                                                                  const AdapterSlot* __restrict__ slot, int slots,
+                                                                  int32_t* __restrict__ perm) {
+    __shared__ int next[GROUP_BINS];
+    __shared__ int sums[GROUP_BINS / 64];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    auto bin_of = [&](int64_t row) {
+        const int id = adapter_of(ids, slot, slots, row, n);
+        return id < 0 ? 0 : 1 + id % (GROUP_BINS - 1);
+    };
+    // the wave's lanes with the same bin: the first of them takes places for all
+    auto places = [&](int bin, bool there) {
+        unsigned long long same = __ballot(there);
+#pragma unroll
+        for (int b = 0; b < GROUP_BITS; ++b) {
+            const unsigned long long m = __ballot(bin >> b & 1);
+            same &= bin >> b & 1 ? m : ~m;
+        }
+        const int before = __popcll(same & ((1ull << lane) - 1));
+        int at = 0;
+        if (there && before == 0) at = atomicAdd(&next[bin], __popcll(same));
+        return __shfl(at, there ? __ffsll(same) - 1 : lane) + before;
+    };
+    for (int b = t; b < GROUP_BINS; b += GROUP_THREADS) next[b] = 0;
+    __syncthreads();
+    for (int64_t i = t; i - lane < n; i += GROUP_THREADS) places(bin_of(i), i < n);
+    __syncthreads();
+    int v = 0, scan = 0;
+    if (t < GROUP_BINS) {
+        v = scan = next[t];
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int u = __shfl_up(scan, o);
+            scan += lane >= o ? u : 0;
+        }
+        if (lane == 63) sums[wave] = scan;
+    }
+    __syncthreads();
+    if (t < GROUP_BINS) {
+        int from = scan - v;
+        for (int w = 0; w < wave; ++w) from += sums[w];
+        next[t] = from;
+    }
+    __syncthreads();
+    for (int64_t i = t; i - lane < n; i += GROUP_THREADS) {
+        const int at = places(bin_of(i), i < n);
+        if (i < n) perm[at] = (int32_t)i;
+    }
+}
+
+// ---------------------------------------------------------------- t = s A x
+// What the projection reads of t. Few rows: f32, `f`. Tiles: pieces of T, hi + lo, 16 (bf16) or 22
+// (f16) bits of each value, so that t's rounding is far below y's (f32: hi alone); f16: a row whose
+// largest value is not in [2^-3, 2^15) is scaled by a power of two to [2^14, 2^15), undone by `back`.
+template <class T>
+struct Mid {
+    float* f;
+    T *hi, *lo;
+    float* back;
+    int ld;
+};
+
+// A block: 16 * SM rows (of the permutation), the waves split the sum over `in`. The block's y-th,
+// (y + gridDim.y)-th .. different adapter is its work.
+template <class T, int SM, int RT, int WAVES, bool SPLIT>
+__global__ __launch_bounds__(64 * WAVES) void shrink_kernel(const T* __restrict__ x, int ldx, int64_t n,
+                                                           const int32_t* __restrict__ perm, const T* __restrict__ a,
+                                                           int64_t a_slot, int kt, const int32_t* __restrict__ ids,
+                                                           const AdapterSlot* __restrict__ slot, int slots, Mid<T> t) {
     using V = typename Mma<T>::V;
     constexpr int N = PIECE<T>;
-    __shared__ f32x4 red[SH_WAVES][SM * RT][64];
+    __shared__ f32x4 red[WAVES][SM * RT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t row0 = (int64_t)blockIdx.x * (16 * SM);
-    const int mine = lane < 16 * SM ? adapter_of(ids, slot, slots, row0 + lane, n) : -1;
+    const int64_t place = min(row0 + (lane & (16 * SM - 1)), n - 1);
+    const int64_t my_row = SPLIT ? perm[place] : place;
+    const int mine = lane < 16 * SM && row0 + lane < n ? adapter_of(ids, slot, slots, my_row, n) : -1;
     unsigned long long todo = __ballot(mine >= 0);
+    if (!todo) return;
     const T* xp[SM];
 #pragma unroll
     for (int m = 0; m < SM; ++m)
-        xp[m] = x + min(row0 + m * 16 + (lane & 15), n - 1) * ldx + (lane >> 4) * N;
-    const int per = (kt + SH_WAVES - 1) / SH_WAVES, k0 = min(kt, wave * per), k1 = min(kt, k0 + per);
+        xp[m] = x + (int64_t)__shfl((int)my_row, m * 16 + (lane & 15)) * ldx + (lane >> 4) * N;
+    const int per = (kt + WAVES - 1) / WAVES, k0 = min(kt, wave * per), k1 = min(kt, k0 + per);
     for (int turn = 0; todo; ++turn) {
         const int id = __builtin_amdgcn_readlane(mine, __ffsll(todo) - 1);
         todo &= ~__ballot(mine == id);
@@ -125,7 +199,7 @@ __global__ __launch_bounds__(64 * SH_WAVES) void shrink_kernel(const T* __restri
             for (int r = 0; r < RT; ++r) {
                 const V av = load_piece(ap + ((int64_t)r * kt + k) * (64 * N));
 #pragma unroll
-                for (int m = 0; m < SM; ++m) acc[m][r] = Mma<T>::run(xv[m], av, acc[m][r]);
+                for (int m = 0; m < SM; ++m) acc[m][r] = Mma<T>::run(av, xv[m], acc[m][r]);
             }
         }
 #pragma unroll
@@ -134,16 +208,55 @@ __global__ __launch_bounds__(64 * SH_WAVES) void shrink_kernel(const T* __restri
             for (int r = 0; r < RT; ++r) red[wave][m * RT + r][lane] = acc[m][r];
         __syncthreads();
         const AdapterSlot info = slot[id];
-        for (int i = wave; i < SM * RT; i += SH_WAVES) {
-            f32x4 s = red[0][i][lane];
+        // a wave a 16-row tile: lane l has ranks r * 16 + (l / 16) * 4 .. of row l % 16
+        for (int m = wave; m < SM; m += WAVES) {
+            float v[RT][4], most = 0.0f;
 #pragma unroll
-            for (int w = 1; w < SH_WAVES; ++w) s += red[w][i][lane];
-            const int m = i / RT, r = i - m * RT;
+            for (int r = 0; r < RT; ++r) {
+                f32x4 sum = red[0][m * RT + r][lane];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int64_t row = row0 + m * 16 + (lane >> 4) * 4 + j;
-                const int c = r * 16 + (lane & 15);  // past the adapter's rank: zeros, whatever x holds
-                if (adapter_of(ids, slot, slots, row, n) == id) t[row * ldt + c] = c < info.rank ? s[j] * info.scale : 0.0f;
+                for (int w = 1; w < WAVES; ++w) sum += red[w][m * RT + r][lane];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    // past the adapter's rank: zeros, whatever x holds
+                    v[r][j] = r * 16 + (lane >> 4) * 4 + j < info.rank ? sum[j] * info.scale : 0.0f;
+                    most = fmaxf(most, fabsf(v[r][j]));
+                }
+            }
+            float up = 1.0f, down = 1.0f;
+            if constexpr (SPLIT && __is_same(T, _Float16)) {
+                most = fmaxf(most, __shfl_xor(most, 16));
+                most = fmaxf(most, __shfl_xor(most, 32));
+                if (most > 0.0f && most < INFINITY && !(most >= 0.125f && most < 32768.0f)) {
+                    const int e = min(126, max(-126, 14 - ilogbf(most)));
+                    up = ldexpf(1.0f, e), down = ldexpf(1.0f, -e);
+                }
+            }
+            const int64_t at = row0 + m * 16 + (lane & 15);  // the place in the permutation
+            if (__shfl(mine, m * 16 + (lane & 15)) != id) continue;
+            if constexpr (!SPLIT) {
+#pragma unroll
+                for (int r = 0; r < RT; ++r) __builtin_memcpy(t.f + at * t.ld + r * 16 + (lane >> 4) * 4, v[r], 16);
+            } else {
+                if (t.back && lane < 16) t.back[at] = down;
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    T hi[4], lo[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        hi[j] = (T)(v[r][j] * up);
+                        lo[j] = (T)(v[r][j] * up - (float)hi[j]);
+                    }
+                    const int64_t o = at * t.ld + r * 16 + (lane >> 4) * 4;
+                    __builtin_memcpy(t.hi + o, hi, sizeof(hi));
+                    if (sizeof(T) == 2) __builtin_memcpy(t.lo + o, lo, sizeof(lo));
+                }
+                if (RT == 1 && t.ld > 16) {  // a fragment is 32 ranks deep
+                    const int64_t o = at * t.ld + 16 + (lane >> 4) * 4;
+                    const T zero[4] = {};
+                    __builtin_memcpy(t.hi + o, zero, sizeof(zero));
+                    __builtin_memcpy(t.lo + o, zero, sizeof(zero));
+                }
             }
         }
         __syncthreads();
@@ -151,9 +264,9 @@ __global__ __launch_bounds__(64 * SH_WAVES) void shrink_kernel(const T* __restri
 }
 
 // ---------------------------------------------------------------- few rows
-// A block: 16 columns of y for all (<= 16 MT) rows; its waves split the sum and join in LDS. Bound
-// by reading W once.
-constexpr int FEW_WAVES = 8;
+// A block: a fragment tile's 16 outputs for all (<= 16 MT) rows; its waves split the sum and join in
+// LDS. Bound by reading W once.
+constexpr int FEW_WAVES = 16;
 
 template <class T, int MT>
 __global__ __launch_bounds__(64 * FEW_WAVES) void few_rows_kernel(const T* __restrict__ x, int ldx, int n,
@@ -169,74 +282,98 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_rows_kernel(const T* __res
     __shared__ f32x4 red[FEW_WAVES][MT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int nt = blockIdx.x;
+    // this thread's output: o = (row tile, row, output), one each (16 rows: of the first 256 threads)
+    const int o = threadIdx.x, row = o >> 4, c = o & 15, col = out_of(nt, c);
+    const bool there = o < MT * 256 && row < n && col < out;
+    const int id = there ? adapter_of(ids, slot, slots, row, n) : -1;
+    const int rank = id >= 0 ? slot[id].rank : 0;
     const int per = (kt + FEW_WAVES - 1) / FEW_WAVES, k0 = min(kt, wave * per), k1 = min(kt, k0 + per);
     const T* wp = w + (int64_t)nt * kt * (64 * N) + lane * N;
     const T* xp[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) xp[m] = x + (int64_t)min(m * 16 + (lane & 15), n - 1) * ldx + (lane >> 4) * N;
     f32x4 acc[MT] = {};
-#pragma unroll 4
-    for (int k = k0; k < k1; ++k) {
+    constexpr int U = MT == 4 ? 4 : 8;  // loads in flight, by registers
+    int k = k0;
+    for (; k + U <= k1; k += U) {
+        V wv[U], xv[U][MT];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            wv[u] = load_piece(wp + (int64_t)(k + u) * (64 * N));
+#pragma unroll
+            for (int m = 0; m < MT; ++m) xv[u][m] = load_piece(xp[m] + (k + u) * DEPTH<T>);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) acc[m] = Mma<T>::run(wv[u], xv[u][m], acc[m]);
+    }
+#pragma unroll 2
+    for (; k < k1; ++k) {
         const V wv = load_piece(wp + (int64_t)k * (64 * N));
 #pragma unroll
-        for (int m = 0; m < MT; ++m) acc[m] = Mma<T>::run(load_piece(xp[m] + k * DEPTH<T>), wv, acc[m]);
+        for (int m = 0; m < MT; ++m) acc[m] = Mma<T>::run(wv, load_piece(xp[m] + k * DEPTH<T>), acc[m]);
     }
 #pragma unroll
     for (int m = 0; m < MT; ++m) red[wave][m][lane] = acc[m];
-    __syncthreads();
-    for (int o = threadIdx.x; o < MT * 256; o += 64 * FEW_WAVES) {
-        const int m = o >> 8, row = m * 16 + (o >> 4 & 15), c = o & 15, col = nt * 16 + c;
-        if (row >= n || col >= out) continue;
-        float v = 0.0f;
+    // B's row of this output: the piece of ranks p N .. is lane (p % 4) * 16 + c of fragment p / 4
+    float d = 0.0f;
+    if (id >= 0) {
+        const T* bp = b + id * b_slot + (int64_t)nt * rk * (64 * N) + c * N;
+        const float* tp = t + (int64_t)row * ldt;
+        for (int p = 0; p * N < rank; ++p) {
+            const V bv = load_piece(bp + ((p >> 2) * 64 + (p & 3) * 16) * N);
 #pragma unroll
-        for (int q = 0; q < FEW_WAVES; ++q) v += red[q][m][(o >> 6 & 3) * 16 + c][o >> 4 & 3];
-        const int id = adapter_of(ids, slot, slots, row, n);
-        if (id >= 0) {
-            // B's row `col`: the piece of ranks 8 p .. (f32: 4 p ..) is lane (p % 4) * 16 + c of fragment p / 4
-            const T* bp = b + id * b_slot + (int64_t)nt * rk * (64 * N) + c * N;
-            const float* tp = t + (int64_t)row * ldt;
-            const int pieces = (slot[id].rank + N - 1) / N;
-            float d = 0.0f;
-            for (int p = 0; p < pieces; ++p) {
-                const V bv = load_piece(bp + ((p >> 2) * 64 + (p & 3) * 16) * N);
-#pragma unroll
-                for (int j = 0; j < N; ++j) d = fmaf(tp[p * N + j], (float)bv[j], d);
-            }
-            v += d;
+            for (int j = 0; j < N; ++j) d = fmaf(tp[p * N + j], (float)bv[j], d);
         }
-        if (bias) v += (float)bias[col];
-        y[(int64_t)row * out + col] = (T)v;
     }
+    __syncthreads();
+    if (!there) return;
+    float v = 0.0f;
+#pragma unroll
+    for (int q = 0; q < FEW_WAVES; ++q) v += red[q][row >> 4][(c >> 2) * 16 + (row & 15)][c & 3];
+    v += d;
+    if (bias) v += (float)bias[col];
+    y[(int64_t)row * out + col] = (T)v;
 }
 
 // ---------------------------------------------------------------- many rows
-// The epilogue takes t's rows as fragments of T, hi + lo: 16 (bf16) or 22 (f16) bits of each
-// value, so that t's rounding is far below y's. f16: the row is first scaled by a power of two
-// to below 2^15 (t may be larger than f16 holds); `back` undoes it.
-template <class T, int BM, int BN, int WM, int WN>
+// A block: BM rows (of the permutation) x BN outputs; WM x WN waves; the sum in stages of 2 fragments,
+// NS of which are in LDS or on their way to it (copied there without registers). A stage's second half
+// is read while the first is multiplied, the next stage's first half while the second is; the one
+// barrier of a stage lies between: behind it everybody has read this stage, and has the next.
+template <int BM, int BN, int WM, int WN, int NS>
 struct TileCfg {
     static constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
-    static constexpr int FRAGS = (BM + BN) / 16 * 2;  // 1-KiB pieces of a stage: 2 fragments deep
-    static constexpr int STAGE = FRAGS * 1024;
-    static_assert(FRAGS % WAVES == 0);
+    static constexpr int XF = BM / 16 * 2, WF = BN / 16 * 2;  // 1-KiB fragments of a stage
+    static constexpr int XP = XF / WAVES, WP = WF / WAVES;    // copied by each wave
+    static constexpr int STAGE = (XF + WF) * 1024;
+    static_assert(XF % WAVES == 0 && WF % WAVES == 0 && TN % 2 == 0);
 };
 
-template <class T, int BM, int BN, int WM, int WN>
+// Vm: at most that many of this wave's copies are still on their way
+template <int Vm>
+__device__ __forceinline__ void wait_and_meet() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(Vm) : "memory");
+}
+
+// ADD: y is there already (f32), the adapters' part is added to it.
+template <class T, int BM, int BN, int WM, int WN, int NS, bool ADD>
 __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const T* __restrict__ x, int ldx, int64_t n,
                                                            const T* __restrict__ w, int kt, int nts,
                                                            const T* __restrict__ bias, const T* __restrict__ b,
                                                            int64_t b_slot, int rk, const int32_t* __restrict__ ids,
-                                                           const AdapterSlot* __restrict__ slot, int slots,
-                                                           const float* __restrict__ t, int ldt, int tw, int out,
-                                                           int tiles_m, int tiles_n, T* __restrict__ y) {
-    using Cf = TileCfg<T, BM, BN, WM, WN>;
+                                                           const int32_t* __restrict__ perm,
+                                                           const AdapterSlot* __restrict__ slot, int slots, Mid<T> t,
+                                                           int out, int tiles_m, int tiles_n, T* y) {
+    using Cf = TileCfg<BM, BN, WM, WN, NS>;
     using V = typename Mma<T>::V;
-    constexpr int N = PIECE<T>, TM = Cf::TM, TN = Cf::TN, PER = Cf::FRAGS / Cf::WAVES, A_FRAGS = BM / 16 * 2;
-    __shared__ __align__(16) unsigned char lds[2 * Cf::STAGE];
+    constexpr int N = PIECE<T>, TM = Cf::TM, TN = Cf::TN;
+    __shared__ __align__(16) unsigned char lds[ADD ? 16 : NS * Cf::STAGE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave - wm * WN;
-    // Blocks go to the 8 XCDs in turn: block i of XCD d is tile (d, i) of a cut into 8 parts, so
-    // that an L2 serves neighbouring tiles.
+    // Blocks go to the 8 XCDs in turn: block i of XCD d is the i-th tile of the d-th part, so that an
+    // L2 serves neighbouring tiles; in this order 8 tiles of rows share each tile of outputs.
     const int total = tiles_m * tiles_n;
     int tile = blockIdx.x;
     {
@@ -244,124 +381,152 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const T* __restrict_
         const int full = total - (part - 1) * 8;  // parts of the larger size
         tile = d < full ? d * part + i : full * part + (d - full) * (part - 1) + i;
     }
-    const int tm = tile / tiles_n, tn = tile - tm * tiles_n;
+    const int band = tile / (8 * tiles_n), in_band = tile - band * 8 * tiles_n, rows_of_band = min(8, tiles_m - band * 8);
+    const int tn = in_band / rows_of_band, tm = band * 8 + (in_band - tn * rows_of_band);
     const int64_t row0 = (int64_t)tm * BM;
-    const int nt0 = tn * (BN / 16);
-
-    // this wave's pieces of a stage: fragments f = wave * PER + j; first those of x, then W's
-    const T* src[PER];
-    int step[PER];
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        const int f = wave * PER + j;
-        if (f < A_FRAGS) {
-            const int64_t row = min(row0 + (f >> 1) * 16 + (lane & 15), n - 1);
-            src[j] = x + row * ldx + (f & 1) * DEPTH<T> + (lane >> 4) * N;
-            step[j] = 2 * DEPTH<T>;
-        } else {
-            const int g = f - A_FRAGS;
-            const int nt = min(nt0 + (g >> 1), nts - 1);
-            src[j] = w + ((int64_t)nt * kt + (g & 1)) * (64 * N) + lane * N;
-            step[j] = 2 * 64 * N;
-        }
-    }
-    auto fill = [&](int s, int buf) {
-#pragma unroll
-        for (int j = 0; j < PER; ++j)
-            __builtin_amdgcn_global_load_lds(
-                (const void*)(src[j] + (int64_t)s * step[j]),
-                (__attribute__((address_space(3))) void*)(lds + buf * Cf::STAGE + (wave * PER + j) * 1024), 16, 0, 0);
+    const int nt0 = tn * (BN / 16), ntw = nt0 + wn * TN;
+    auto row_at = [&](int64_t place) -> int64_t {
+        const int64_t p = min(place, n - 1);
+        return perm ? perm[p] : p;
     };
-    f32x4 acc[TM][TN] = {};
-    const int stages = kt / 2;
-    fill(0, 0);
-    for (int s = 0; s < stages; ++s) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();  // stage s is there, and everybody has read stage s - 1
-        if (s + 1 < stages) fill(s + 1, (s + 1) & 1);
-        const unsigned char* base = lds + (s & 1) * Cf::STAGE;
+    f32x4 acc[TM][TN];
+    if constexpr (!ADD) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            V av[TM], bv[TN];
+        for (int i = 0; i < TM; ++i)
 #pragma unroll
-            for (int i = 0; i < TM; ++i) av[i] = *(const V*)(base + ((wm * TM + i) * 2 + h) * 1024 + lane * 16);
+            for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+        const T* xs[Cf::XP];
+        const T* ws[Cf::WP];
 #pragma unroll
-            for (int i = 0; i < TN; ++i) bv[i] = *(const V*)(base + (A_FRAGS + (wn * TN + i) * 2 + h) * 1024 + lane * 16);
+        for (int j = 0; j < Cf::XP; ++j) {
+            const int f = wave * Cf::XP + j;
+            xs[j] = x + row_at(row0 + (f >> 1) * 16 + (lane & 15)) * ldx + (f & 1) * DEPTH<T> + (lane >> 4) * N;
+        }
+#pragma unroll
+        for (int j = 0; j < Cf::WP; ++j) {
+            const int f = wave * Cf::WP + j;
+            ws[j] = w + ((int64_t)min(nt0 + (f >> 1), nts - 1) * kt + (f & 1)) * (64 * N);
+        }
+        auto fill = [&](int s, int buf) {
+            unsigned char* base = lds + buf * Cf::STAGE;
+#pragma unroll
+            for (int j = 0; j < Cf::XP; ++j)
+                __builtin_amdgcn_global_load_lds(
+                    (const void*)(xs[j] + s * (2 * DEPTH<T>)),
+                    (__attribute__((address_space(3))) void*)(base + (wave * Cf::XP + j) * 1024), 16, 0, 0);
+#pragma unroll
+            for (int j = 0; j < Cf::WP; ++j)
+                __builtin_amdgcn_global_load_lds(
+                    (const void*)(ws[j] + (int64_t)s * (2 * 64 * N) + lane * N),
+                    (__attribute__((address_space(3))) void*)(base + (Cf::XF + wave * Cf::WP + j) * 1024), 16, 0, 0);
+        };
+        V xv[2][TM], wv[2][TN];
+        auto read = [&](int h, int buf) {
+            const unsigned char* base = lds + buf * Cf::STAGE + lane * 16;
+#pragma unroll
+            for (int j = 0; j < TN; ++j) wv[h][j] = *(const V*)(base + (Cf::XF + (wn * TN + j) * 2 + h) * 1024);
+#pragma unroll
+            for (int i = 0; i < TM; ++i) xv[h][i] = *(const V*)(base + ((wm * TM + i) * 2 + h) * 1024);
+        };
+        auto multiply = [&](int h) {
 #pragma unroll
             for (int i = 0; i < TM; ++i)
 #pragma unroll
-                for (int j = 0; j < TN; ++j) acc[i][j] = Mma<T>::run(av[i], bv[j], acc[i][j]);
+                for (int j = 0; j < TN; ++j) acc[i][j] = Mma<T>::run(wv[h][j], xv[h][i], acc[i][j]);
+        };
+        const int stages = kt / 2;
+        for (int s = 0; s < NS - 1 && s < stages; ++s) fill(s, s);
+        wait_and_meet<0>();
+        if (NS - 1 < stages) fill(NS - 1, NS - 1);
+        read(0, 0);
+        int buf = 0;
+        for (int s = 0; s < stages; ++s) {
+            const int next = buf + 1 == NS ? 0 : buf + 1;
+            read(1, buf);
+            multiply(0);
+            // behind the copies of stages s + 2 .. s + NS - 1, where they were begun
+            if (s + NS - 1 < stages) wait_and_meet<(NS - 2) * (Cf::XP + Cf::WP)>();
+            else wait_and_meet<0>();
+            if (s + NS < stages) fill(s + NS, buf);
+            if (s + 1 < stages) read(0, next);
+            multiply(1);
+            buf = next;
         }
     }
 
-    const int ntw = nt0 + wn * TN;
+    // y's pieces: lane l has outputs out_of(ntw + j, (l / 16) * 4 + r) of row l % 16 of tile i
+    int64_t row[TM];
+    int who[TM];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+        const int64_t place = row0 + (wm * TM + i) * 16 + (lane & 15);
+        row[i] = row_at(place);
+        who[i] = place < n ? adapter_of(ids, slot, slots, row[i], n) : -1;
+        if (place >= n) row[i] = -1;
+    }
+    const int col0 = ntw * 16 + (lane >> 4) * 8;  // of the pair j, j + 1: col0 + j * 16 ..
+    if constexpr (ADD) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int col = col0 + (j >> 1) * 32 + (j & 1) * 4 + r;
+                    acc[i][j][r] = row[i] >= 0 && col < out ? (float)y[row[i] * out + col] : 0.0f;
+                }
+    }
     if (ids) {
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
-            const int64_t r0 = row0 + (wm * TM + i) * 16;
-            const int mine = lane < 16 ? adapter_of(ids, slot, slots, r0 + lane, n) : -1;
-            unsigned long long todo = __ballot(mine >= 0);
-            int at[4];  // the adapters of this lane's four rows of C
-#pragma unroll
-            for (int r = 0; r < 4; ++r) at[r] = __shfl(mine, (lane >> 4) * 4 + r);
+            const int64_t place = min(row0 + (wm * TM + i) * 16 + (lane & 15), n - 1);
+            unsigned long long todo = __ballot(who[i] >= 0);
+            float back = 1.0f;
+            if constexpr (__is_same(T, _Float16)) back = who[i] >= 0 ? t.back[place] : 1.0f;
             while (todo) {
-                const int id = __builtin_amdgcn_readlane(mine, __ffsll(todo) - 1);
-                todo &= ~__ballot(mine == id);
+                const int id = __builtin_amdgcn_readlane(who[i], __ffsll(todo) - 1);
+                todo &= ~__ballot(who[i] == id);
+                // rows of other adapters give products that are dropped
                 f32x4 add[TN] = {};
-                float back[4] = {1.0f, 1.0f, 1.0f, 1.0f};
-                // rows of other adapters give products that are dropped below
-                const float* tp = t + min(r0 + (lane & 15), n - 1) * ldt + (lane >> 4) * N;
-                float up = 1.0f;
-                if constexpr (sizeof(T) == 2 && !__is_same(T, __bf16)) {
-                    float m = 0.0f;
-                    for (int k = 0; k < rk; ++k)
-#pragma unroll
-                        for (int j = 0; j < N; ++j)
-                            m = fmaxf(m, k * DEPTH<T> + (lane >> 4) * N < tw ? fabsf(tp[k * DEPTH<T> + j]) : 0.0f);
-                    m = fmaxf(m, __shfl_xor(m, 16));
-                    m = fmaxf(m, __shfl_xor(m, 32));
-                    const int e = m > 0.0f && m < INFINITY ? min(126, max(-126, 14 - ilogbf(m))) : 0;
-                    up = ldexpf(1.0f, e);
-                    const float down = ldexpf(1.0f, -e);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) back[r] = __shfl(down, (lane >> 4) * 4 + r);
-                }
                 for (int k = 0; k < rk; ++k) {
-                    V hi, lo;
-#pragma unroll
-                    for (int j = 0; j < N; ++j) {
-                        const float v = k * DEPTH<T> + (lane >> 4) * N < tw ? tp[k * DEPTH<T> + j] * up : 0.0f;
-                        hi[j] = (T)v;
-                        lo[j] = (T)(v - (float)hi[j]);
-                    }
+                    const int64_t at = place * t.ld + k * DEPTH<T> + (lane >> 4) * N;
+                    const V hi = load_piece(t.hi + at);
+                    V lo;
+                    if constexpr (sizeof(T) == 2) lo = load_piece(t.lo + at);
 #pragma unroll
                     for (int j = 0; j < TN; ++j) {
                         const int nt = min(ntw + j, nts - 1);
                         const V bv = load_piece(b + id * b_slot + ((int64_t)nt * rk + k) * (64 * N) + lane * N);
-                        add[j] = Mma<T>::run(hi, bv, add[j]);
-                        if constexpr (sizeof(T) == 2) add[j] = Mma<T>::run(lo, bv, add[j]);
+                        add[j] = Mma<T>::run(bv, hi, add[j]);
+                        if constexpr (sizeof(T) == 2) add[j] = Mma<T>::run(bv, lo, add[j]);
                     }
                 }
 #pragma unroll
                 for (int j = 0; j < TN; ++j)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        if (at[r] == id) acc[i][j][r] = fmaf(add[j][r], back[r], acc[i][j][r]);
+                        acc[i][j][r] = who[i] == id ? fmaf(add[j][r], back, acc[i][j][r]) : acc[i][j][r];
             }
         }
     }
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-        const int col = (ntw + j) * 16 + (lane & 15);
-        if (col >= out) continue;
-        const float bs = bias ? (float)bias[col] : 0.0f;
+    for (int j = 0; j < TN; j += 2) {
+        const int col = col0 + j * 16;
+        float bs[8];
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
+        for (int r = 0; r < 8; ++r) bs[r] = !ADD && bias && col + r < out ? (float)bias[col + r] : 0.0f;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int64_t row = row0 + (wm * TM + i) * 16 + (lane >> 4) * 4 + r;
-                if (row < n) y[row * out + col] = (T)(acc[i][j][r] + bs);
-            }
+        for (int i = 0; i < TM; ++i) {
+            T v[8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) v[r] = (T)(acc[i][j + (r >> 2)][r & 3] + bs[r]);
+            T* o = y + row[i] * out + col;
+            if (row[i] >= 0 && col + 8 <= out) __builtin_memcpy(o, v, sizeof(v));
+            else if (row[i] >= 0)
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if (col + r < out) o[r] = v[r];
+        }
     }
 }
 
@@ -372,7 +537,7 @@ AdapterShape adapter_shape(int32_t dtype, int32_t in, int32_t out, int32_t max_r
     AdapterShape s{};
     s.dtype = dtype, s.in = in, s.out = out, s.slots = slots;
     s.kt = (in + 2 * depth - 1) / (2 * depth) * 2;
-    s.nt = (out + 15) / 16;
+    s.nt = (out + 31) / 32 * 2;
     s.rt = (max_rank + 15) / 16;
     s.rt = s.rt <= 2 ? s.rt : s.rt <= 4 ? 4 : 8;  // the shrink kernel's forms
     s.rk = (max_rank + depth - 1) / depth;
@@ -381,17 +546,39 @@ AdapterShape adapter_shape(int32_t dtype, int32_t in, int32_t out, int32_t max_r
     return s;
 }
 
-void adapter_pack(int32_t dtype, const void* src, int rows, int cols, int tiles, int frags, void* dst) {
+void adapter_pack(int32_t dtype, const void* src, int rows, int cols, int tiles, int frags, bool outputs, void* dst) {
     with_dtype(dtype, [&](auto zero) {
         using T = decltype(zero);
         const int64_t pieces = (int64_t)tiles * frags * 64;
         RVX_LAUNCH("adapter_pack", pack_kernel<T>, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, (const T*)src,
-                   rows, cols, pieces, frags, (T*)dst);
+                   rows, cols, pieces, frags, outputs, (T*)dst);
     });
+}
+
+template <class T>
+static void pad_rows(const T* x, int64_t n, int in, int ld, T* out) {
+    RVX_LAUNCH("adapter_pad", pad_kernel<T>,
+               dim3((unsigned)std::min<int64_t>((n * ld + 255) / 256, 16LL * device().num_cus)), dim3(256), 0, x, n, in, ld,
+               out);
+}
+
+int64_t adapter_split_bytes(const AdapterShape& s) {
+    const int64_t k = s.kt * DEPTH<float>;
+    return s.dtype == RVX_DTYPE_F32 ? 4 * k * s.out : 0;
+}
+void adapter_split(const AdapterShape& s, const float* w, void* planes, float* inv) {
+    const int k = s.kt * DEPTH<float>;
+    if (k != s.in) {
+        float* padded = scratch_f32("adapter_x", (int64_t)s.out * k);
+        pad_rows<float>(w, s.out, s.in, k, padded);
+        w = padded;
+    }
+    split_h2_rows(w, nullptr, s.out, k, (_Float16*)planes, nullptr, inv);
 }
 
 void adapter_forward(const AdapterArgs& g) {
     const AdapterShape& s = g.s;
+    using std::integral_constant;
     with_dtype(s.dtype, [&](auto zero) {
         using T = decltype(zero);
         const T *x = (const T*)g.x, *w = (const T*)g.w, *bias = (const T*)g.bias, *b = (const T*)g.b;
@@ -402,56 +589,87 @@ void adapter_forward(const AdapterArgs& g) {
         if (s.in != s.kt * DEPTH<T>) {
             ldx = s.kt * DEPTH<T>;
             T* padded = (T*)scratch_bytes("adapter_x", n * ldx * (int64_t)sizeof(T));
-            RVX_LAUNCH("adapter_pad", pad_kernel<T>, dim3((unsigned)std::min<int64_t>((n * ldx + 255) / 256, 16LL * cus)),
-                       dim3(256), 0, x, n, s.in, ldx, padded);
+            pad_rows<T>(x, n, s.in, ldx, padded);
             x = padded;
         }
-        const int ldt = std::max(s.rk * DEPTH<T>, s.rt * 16);
-        float* t = nullptr;
+        const bool few = n <= 64;
+        Mid<T> t{};
+        int32_t* perm = nullptr;
         if (g.ids) {
-            t = scratch_f32("adapter_t", n * ldt);
-            auto go = [&](auto sm, auto rt) {
-                constexpr int SM = decltype(sm)::value, RT = decltype(rt)::value;
-                const unsigned tiles = (unsigned)((n + 16 * SM - 1) / (16 * SM));
-                const unsigned turns = SM == 1 ? 16 : 1;
-                RVX_LAUNCH("adapter_shrink", (shrink_kernel<T, SM, RT>), dim3(tiles, turns), dim3(64 * SH_WAVES), 0, x, ldx,
-                           n, (const T*)g.a, s.a_slot, s.kt, g.ids, g.slot, s.slots, t, ldt);
+            t.ld = std::max(s.rk * DEPTH<T>, s.rt * 16);
+            if (few) {
+                t.f = scratch_f32("adapter_t", n * t.ld);
+            } else {
+                perm = (int32_t*)scratch_bytes("adapter_rows", n * 4);
+                RVX_LAUNCH("adapter_group", group_rows_kernel, dim3(1), dim3(GROUP_THREADS), 0, g.ids, n, g.slot, s.slots,
+                           perm);
+                const int64_t plane = n * t.ld;
+                t.hi = (T*)scratch_bytes("adapter_t", 2 * plane * (int64_t)sizeof(T) + n * 4);
+                t.lo = t.hi + plane;
+                t.back = __is_same(T, _Float16) ? (float*)(t.lo + plane) : nullptr;
+            }
+            auto go = [&](auto sm, auto rt, auto waves, auto split) {
+                constexpr int SM = decltype(sm)::value, RT = decltype(rt)::value, W = decltype(waves)::value;
+                RVX_LAUNCH("adapter_shrink", (shrink_kernel<T, SM, RT, W, decltype(split)::value>),
+                           dim3((unsigned)((n + 16 * SM - 1) / (16 * SM)), few ? 16 : 1), dim3(64 * W), 0, x, ldx, n,
+                           (const int32_t*)perm, (const T*)g.a, s.a_slot, s.kt, g.ids, g.slot, s.slots, t);
             };
-            auto by_rank = [&](auto sm) {
-                if (s.rt == 1) go(sm, std::integral_constant<int, 1>{});
-                else if (s.rt == 2) go(sm, std::integral_constant<int, 2>{});
-                else if (s.rt == 4) go(sm, std::integral_constant<int, 4>{});
-                else go(sm, std::integral_constant<int, 8>{});
+            auto by_rank = [&](auto sm, auto waves, auto split) {
+                if (s.rt == 1) go(sm, integral_constant<int, 1>{}, waves, split);
+                else if (s.rt == 2) go(sm, integral_constant<int, 2>{}, waves, split);
+                else if (s.rt == 4) go(sm, integral_constant<int, 4>{}, waves, split);
+                else go(sm, integral_constant<int, 8>{}, integral_constant<int, 8>{}, split);
             };
-            if (n <= 1024) by_rank(std::integral_constant<int, 1>{});
-            else by_rank(std::integral_constant<int, 2>{});
+            if (few) by_rank(integral_constant<int, 1>{}, integral_constant<int, 16>{}, std::false_type{});
+            else if (n <= 2048) by_rank(integral_constant<int, 1>{}, integral_constant<int, 8>{}, std::true_type{});
+            else by_rank(integral_constant<int, 2>{}, integral_constant<int, 8>{}, std::true_type{});
         }
-        if (n <= 64) {
+        if (few) {
             auto go = [&](auto mt) {
                 constexpr int MT = decltype(mt)::value;
                 RVX_LAUNCH("adapter_few_rows", (few_rows_kernel<T, MT>), dim3(s.nt), dim3(64 * FEW_WAVES), 0, x, ldx, (int)n,
-                           w, s.kt, bias, b, s.b_slot, s.rk, g.ids, g.slot, s.slots, (const float*)t, ldt, s.out, y);
+                           w, s.kt, bias, b, s.b_slot, s.rk, g.ids, g.slot, s.slots, (const float*)t.f, t.ld, s.out, y);
             };
-            if (n <= 16) go(std::integral_constant<int, 1>{});
-            else if (n <= 32) go(std::integral_constant<int, 2>{});
-            else go(std::integral_constant<int, 4>{});
+            if (n <= 16) go(integral_constant<int, 1>{});
+            else if (n <= 32) go(integral_constant<int, 2>{});
+            else go(integral_constant<int, 4>{});
             return;
         }
-        auto go = [&](auto bm, auto bn, auto wm, auto wn) {
-            constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WM = decltype(wm)::value, WN = decltype(wn)::value;
+        auto go = [&](auto bm, auto bn, auto wm, auto wn, auto ns, auto add) {
+            constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WM = decltype(wm)::value,
+                          WN = decltype(wn)::value, NS = decltype(ns)::value;
             const int tm = (int)((n + BM - 1) / BM), tn = (s.out + BN - 1) / BN;
-            RVX_LAUNCH("adapter_tile", (tile_kernel<T, BM, BN, WM, WN>), dim3((unsigned)(tm * tn)), dim3(64 * WM * WN), 0, x,
-                       ldx, n, w, s.kt, s.nt, bias, b, s.b_slot, s.rk, g.ids, g.slot, s.slots, (const float*)t, ldt,
-                       s.rt * 16, s.out, tm, tn, y);
+            RVX_LAUNCH("adapter_tile", (tile_kernel<T, BM, BN, WM, WN, NS, decltype(add)::value>), dim3((unsigned)(tm * tn)),
+                       dim3(64 * WM * WN), 0, x, ldx, n, w, s.kt, s.nt, bias, b, s.b_slot, s.rk, g.ids, (const int32_t*)perm,
+                       g.slot, s.slots, t, s.out, tm, tn, y);
         };
-        using std::integral_constant;
         auto tiles = [&](int64_t bm, int64_t bn) { return (n + bm - 1) / bm * ((s.out + bn - 1) / bn); };
+        if constexpr (__is_same(T, float)) {
+            // The framework's split-f16 product has about twice the rate of f32 matrix instructions; it
+            // takes its operands row-major and knows no adapters, so their part is added to y.
+            GemmOperand op{x, ldx, nullptr, ldx, ldx};
+            op.Bh = (const _Float16*)g.w_split, op.Bh_plane = (int64_t)s.out * ldx, op.b_inv = g.w_inv;
+            if (g.w_split && tiles(128, 128) >= cus && gemm_h2_ok(n, s.out, op, nullptr)) {
+                GemmEpilogue ep;
+                ep.bias0 = bias;
+                float* scale = scratch_f32("gemm_auto_scale", n);
+                row_scale_h2(x, ldx, ldx, nullptr, 0, 0, n, scale);
+                gemm_nt_h2(n, s.out, op, op.Bh, nullptr, nullptr, scale, op.b_inv, ep, y, s.out, "adapter_gemm");
+                if (g.ids)
+                    go(integral_constant<int, 64>{}, integral_constant<int, 64>{}, integral_constant<int, 2>{},
+                       integral_constant<int, 2>{}, integral_constant<int, 2>{}, std::true_type{});
+                return;
+            }
+        }
         if (tiles(256, 256) >= cus)
-            go(integral_constant<int, 256>{}, integral_constant<int, 256>{}, integral_constant<int, 2>{}, integral_constant<int, 4>{});
+            go(integral_constant<int, 256>{}, integral_constant<int, 256>{}, integral_constant<int, 2>{},
+               integral_constant<int, 4>{}, integral_constant<int, 2>{}, std::false_type{});
         else if (tiles(128, 128) >= cus)
-            go(integral_constant<int, 128>{}, integral_constant<int, 128>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{});
+            go(integral_constant<int, 128>{}, integral_constant<int, 128>{}, integral_constant<int, 2>{},
+               integral_constant<int, 2>{}, integral_constant<int, 4>{}, std::false_type{});
         else
-            go(integral_constant<int, 64>{}, integral_constant<int, 64>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{});
+            go(integral_constant<int, 64>{}, integral_constant<int, 64>{}, integral_constant<int, 2>{},
+               integral_constant<int, 2>{}, integral_constant<int, 4>{}, std::false_type{});
     });
 }
 
