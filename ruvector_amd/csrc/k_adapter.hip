@@ -123,9 +123,20 @@ __global__ __launch_bounds__(GROUP_THREADS) void group_rows_kernel(const int32_t
         if (there && before == 0) at = atomicAdd(&next[bin], __popcll(same));
         return __shfl(at, there ? __ffsll(same) - 1 : lane) + before;
     };
+    constexpr int U = 8;  // rows of a thread at a time: their ids are loaded together
+    int bin[U];
+    auto load = [&](int64_t at) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) bin[u] = bin_of(at + u * GROUP_THREADS + t);
+    };
     for (int b = t; b < GROUP_BINS; b += GROUP_THREADS) next[b] = 0;
     __syncthreads();
-    for (int64_t i = t; i - lane < n; i += GROUP_THREADS) places(bin_of(i), i < n);
+    for (int64_t at = 0; at < n; at += U * GROUP_THREADS) {
+        load(at);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (at + u * GROUP_THREADS + wave * 64 < n) places(bin[u], at + u * GROUP_THREADS + t < n);
+    }
     __syncthreads();
     int v = 0, scan = 0;
     if (t < GROUP_BINS) {
@@ -144,9 +155,15 @@ __global__ __launch_bounds__(GROUP_THREADS) void group_rows_kernel(const int32_t
         next[t] = from;
     }
     __syncthreads();
-    for (int64_t i = t; i - lane < n; i += GROUP_THREADS) {
-        const int at = places(bin_of(i), i < n);
-        if (i < n) perm[at] = (int32_t)i;
+    for (int64_t at = 0; at < n; at += U * GROUP_THREADS) {
+        if (n > U * GROUP_THREADS) load(at);  // else it still holds them
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t i = at + u * GROUP_THREADS + t;
+            if (i - lane >= n) continue;
+            const int to = places(bin[u], i < n);
+            if (i < n) perm[to] = (int32_t)i;
+        }
     }
 }
 
@@ -338,23 +355,50 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_rows_kernel(const T* __res
 }
 
 // ---------------------------------------------------------------- many rows
-// A block: BM rows (of the permutation) x BN outputs; WM x WN waves; the sum in stages of 2 fragments,
-// NS of which are in LDS or on their way to it (copied there without registers). A stage's second half
-// is read while the first is multiplied, the next stage's first half while the second is; the one
-// barrier of a stage lies between: behind it everybody has read this stage, and has the next.
+// A block: BM rows (of the permutation) x BN outputs; WM x WN waves; the sum in stages one fragment
+// deep, NS of which are in LDS or on their way to it (copied there without registers). While a stage is
+// multiplied from registers, the next one is read into others. Behind a stage's one barrier everybody
+// has read it, so its place is free for stage s + NS, and has the next: the copies of NS - 2 stages
+// more may still be on their way, which is what hides their latency.
 template <int BM, int BN, int WM, int WN, int NS>
 struct TileCfg {
     static constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
-    static constexpr int XF = BM / 16 * 2, WF = BN / 16 * 2;  // 1-KiB fragments of a stage
+    static constexpr int XF = BM / 16, WF = BN / 16;          // 1-KiB fragments of a stage
     static constexpr int XP = XF / WAVES, WP = WF / WAVES;    // copied by each wave
     static constexpr int STAGE = (XF + WF) * 1024;
     static_assert(XF % WAVES == 0 && WF % WAVES == 0 && TN % 2 == 0);
 };
 
-// Vm: at most that many of this wave's copies are still on their way
+// All waves have read LDS as far as they asked for, and at most Vm of their copies are on their way.
+// (Builtins, so that the compiler knows what has arrived.)
 template <int Vm>
 __device__ __forceinline__ void wait_and_meet() {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(Vm) : "memory");
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt((Vm & 15) | (Vm >> 4) << 14 | 7 << 4);  // lgkmcnt 0
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+}
+
+// The order of a half stage's instructions: one copy or one read of LDS between products, so that
+// none of the three units waits for the others' turns.
+template <int READS, int COPIES, int PRODUCTS>
+__device__ __forceinline__ void spread() {
+#ifndef NO_SPREAD
+    constexpr int EACH = PRODUCTS / (READS + COPIES) > 0 ? PRODUCTS / (READS + COPIES) : 1;
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < READS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS, 0);
+#endif
 }
 
 // ADD: y is there already (f32), the adapters' part is added to it.
@@ -368,7 +412,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const T* __restrict_
                                                            int out, int tiles_m, int tiles_n, T* y) {
     using Cf = TileCfg<BM, BN, WM, WN, NS>;
     using V = typename Mma<T>::V;
-    constexpr int N = PIECE<T>, TM = Cf::TM, TN = Cf::TN;
+    constexpr int N = PIECE<T>, TM = Cf::TM, TN = Cf::TN, MMA = sizeof(T) == 2 ? 1 : 4;
     __shared__ __align__(16) unsigned char lds[ADD ? 16 : NS * Cf::STAGE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave - wm * WN;
@@ -398,59 +442,70 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const T* __restrict_
         const T* xs[Cf::XP];
         const T* ws[Cf::WP];
 #pragma unroll
-        for (int j = 0; j < Cf::XP; ++j) {
-            const int f = wave * Cf::XP + j;
-            xs[j] = x + row_at(row0 + (f >> 1) * 16 + (lane & 15)) * ldx + (f & 1) * DEPTH<T> + (lane >> 4) * N;
-        }
+        for (int j = 0; j < Cf::XP; ++j)
+            xs[j] = x + row_at(row0 + (wave * Cf::XP + j) * 16 + (lane & 15)) * ldx + (lane >> 4) * N;
 #pragma unroll
-        for (int j = 0; j < Cf::WP; ++j) {
-            const int f = wave * Cf::WP + j;
-            ws[j] = w + ((int64_t)min(nt0 + (f >> 1), nts - 1) * kt + (f & 1)) * (64 * N);
-        }
+        for (int j = 0; j < Cf::WP; ++j) ws[j] = w + (int64_t)min(nt0 + wave * Cf::WP + j, nts - 1) * kt * (64 * N);
         auto fill = [&](int s, int buf) {
             unsigned char* base = lds + buf * Cf::STAGE;
 #pragma unroll
             for (int j = 0; j < Cf::XP; ++j)
                 __builtin_amdgcn_global_load_lds(
-                    (const void*)(xs[j] + s * (2 * DEPTH<T>)),
+                    (const void*)(xs[j] + s * DEPTH<T>),
                     (__attribute__((address_space(3))) void*)(base + (wave * Cf::XP + j) * 1024), 16, 0, 0);
 #pragma unroll
             for (int j = 0; j < Cf::WP; ++j)
                 __builtin_amdgcn_global_load_lds(
-                    (const void*)(ws[j] + (int64_t)s * (2 * 64 * N) + lane * N),
+                    (const void*)(ws[j] + (int64_t)s * (64 * N) + lane * N),
                     (__attribute__((address_space(3))) void*)(base + (Cf::XF + wave * Cf::WP + j) * 1024), 16, 0, 0);
         };
         V xv[2][TM], wv[2][TN];
-        auto read = [&](int h, int buf) {
+        auto read = [&](auto to, int buf) {
+            constexpr int h = decltype(to)::value;
             const unsigned char* base = lds + buf * Cf::STAGE + lane * 16;
 #pragma unroll
-            for (int j = 0; j < TN; ++j) wv[h][j] = *(const V*)(base + (Cf::XF + (wn * TN + j) * 2 + h) * 1024);
+            for (int j = 0; j < TN; ++j) wv[h][j] = *(const V*)(base + (Cf::XF + wn * TN + j) * 1024);
 #pragma unroll
-            for (int i = 0; i < TM; ++i) xv[h][i] = *(const V*)(base + ((wm * TM + i) * 2 + h) * 1024);
+            for (int i = 0; i < TM; ++i) xv[h][i] = *(const V*)(base + (wm * TM + i) * 1024);
         };
-        auto multiply = [&](int h) {
+        auto multiply = [&](auto from) {
+            constexpr int h = decltype(from)::value;
 #pragma unroll
             for (int i = 0; i < TM; ++i)
 #pragma unroll
                 for (int j = 0; j < TN; ++j) acc[i][j] = Mma<T>::run(wv[h][j], xv[h][i], acc[i][j]);
         };
-        const int stages = kt / 2;
-        for (int s = 0; s < NS - 1 && s < stages; ++s) fill(s, s);
+        constexpr int COPIES = Cf::XP + Cf::WP;
+        for (int s = 0; s < NS && s < kt; ++s) fill(s, s);
         wait_and_meet<0>();
-        if (NS - 1 < stages) fill(NS - 1, NS - 1);
-        read(0, 0);
-        int buf = 0;
-        for (int s = 0; s < stages; ++s) {
+        read(std::integral_constant<int, 0>{}, 0);
+        int s = 0, buf = 0;
+        auto step = [&](auto at, bool full) {  // stage s is in registers, or on its way from LDS
+            constexpr int h = decltype(at)::value;
             const int next = buf + 1 == NS ? 0 : buf + 1;
-            read(1, buf);
-            multiply(0);
-            // behind the copies of stages s + 2 .. s + NS - 1, where they were begun
-            if (s + NS - 1 < stages) wait_and_meet<(NS - 2) * (Cf::XP + Cf::WP)>();
-            else wait_and_meet<0>();
-            if (s + NS < stages) fill(s + NS, buf);
-            if (s + 1 < stages) read(0, next);
-            multiply(1);
+            if (full) {
+                wait_and_meet<(NS - 2) * COPIES>();
+                fill(s + NS, buf);
+                read(std::integral_constant<int, 1 - h>{}, next);
+                multiply(at);
+                spread<TM + TN, COPIES, TM * TN * MMA>();
+                __builtin_amdgcn_sched_barrier(0);
+            } else {
+                wait_and_meet<0>();
+                if (s + NS < kt) fill(s + NS, buf);
+                if (s + 1 < kt) read(std::integral_constant<int, 1 - h>{}, next);
+                multiply(at);
+            }
             buf = next;
+            ++s;
+        };
+        for (; s + 1 + NS < kt;) {  // kt is even
+            step(std::integral_constant<int, 0>{}, true);
+            step(std::integral_constant<int, 1>{}, true);
+        }
+        for (; s < kt;) {
+            step(std::integral_constant<int, 0>{}, false);
+            step(std::integral_constant<int, 1>{}, false);
         }
     }
 
@@ -477,35 +532,46 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const T* __restrict_
                 }
     }
     if (ids) {
+        float back[TM];
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
-            const int64_t place = min(row0 + (wm * TM + i) * 16 + (lane & 15), n - 1);
-            unsigned long long todo = __ballot(who[i] >= 0);
-            float back = 1.0f;
-            if constexpr (__is_same(T, _Float16)) back = who[i] >= 0 ? t.back[place] : 1.0f;
-            while (todo) {
-                const int id = __builtin_amdgcn_readlane(who[i], __ffsll(todo) - 1);
-                todo &= ~__ballot(who[i] == id);
-                // rows of other adapters give products that are dropped
-                f32x4 add[TN] = {};
-                for (int k = 0; k < rk; ++k) {
-                    const int64_t at = place * t.ld + k * DEPTH<T> + (lane >> 4) * N;
-                    const V hi = load_piece(t.hi + at);
-                    V lo;
-                    if constexpr (sizeof(T) == 2) lo = load_piece(t.lo + at);
+        for (int i = 0; i < TM; ++i) back[i] = 1.0f;
+        if constexpr (__is_same(T, _Float16))
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+                if (who[i] >= 0) back[i] = t.back[row0 + (wm * TM + i) * 16 + (lane & 15)];
+        for (int k = 0; k < rk; ++k) {
+            V hi[TM], lo[TM];  // rows without an adapter hold anything: their products are dropped
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                const int64_t place = min(row0 + (wm * TM + i) * 16 + (lane & 15), n - 1);
+                const int64_t at = place * t.ld + k * DEPTH<T> + (lane >> 4) * N;
+                hi[i] = load_piece(t.hi + at);
+                if constexpr (sizeof(T) == 2) lo[i] = load_piece(t.lo + at);
+            }
+            int held = -1;
+            V bv[TN];
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                unsigned long long todo = __ballot(who[i] >= 0);
+                while (todo) {
+                    const int id = __builtin_amdgcn_readlane(who[i], __ffsll(todo) - 1);
+                    todo &= ~__ballot(who[i] == id);
+                    if (id != held) {
+#pragma unroll
+                        for (int j = 0; j < TN; ++j)
+                            bv[j] = load_piece(b + id * b_slot + ((int64_t)min(ntw + j, nts - 1) * rk + k) * (64 * N) +
+                                               lane * N);
+                        held = id;
+                    }
 #pragma unroll
                     for (int j = 0; j < TN; ++j) {
-                        const int nt = min(ntw + j, nts - 1);
-                        const V bv = load_piece(b + id * b_slot + ((int64_t)nt * rk + k) * (64 * N) + lane * N);
-                        add[j] = Mma<T>::run(bv, hi, add[j]);
-                        if constexpr (sizeof(T) == 2) add[j] = Mma<T>::run(bv, lo, add[j]);
+                        f32x4 add = Mma<T>::run(bv[j], hi[i], f32x4{0, 0, 0, 0});
+                        if constexpr (sizeof(T) == 2) add = Mma<T>::run(bv[j], lo[i], add);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            acc[i][j][r] = who[i] == id ? fmaf(add[r], back[i], acc[i][j][r]) : acc[i][j][r];
                     }
                 }
-#pragma unroll
-                for (int j = 0; j < TN; ++j)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        acc[i][j][r] = who[i] == id ? fmaf(add[j][r], back, acc[i][j][r]) : acc[i][j][r];
             }
         }
     }
@@ -663,7 +729,7 @@ void adapter_forward(const AdapterArgs& g) {
         }
         if (tiles(256, 256) >= cus)
             go(integral_constant<int, 256>{}, integral_constant<int, 256>{}, integral_constant<int, 2>{},
-               integral_constant<int, 4>{}, integral_constant<int, 2>{}, std::false_type{});
+               integral_constant<int, 4>{}, integral_constant<int, 4>{}, std::false_type{});
         else if (tiles(128, 128) >= cus)
             go(integral_constant<int, 128>{}, integral_constant<int, 128>{}, integral_constant<int, 2>{},
                integral_constant<int, 2>{}, integral_constant<int, 4>{}, std::false_type{});
