@@ -24,9 +24,8 @@ struct AdapterShape {
 };
 AdapterShape adapter_shape(int32_t dtype, int32_t in, int32_t out, int32_t max_rank, int32_t slots);
 
-// src [rows][cols] row-major to fragments [tiles][frags][64 lanes][16 bytes], zero padded; outputs: the
-// rows are outputs (W, B), interleaved over pairs of tiles
-void adapter_pack(int32_t dtype, const void* src, int rows, int cols, int tiles, int frags, bool outputs, void* dst);
+// src [rows][cols] row-major to fragments [tiles][frags][64 lanes][16 bytes], zero padded; what: 0 W, 1 A, 2 B
+void adapter_pack(int32_t dtype, const void* src, int rows, int cols, int tiles, int frags, int what, void* dst);
 // f32 layers: W as the split-f16 planes of the framework's GEMM (bytes; planes and column scales from w)
 int64_t adapter_split_bytes(const AdapterShape& s);
 void adapter_split(const AdapterShape& s, const float* w, void* planes, float* inv);

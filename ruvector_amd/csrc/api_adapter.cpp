@@ -40,7 +40,7 @@ rvx_status rvx_adapter_linear_create(const rvx_adapter_linear_config* cfg, const
         l->device = device().id;
         const AdapterShape& s = l->s;
         l->w.reset((int64_t)s.nt * s.kt * 1024);
-        adapter_pack(s.dtype, weight->mem.p, s.out, s.in, s.nt, s.kt, true, l->w.p);
+        adapter_pack(s.dtype, weight->mem.p, s.out, s.in, s.nt, s.kt, 0, l->w.p);
         if (const int64_t bytes = adapter_split_bytes(s)) {
             l->split.reset(bytes);
             l->split_inv.reset((int64_t)s.out * 4);
@@ -83,8 +83,8 @@ rvx_status rvx_adapter_linear_set(rvx_adapter_linear* l, int32_t slot, int32_t r
         }
         ComputeLock cl;
         if (rank) {
-            adapter_pack(s.dtype, a->mem.p, rank, s.in, s.rt, s.kt, false, (char*)l->a.p + slot * s.a_slot * size);
-            adapter_pack(s.dtype, b->mem.p, s.out, rank, s.nt, s.rk, true, (char*)l->b.p + slot * s.b_slot * size);
+            adapter_pack(s.dtype, a->mem.p, rank, s.in, s.rt, s.kt, 1, (char*)l->a.p + slot * s.a_slot * size);
+            adapter_pack(s.dtype, b->mem.p, s.out, rank, s.nt, s.rk, 2, (char*)l->b.p + slot * s.b_slot * size);
         }
         l->host_slot[slot] = AdapterSlot{scale, rank};
         l->slot.upload(&l->host_slot[slot], sizeof(AdapterSlot), (int64_t)slot * sizeof(AdapterSlot));  // waits

@@ -5,12 +5,16 @@
 // kernels then go through a permutation of the rows, in which a 16-row tile holds one adapter or
 // two, and take one turn for each. The products of a row do not depend on its place.
 //
-// Weights lie in fragment order: the 16 rows x 64 bytes that one matrix instruction takes from
+// All operands lie in fragment order: the 16 rows x 64 bytes that one matrix instruction takes from
 // one operand are 1 KiB, lane l's 16 bytes at l * 16 (row l % 16, elements (l / 16) * N ..). A
 // wave loads a fragment with one coalesced instruction, copies it to LDS as it is, and reads it
-// back without bank conflicts. W and B are the first operand, x and t the second, so that a lane
+// back without bank conflicts. Weights are laid out when they are set, x by the launch that computes
+// t, which reads it anyway: a CU takes 75 to 110 bytes a ns from L2 in whole KiB, but only 35 where
+// each load gathers 16 rows, and the projection reads x many times. W and B are the first operand, x and t the second, so that a lane
 // holds 4 outputs of one row; the 32 outputs of two neighbouring fragments are interleaved by 4
-// (`out_of`), so that the two give it 8 neighbouring outputs.
+// (`out_of`), so that the two give it 8 neighbouring outputs. Along `in`, two neighbouring fragments
+// are interleaved by pieces (`in_of`): a row's two pieces of one lane are neighbours, and the loads of
+// a pair touch whole 128-byte lines of x.
 #include "adapter.hpp"
 #include "kernels.hpp"
 
@@ -62,16 +66,24 @@ __host__ __device__ __forceinline__ int out_of(int nt, int m) {
     return (nt >> 1) * 32 + (m >> 2) * 8 + (nt & 1) * 4 + (m & 3);
 }
 
+// where piece `lane / 16` of fragment f begins along `in` (an even number of fragments)
+template <class T>
+__host__ __device__ __forceinline__ int in_of(int f, int piece) {
+    return (f >> 1) * (2 * DEPTH<T>)+piece * (2 * PIECE<T>)+(f & 1) * PIECE<T>;
+}
+
+enum { PACK_W, PACK_A, PACK_B };  // W [out][in], A [rank][in], B [out][rank]
+
 template <class T>
 __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ src, int rows, int cols, int64_t pieces,
-                                                  int frags, bool outputs, T* __restrict__ dst) {
+                                                  int frags, int what, T* __restrict__ dst) {
     constexpr int N = PIECE<T>;
     const int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (p >= pieces) return;
     const int lane = (int)(p & 63);
     const int64_t f = p >> 6;
-    const int tile = (int)(f / frags), row = outputs ? out_of(tile, lane & 15) : tile * 16 + (lane & 15);
-    const int col = (int)(f % frags) * DEPTH<T> + (lane >> 4) * N;
+    const int tile = (int)(f / frags), row = what == PACK_A ? tile * 16 + (lane & 15) : out_of(tile, lane & 15);
+    const int frag = (int)(f % frags), col = what == PACK_B ? frag * DEPTH<T> + (lane >> 4) * N : in_of<T>(frag, lane >> 4);
     T v[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) v[j] = row < rows && col + j < cols ? src[(int64_t)row * cols + col + j] : (T)0.0f;
@@ -96,25 +108,23 @@ __device__ __forceinline__ int adapter_of(const int32_t* ids, const AdapterSlot*
 }
 
 // ---------------------------------------------------------------- grouping rows
-// perm: the rows in the order of their adapters (adapters that agree modulo GROUP_BINS - 1 may mix:
-// the order is for speed alone). One block: it is a small part of what follows.
-constexpr int GROUP_THREADS = 1024, GROUP_BITS = 9, GROUP_BINS = 1 << GROUP_BITS;
+// perm: GROUP_ROWS rows at a time, a block each, in the order of their adapters (adapters that agree
+// modulo GROUP_BINS - 1 may mix: the order is for speed alone).
+constexpr int GROUP_THREADS = 1024, GROUP_ROWS = 2 * GROUP_THREADS, GROUP_BITS = 9, GROUP_BINS = 1 << GROUP_BITS;
 
 __global__ __launch_bounds__(GROUP_THREADS) void group_rows_kernel(const int32_t* __restrict__ ids, int64_t n,
-                                                                  const AdapterSlot* __restrict__ slot, int slots,
-                                                                  int32_t* __restrict__ perm) {
+                                                                  int slots, int bits, int32_t* __restrict__ perm) {
     __shared__ int next[GROUP_BINS];
     __shared__ int sums[GROUP_BINS / 64];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     auto bin_of = [&](int64_t row) {
-        const int id = adapter_of(ids, slot, slots, row, n);
-        return id < 0 ? 0 : 1 + id % (GROUP_BINS - 1);
+        const int id = row < n ? ids[row] : -1;
+        return id < 0 || id >= slots ? 0 : 1 + id % (GROUP_BINS - 1);
     };
     // the wave's lanes with the same bin: the first of them takes places for all
     auto places = [&](int bin, bool there) {
         unsigned long long same = __ballot(there);
-#pragma unroll
-        for (int b = 0; b < GROUP_BITS; ++b) {
+        for (int b = 0; b < bits; ++b) {  // bits: of the largest bin there can be
             const unsigned long long m = __ballot(bin >> b & 1);
             same &= bin >> b & 1 ? m : ~m;
         }
@@ -123,20 +133,15 @@ __global__ __launch_bounds__(GROUP_THREADS) void group_rows_kernel(const int32_t
         if (there && before == 0) at = atomicAdd(&next[bin], __popcll(same));
         return __shfl(at, there ? __ffsll(same) - 1 : lane) + before;
     };
-    constexpr int U = 8;  // rows of a thread at a time: their ids are loaded together
+    const int64_t row0 = (int64_t)blockIdx.x * GROUP_ROWS;
+    constexpr int U = GROUP_ROWS / GROUP_THREADS;
     int bin[U];
-    auto load = [&](int64_t at) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) bin[u] = bin_of(at + u * GROUP_THREADS + t);
-    };
+    for (int u = 0; u < U; ++u) bin[u] = bin_of(row0 + u * GROUP_THREADS + t);
     for (int b = t; b < GROUP_BINS; b += GROUP_THREADS) next[b] = 0;
     __syncthreads();
-    for (int64_t at = 0; at < n; at += U * GROUP_THREADS) {
-        load(at);
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (at + u * GROUP_THREADS + wave * 64 < n) places(bin[u], at + u * GROUP_THREADS + t < n);
-    }
+    for (int u = 0; u < U; ++u) places(bin[u], row0 + u * GROUP_THREADS + t < n);
     __syncthreads();
     int v = 0, scan = 0;
     if (t < GROUP_BINS) {
@@ -155,15 +160,11 @@ __global__ __launch_bounds__(GROUP_THREADS) void group_rows_kernel(const int32_t
         next[t] = from;
     }
     __syncthreads();
-    for (int64_t at = 0; at < n; at += U * GROUP_THREADS) {
-        if (n > U * GROUP_THREADS) load(at);  // else it still holds them
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t i = at + u * GROUP_THREADS + t;
-            if (i - lane >= n) continue;
-            const int to = places(bin[u], i < n);
-            if (i < n) perm[to] = (int32_t)i;
-        }
+    for (int u = 0; u < U; ++u) {
+        const int64_t i = row0 + u * GROUP_THREADS + t;
+        const int to = places(bin[u], i < n);
+        if (i < n) perm[row0 + to] = (int32_t)i;
     }
 }
 
@@ -179,104 +180,139 @@ struct Mid {
     int ld;
 };
 
-// A block: 16 * SM rows (of the permutation), the waves split the sum over `in`. The block's y-th,
-// (y + gridDim.y)-th .. different adapter is its work.
-template <class T, int SM, int RT, int WAVES, bool SPLIT>
-__global__ __launch_bounds__(64 * WAVES) void shrink_kernel(const T* __restrict__ x, int ldx, int64_t n,
+// N values of a row from column c on, zeros past `in`
+template <class T>
+__device__ __forceinline__ typename Mma<T>::V row_piece(const T* row, int c, int in, bool whole) {
+    if (whole || c + PIECE<T> <= in) return load_piece(row + c);
+    typename Mma<T>::V v;
+#pragma unroll
+    for (int j = 0; j < PIECE<T>; ++j) v[j] = c + j < in ? row[c + j] : (T)0.0f;
+    return v;
+}
+
+// A block: 16 rows (of the permutation), the waves split the sum over `in`. Lays the rows out in
+// fragment order (PACK) and computes t for them: the block's y-th, (y + gridDim.y)-th .. different
+// adapter is its work; RT == 0: no adapters.
+template <class T, int RT, int WAVES, bool SPLIT, bool PACK>
+__global__ __launch_bounds__(64 * WAVES) void shrink_kernel(const T* __restrict__ x, int in, int64_t n,
                                                            const int32_t* __restrict__ perm, const T* __restrict__ a,
                                                            int64_t a_slot, int kt, const int32_t* __restrict__ ids,
-                                                           const AdapterSlot* __restrict__ slot, int slots, Mid<T> t) {
+                                                           const AdapterSlot* __restrict__ slot, int slots, Mid<T> t,
+                                                           T* __restrict__ packed) {
     using V = typename Mma<T>::V;
-    constexpr int N = PIECE<T>;
-    __shared__ f32x4 red[WAVES][SM * RT][64];
+    constexpr int N = PIECE<T>, R = RT ? RT : 1;
+    __shared__ f32x4 red[RT ? WAVES : 1][R][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t row0 = (int64_t)blockIdx.x * (16 * SM);
-    const int64_t place = min(row0 + (lane & (16 * SM - 1)), n - 1);
-    const int64_t my_row = SPLIT ? perm[place] : place;
-    const int mine = lane < 16 * SM && row0 + lane < n ? adapter_of(ids, slot, slots, my_row, n) : -1;
+    const int64_t row0 = (int64_t)blockIdx.x * 16;
+    const int64_t place = min(row0 + (lane & 15), n - 1);
+    const int64_t my_row = perm ? perm[place] : place;
+    const int mine = RT && lane < 16 && row0 + lane < n ? adapter_of(ids, slot, slots, my_row, n) : -1;
     unsigned long long todo = __ballot(mine >= 0);
-    if (!todo) return;
-    const T* xp[SM];
-#pragma unroll
-    for (int m = 0; m < SM; ++m)
-        xp[m] = x + (int64_t)__shfl((int)my_row, m * 16 + (lane & 15)) * ldx + (lane >> 4) * N;
-    const int per = (kt + WAVES - 1) / WAVES, k0 = min(kt, wave * per), k1 = min(kt, k0 + per);
-    for (int turn = 0; todo; ++turn) {
-        const int id = __builtin_amdgcn_readlane(mine, __ffsll(todo) - 1);
+    const T* xp = x + my_row * in;
+    const int per = (kt / 2 + WAVES - 1) / WAVES * 2, k0 = min(kt, wave * per), k1 = min(kt, k0 + per);
+    const int whole = in / (2 * DEPTH<T>)*2;  // fragments without a zero
+    T* to = packed + (int64_t)blockIdx.x * kt * (64 * N) + lane * N;
+    bool pack = PACK && blockIdx.y == 0;
+    for (int turn = 0; todo || pack; ++turn) {
+        const int id = todo ? __builtin_amdgcn_readlane(mine, __ffsll(todo) - 1) : -1;
         todo &= ~__ballot(mine == id);
-        if (turn % gridDim.y != blockIdx.y) continue;
-        f32x4 acc[SM][RT] = {};
-        const T* ap = a + id * a_slot + lane * N;
-#pragma unroll 4
-        for (int k = k0; k < k1; ++k) {
-            V xv[SM];
+        const bool multiply = RT && id >= 0 && turn % gridDim.y == blockIdx.y;
+        if (!multiply && !pack) continue;
+        f32x4 acc[R] = {};
+        const T* ap = a + (multiply ? id : 0) * a_slot + lane * N;
+        auto sweep = [&](auto packs, auto multiplies) {
+            constexpr bool PK = decltype(packs)::value, MU = decltype(multiplies)::value && RT > 0;
+            constexpr int U = !MU || R <= 2 ? 8 : 16 / R;  // loads in flight, by registers
+            int k = k0;
+            for (; k + U <= min(k1, whole); k += U) {
+                V xv[U], av[U][R];
 #pragma unroll
-            for (int m = 0; m < SM; ++m) xv[m] = load_piece(xp[m] + k * DEPTH<T>);
+                for (int u = 0; u < U; ++u) {
+                    xv[u] = load_piece(xp + in_of<T>(k + u, lane >> 4));
+                    if constexpr (MU)
 #pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                const V av = load_piece(ap + ((int64_t)r * kt + k) * (64 * N));
+                        for (int r = 0; r < R; ++r) av[u][r] = load_piece(ap + ((int64_t)r * kt + k + u) * (64 * N));
+                }
 #pragma unroll
-                for (int m = 0; m < SM; ++m) acc[m][r] = Mma<T>::run(av, xv[m], acc[m][r]);
-            }
-        }
+                for (int u = 0; u < U; ++u) {
+                    if constexpr (PK) __builtin_memcpy(to + (int64_t)(k + u) * (64 * N), &xv[u], 16);
+                    if constexpr (MU)
 #pragma unroll
-        for (int m = 0; m < SM; ++m)
-#pragma unroll
-            for (int r = 0; r < RT; ++r) red[wave][m * RT + r][lane] = acc[m][r];
-        __syncthreads();
-        const AdapterSlot info = slot[id];
-        // a wave a 16-row tile: lane l has ranks r * 16 + (l / 16) * 4 .. of row l % 16
-        for (int m = wave; m < SM; m += WAVES) {
-            float v[RT][4], most = 0.0f;
-#pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                f32x4 sum = red[0][m * RT + r][lane];
-#pragma unroll
-                for (int w = 1; w < WAVES; ++w) sum += red[w][m * RT + r][lane];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    // past the adapter's rank: zeros, whatever x holds
-                    v[r][j] = r * 16 + (lane >> 4) * 4 + j < info.rank ? sum[j] * info.scale : 0.0f;
-                    most = fmaxf(most, fabsf(v[r][j]));
+                        for (int r = 0; r < R; ++r) acc[r] = Mma<T>::run(av[u][r], xv[u], acc[r]);
                 }
             }
-            float up = 1.0f, down = 1.0f;
-            if constexpr (SPLIT && __is_same(T, _Float16)) {
-                most = fmaxf(most, __shfl_xor(most, 16));
-                most = fmaxf(most, __shfl_xor(most, 32));
-                if (most > 0.0f && most < INFINITY && !(most >= 0.125f && most < 32768.0f)) {
-                    const int e = min(126, max(-126, 14 - ilogbf(most)));
-                    up = ldexpf(1.0f, e), down = ldexpf(1.0f, -e);
-                }
-            }
-            const int64_t at = row0 + m * 16 + (lane & 15);  // the place in the permutation
-            if (__shfl(mine, m * 16 + (lane & 15)) != id) continue;
-            if constexpr (!SPLIT) {
+            for (; k < k1; ++k) {
+                const V xv = row_piece(xp, in_of<T>(k, lane >> 4), in, k < whole);
+                if constexpr (PK) __builtin_memcpy(to + (int64_t)k * (64 * N), &xv, 16);
+                if constexpr (MU)
 #pragma unroll
-                for (int r = 0; r < RT; ++r) __builtin_memcpy(t.f + at * t.ld + r * 16 + (lane >> 4) * 4, v[r], 16);
-            } else {
-                if (t.back && lane < 16) t.back[at] = down;
+                    for (int r = 0; r < R; ++r)
+                        acc[r] = Mma<T>::run(load_piece(ap + ((int64_t)r * kt + k) * (64 * N)), xv, acc[r]);
+            }
+        };
+        if (pack) sweep(std::integral_constant<bool, PACK>{}, std::true_type{});  // any adapter, where it has none
+        else if constexpr (RT > 0) sweep(std::false_type{}, std::true_type{});
+        pack = false;
+        if (!multiply) continue;
+        if constexpr (RT > 0) {
+#pragma unroll
+            for (int r = 0; r < RT; ++r) red[wave][r][lane] = acc[r];
+            __syncthreads();
+            if (wave == 0) {
+                // lane l has ranks r * 16 + (l / 16) * 4 .. of row l % 16
+                const AdapterSlot info = slot[id];
+                float v[RT][4], most = 0.0f;
 #pragma unroll
                 for (int r = 0; r < RT; ++r) {
-                    T hi[4], lo[4];
+                    f32x4 sum = red[0][r][lane];
+#pragma unroll
+                    for (int w = 1; w < WAVES; ++w) sum += red[w][r][lane];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        hi[j] = (T)(v[r][j] * up);
-                        lo[j] = (T)(v[r][j] * up - (float)hi[j]);
+                        // past the adapter's rank: zeros, whatever x holds
+                        v[r][j] = r * 16 + (lane >> 4) * 4 + j < info.rank ? sum[j] * info.scale : 0.0f;
+                        most = fmaxf(most, fabsf(v[r][j]));
                     }
-                    const int64_t o = at * t.ld + r * 16 + (lane >> 4) * 4;
-                    __builtin_memcpy(t.hi + o, hi, sizeof(hi));
-                    if (sizeof(T) == 2) __builtin_memcpy(t.lo + o, lo, sizeof(lo));
                 }
-                if (RT == 1 && t.ld > 16) {  // a fragment is 32 ranks deep
-                    const int64_t o = at * t.ld + 16 + (lane >> 4) * 4;
-                    const T zero[4] = {};
-                    __builtin_memcpy(t.hi + o, zero, sizeof(zero));
-                    __builtin_memcpy(t.lo + o, zero, sizeof(zero));
+                float up = 1.0f, down = 1.0f;
+                if constexpr (SPLIT && __is_same(T, _Float16)) {
+                    most = fmaxf(most, __shfl_xor(most, 16));
+                    most = fmaxf(most, __shfl_xor(most, 32));
+                    if (most > 0.0f && most < INFINITY && !(most >= 0.125f && most < 32768.0f)) {
+                        const int e = min(126, max(-126, 14 - ilogbf(most)));
+                        up = ldexpf(1.0f, e), down = ldexpf(1.0f, -e);
+                    }
+                }
+                const int64_t at = row0 + (lane & 15);  // the place in the permutation
+                if (__shfl(mine, lane & 15) == id) {
+                    if constexpr (!SPLIT) {
+#pragma unroll
+                        for (int r = 0; r < RT; ++r) __builtin_memcpy(t.f + at * t.ld + r * 16 + (lane >> 4) * 4, v[r], 16);
+                    } else {
+                        if (t.back && lane < 16) t.back[at] = down;
+#pragma unroll
+                        for (int r = 0; r < RT; ++r) {
+                            T hi[4], lo[4];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                hi[j] = (T)(v[r][j] * up);
+                                lo[j] = (T)(v[r][j] * up - (float)hi[j]);
+                            }
+                            const int64_t o = at * t.ld + r * 16 + (lane >> 4) * 4;
+                            __builtin_memcpy(t.hi + o, hi, sizeof(hi));
+                            if (sizeof(T) == 2) __builtin_memcpy(t.lo + o, lo, sizeof(lo));
+                        }
+                        if (RT == 1 && t.ld > 16) {  // a fragment is 32 ranks deep
+                            const int64_t o = at * t.ld + 16 + (lane >> 4) * 4;
+                            const T zero[4] = {};
+                            __builtin_memcpy(t.hi + o, zero, sizeof(zero));
+                            __builtin_memcpy(t.lo + o, zero, sizeof(zero));
+                        }
+                    }
                 }
             }
+            __syncthreads();
         }
-        __syncthreads();
     }
 }
 
@@ -285,8 +321,9 @@ __global__ __launch_bounds__(64 * WAVES) void shrink_kernel(const T* __restrict_
 // LDS. Bound by reading W once.
 constexpr int FEW_WAVES = 16;
 
-template <class T, int MT>
-__global__ __launch_bounds__(64 * FEW_WAVES) void few_rows_kernel(const T* __restrict__ x, int ldx, int n,
+// MT == 0: one row tile, x row-major.
+template <class T, int MT0>
+__global__ __launch_bounds__(64 * FEW_WAVES) void few_rows_kernel(const T* __restrict__ x, int in, int n,
                                                                  const T* __restrict__ w, int kt,
                                                                  const T* __restrict__ bias, const T* __restrict__ b,
                                                                  int64_t b_slot, int rk,
@@ -295,7 +332,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_rows_kernel(const T* __res
                                                                  const float* __restrict__ t, int ldt, int out,
                                                                  T* __restrict__ y) {
     using V = typename Mma<T>::V;
-    constexpr int N = PIECE<T>;
+    constexpr int N = PIECE<T>, MT = MT0 ? MT0 : 1;
     __shared__ f32x4 red[FEW_WAVES][MT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int nt = blockIdx.x;
@@ -304,21 +341,27 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_rows_kernel(const T* __res
     const bool there = o < MT * 256 && row < n && col < out;
     const int id = there ? adapter_of(ids, slot, slots, row, n) : -1;
     const int rank = id >= 0 ? slot[id].rank : 0;
-    const int per = (kt + FEW_WAVES - 1) / FEW_WAVES, k0 = min(kt, wave * per), k1 = min(kt, k0 + per);
+    const int per = (kt / 2 + FEW_WAVES - 1) / FEW_WAVES * 2, k0 = min(kt, wave * per), k1 = min(kt, k0 + per);
     const T* wp = w + (int64_t)nt * kt * (64 * N) + lane * N;
-    const T* xp[MT];
+    const T* xp[MT];  // rows past n are not there: their lanes read the last one, or the last tile's
 #pragma unroll
-    for (int m = 0; m < MT; ++m) xp[m] = x + (int64_t)min(m * 16 + (lane & 15), n - 1) * ldx + (lane >> 4) * N;
+    for (int m = 0; m < MT; ++m)
+        xp[m] = MT0 ? x + (int64_t)min(m, (n - 1) >> 4) * kt * (64 * N) + lane * N : x + (int64_t)min(lane & 15, n - 1) * in;
+    const int whole = MT0 ? kt : in / (2 * DEPTH<T>)*2;
+    auto piece = [&](int m, int k, bool all) -> V {
+        if constexpr (MT0 > 0) return load_piece(xp[m] + (int64_t)k * (64 * N));
+        else return row_piece(xp[m], in_of<T>(k, lane >> 4), in, all);
+    };
     f32x4 acc[MT] = {};
     constexpr int U = MT == 4 ? 4 : 8;  // loads in flight, by registers
     int k = k0;
-    for (; k + U <= k1; k += U) {
+    for (; k + U <= min(k1, whole); k += U) {
         V wv[U], xv[U][MT];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             wv[u] = load_piece(wp + (int64_t)(k + u) * (64 * N));
 #pragma unroll
-            for (int m = 0; m < MT; ++m) xv[u][m] = load_piece(xp[m] + (k + u) * DEPTH<T>);
+            for (int m = 0; m < MT; ++m) xv[u][m] = piece(m, k + u, true);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -329,7 +372,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_rows_kernel(const T* __res
     for (; k < k1; ++k) {
         const V wv = load_piece(wp + (int64_t)k * (64 * N));
 #pragma unroll
-        for (int m = 0; m < MT; ++m) acc[m] = Mma<T>::run(wv, load_piece(xp[m] + k * DEPTH<T>), acc[m]);
+        for (int m = 0; m < MT; ++m) acc[m] = Mma<T>::run(wv, piece(m, k, k < whole), acc[m]);
     }
 #pragma unroll
     for (int m = 0; m < MT; ++m) red[wave][m][lane] = acc[m];
@@ -403,7 +446,7 @@ __device__ __forceinline__ void spread() {
 
 // ADD: y is there already (f32), the adapters' part is added to it.
 template <class T, int BM, int BN, int WM, int WN, int NS, bool ADD>
-__global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const T* __restrict__ x, int ldx, int64_t n,
+__global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const T* __restrict__ x, int64_t n,
                                                            const T* __restrict__ w, int kt, int nts,
                                                            const T* __restrict__ bias, const T* __restrict__ b,
                                                            int64_t b_slot, int rk, const int32_t* __restrict__ ids,
@@ -443,7 +486,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const T* __restrict_
         const T* ws[Cf::WP];
 #pragma unroll
         for (int j = 0; j < Cf::XP; ++j)
-            xs[j] = x + row_at(row0 + (wave * Cf::XP + j) * 16 + (lane & 15)) * ldx + (lane >> 4) * N;
+            xs[j] = x + min(row0 / 16 + wave * Cf::XP + j, (n - 1) / 16) * kt * (64 * N);
 #pragma unroll
         for (int j = 0; j < Cf::WP; ++j) ws[j] = w + (int64_t)min(nt0 + wave * Cf::WP + j, nts - 1) * kt * (64 * N);
         auto fill = [&](int s, int buf) {
@@ -451,7 +494,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const T* __restrict_
 #pragma unroll
             for (int j = 0; j < Cf::XP; ++j)
                 __builtin_amdgcn_global_load_lds(
-                    (const void*)(xs[j] + s * DEPTH<T>),
+                    (const void*)(xs[j] + (int64_t)s * (64 * N) + lane * N),
                     (__attribute__((address_space(3))) void*)(base + (wave * Cf::XP + j) * 1024), 16, 0, 0);
 #pragma unroll
             for (int j = 0; j < Cf::WP; ++j)
@@ -612,12 +655,12 @@ AdapterShape adapter_shape(int32_t dtype, int32_t in, int32_t out, int32_t max_r
     return s;
 }
 
-void adapter_pack(int32_t dtype, const void* src, int rows, int cols, int tiles, int frags, bool outputs, void* dst) {
+void adapter_pack(int32_t dtype, const void* src, int rows, int cols, int tiles, int frags, int what, void* dst) {
     with_dtype(dtype, [&](auto zero) {
         using T = decltype(zero);
         const int64_t pieces = (int64_t)tiles * frags * 64;
         RVX_LAUNCH("adapter_pack", pack_kernel<T>, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, (const T*)src,
-                   rows, cols, pieces, frags, outputs, (T*)dst);
+                   rows, cols, pieces, frags, what, (T*)dst);
     });
 }
 
@@ -651,13 +694,6 @@ void adapter_forward(const AdapterArgs& g) {
         T* y = (T*)g.y;
         const int64_t n = g.n;
         const int cus = device().num_cus;
-        int ldx = s.in;
-        if (s.in != s.kt * DEPTH<T>) {
-            ldx = s.kt * DEPTH<T>;
-            T* padded = (T*)scratch_bytes("adapter_x", n * ldx * (int64_t)sizeof(T));
-            pad_rows<T>(x, n, s.in, ldx, padded);
-            x = padded;
-        }
         const bool few = n <= 64;
         Mid<T> t{};
         int32_t* perm = nullptr;
@@ -667,36 +703,58 @@ void adapter_forward(const AdapterArgs& g) {
                 t.f = scratch_f32("adapter_t", n * t.ld);
             } else {
                 perm = (int32_t*)scratch_bytes("adapter_rows", n * 4);
-                RVX_LAUNCH("adapter_group", group_rows_kernel, dim3(1), dim3(GROUP_THREADS), 0, g.ids, n, g.slot, s.slots,
-                           perm);
+                int bits = 1;
+                while (bits < GROUP_BITS && (1 << bits) <= s.slots) ++bits;
+                RVX_LAUNCH("adapter_group", group_rows_kernel, dim3((unsigned)((n + GROUP_ROWS - 1) / GROUP_ROWS)),
+                           dim3(GROUP_THREADS), 0, g.ids, n, s.slots, bits, perm);
                 const int64_t plane = n * t.ld;
                 t.hi = (T*)scratch_bytes("adapter_t", 2 * plane * (int64_t)sizeof(T) + n * 4);
                 t.lo = t.hi + plane;
                 t.back = __is_same(T, _Float16) ? (float*)(t.lo + plane) : nullptr;
             }
-            auto go = [&](auto sm, auto rt, auto waves, auto split) {
-                constexpr int SM = decltype(sm)::value, RT = decltype(rt)::value, W = decltype(waves)::value;
-                RVX_LAUNCH("adapter_shrink", (shrink_kernel<T, SM, RT, W, decltype(split)::value>),
-                           dim3((unsigned)((n + 16 * SM - 1) / (16 * SM)), few ? 16 : 1), dim3(64 * W), 0, x, ldx, n,
-                           (const int32_t*)perm, (const T*)g.a, s.a_slot, s.kt, g.ids, g.slot, s.slots, t);
-            };
-            auto by_rank = [&](auto sm, auto waves, auto split) {
-                if (s.rt == 1) go(sm, integral_constant<int, 1>{}, waves, split);
-                else if (s.rt == 2) go(sm, integral_constant<int, 2>{}, waves, split);
-                else if (s.rt == 4) go(sm, integral_constant<int, 4>{}, waves, split);
-                else go(sm, integral_constant<int, 8>{}, integral_constant<int, 8>{}, split);
-            };
-            if (few) by_rank(integral_constant<int, 1>{}, integral_constant<int, 16>{}, std::false_type{});
-            else if (n <= 2048) by_rank(integral_constant<int, 1>{}, integral_constant<int, 8>{}, std::true_type{});
-            else by_rank(integral_constant<int, 2>{}, integral_constant<int, 8>{}, std::true_type{});
+        }
+        // f32 through the split-f16 product: see below
+        bool split_gemm = false;
+        int ldx = s.kt * DEPTH<T>;
+        GemmOperand op{};
+        auto tiles = [&](int64_t bm, int64_t bn) { return (n + bm - 1) / bm * ((s.out + bn - 1) / bn); };
+        if constexpr (__is_same(T, float)) {
+            if (g.w_split && tiles(128, 128) >= cus) {
+                op = GemmOperand{x, ldx, nullptr, ldx, ldx};
+                op.Bh = (const _Float16*)g.w_split, op.Bh_plane = (int64_t)s.out * ldx, op.b_inv = g.w_inv;
+                split_gemm = gemm_h2_ok(n, s.out, op, nullptr);
+            }
+        }
+        const int64_t row_tiles = (n + 15) / 16;
+        // one row tile is read as it is: its 16-row loads cost less than another launch
+        T* packed = split_gemm || n <= 16 ? nullptr : (T*)scratch_bytes("adapter_x", row_tiles * s.kt * 1024);
+        auto shrink = [&](auto rt, auto waves, auto split, auto pack) {
+            constexpr int RT = decltype(rt)::value, W = decltype(waves)::value;
+            RVX_LAUNCH("adapter_shrink", (shrink_kernel<T, RT, W, decltype(split)::value, decltype(pack)::value>),
+                       dim3((unsigned)row_tiles, few && RT ? 16 : 1), dim3(64 * W), 0, x, s.in, n, (const int32_t*)perm,
+                       (const T*)g.a, s.a_slot, s.kt, g.ids, g.slot, s.slots, t, packed);
+        };
+        auto by_rank = [&](auto waves, auto split, auto pack) {
+            if (!g.ids) shrink(integral_constant<int, 0>{}, waves, split, std::true_type{});
+            else if (s.rt == 1) shrink(integral_constant<int, 1>{}, waves, split, pack);
+            else if (s.rt == 2) shrink(integral_constant<int, 2>{}, waves, split, pack);
+            else if (s.rt == 4) shrink(integral_constant<int, 4>{}, waves, split, pack);
+            else shrink(integral_constant<int, 8>{}, integral_constant<int, 8>{}, split, pack);
+        };
+        if (few) {
+            if (packed) by_rank(integral_constant<int, 16>{}, std::false_type{}, std::true_type{});
+            else if (g.ids) by_rank(integral_constant<int, 16>{}, std::false_type{}, std::false_type{});
+        } else {
+            if (packed) by_rank(integral_constant<int, 8>{}, std::true_type{}, std::true_type{});
+            else if (g.ids) by_rank(integral_constant<int, 8>{}, std::true_type{}, std::false_type{});
         }
         if (few) {
             auto go = [&](auto mt) {
                 constexpr int MT = decltype(mt)::value;
-                RVX_LAUNCH("adapter_few_rows", (few_rows_kernel<T, MT>), dim3(s.nt), dim3(64 * FEW_WAVES), 0, x, ldx, (int)n,
-                           w, s.kt, bias, b, s.b_slot, s.rk, g.ids, g.slot, s.slots, (const float*)t.f, t.ld, s.out, y);
+                RVX_LAUNCH("adapter_few_rows", (few_rows_kernel<T, MT>), dim3(s.nt), dim3(64 * FEW_WAVES), 0,
+                           packed ? (const T*)packed : x, s.in, (int)n, w, s.kt, bias, b, s.b_slot, s.rk, g.ids, g.slot, s.slots, (const float*)t.f, t.ld, s.out, y);
             };
-            if (n <= 16) go(integral_constant<int, 1>{});
+            if (n <= 16) go(integral_constant<int, 0>{});
             else if (n <= 32) go(integral_constant<int, 2>{});
             else go(integral_constant<int, 4>{});
             return;
@@ -706,20 +764,22 @@ void adapter_forward(const AdapterArgs& g) {
                           WN = decltype(wn)::value, NS = decltype(ns)::value;
             const int tm = (int)((n + BM - 1) / BM), tn = (s.out + BN - 1) / BN;
             RVX_LAUNCH("adapter_tile", (tile_kernel<T, BM, BN, WM, WN, NS, decltype(add)::value>), dim3((unsigned)(tm * tn)),
-                       dim3(64 * WM * WN), 0, x, ldx, n, w, s.kt, s.nt, bias, b, s.b_slot, s.rk, g.ids, (const int32_t*)perm,
+                       dim3(64 * WM * WN), 0, (const T*)packed, n, w, s.kt, s.nt, bias, b, s.b_slot, s.rk, g.ids, (const int32_t*)perm,
                        g.slot, s.slots, t, s.out, tm, tn, y);
         };
-        auto tiles = [&](int64_t bm, int64_t bn) { return (n + bm - 1) / bm * ((s.out + bn - 1) / bn); };
         if constexpr (__is_same(T, float)) {
             // The framework's split-f16 product has about twice the rate of f32 matrix instructions; it
             // takes its operands row-major and knows no adapters, so their part is added to y.
-            GemmOperand op{x, ldx, nullptr, ldx, ldx};
-            op.Bh = (const _Float16*)g.w_split, op.Bh_plane = (int64_t)s.out * ldx, op.b_inv = g.w_inv;
-            if (g.w_split && tiles(128, 128) >= cus && gemm_h2_ok(n, s.out, op, nullptr)) {
+            if (split_gemm) {
+                if (ldx != s.in) {
+                    float* padded = scratch_f32("adapter_x", n * ldx);
+                    pad_rows<float>(x, n, s.in, ldx, padded);
+                    op.A = padded;
+                }
                 GemmEpilogue ep;
                 ep.bias0 = bias;
                 float* scale = scratch_f32("gemm_auto_scale", n);
-                row_scale_h2(x, ldx, ldx, nullptr, 0, 0, n, scale);
+                row_scale_h2(op.A, ldx, ldx, nullptr, 0, 0, n, scale);
                 gemm_nt_h2(n, s.out, op, op.Bh, nullptr, nullptr, scale, op.b_inv, ep, y, s.out, "adapter_gemm");
                 if (g.ids)
                     go(integral_constant<int, 64>{}, integral_constant<int, 64>{}, integral_constant<int, 2>{},
@@ -735,7 +795,7 @@ void adapter_forward(const AdapterArgs& g) {
                integral_constant<int, 2>{}, integral_constant<int, 4>{}, std::false_type{});
         else
             go(integral_constant<int, 64>{}, integral_constant<int, 64>{}, integral_constant<int, 2>{},
-               integral_constant<int, 2>{}, integral_constant<int, 4>{}, std::false_type{});
+               integral_constant<int, 2>{}, integral_constant<int, 8>{}, std::false_type{});
     });
 }
 
