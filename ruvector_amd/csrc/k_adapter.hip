@@ -169,9 +169,10 @@ __global__ __launch_bounds__(GROUP_THREADS) void group_rows_kernel(const int32_t
 }
 
 // ---------------------------------------------------------------- t = s A x
-// What the projection reads of t. Few rows: f32, `f`. Tiles: pieces of T, hi + lo, 16 (bf16) or 22
+// What the projection reads of t. Few rows: f32, `f`, as FEW_PARTS parts to be added up. Tiles: pieces of T, hi + lo, 16 (bf16) or 22
 // (f16) bits of each value, so that t's rounding is far below y's (f32: hi alone); f16: a row whose
 // largest value is not in [2^-3, 2^15) is scaled by a power of two to [2^14, 2^15), undone by `back`.
+constexpr int FEW_PARTS = 4;
 template <class T>
 struct Mid {
     float* f;
@@ -209,7 +210,9 @@ __global__ __launch_bounds__(64 * WAVES) void shrink_kernel(const T* __restrict_
     const int mine = RT && lane < 16 && row0 + lane < n ? adapter_of(ids, slot, slots, my_row, n) : -1;
     unsigned long long todo = __ballot(mine >= 0);
     const T* xp = x + my_row * in;
-    const int per = (kt / 2 + WAVES - 1) / WAVES * 2, k0 = min(kt, wave * per), k1 = min(kt, k0 + per);
+    // several blocks may share the sum (gridDim.z): each then writes a part of t of its own
+    const int parts = WAVES * gridDim.z, part = wave + WAVES * blockIdx.z;
+    const int per = (kt / 2 + parts - 1) / parts * 2, k0 = min(kt, part * per), k1 = min(kt, k0 + per);
     const int whole = in / (2 * DEPTH<T>)*2;  // fragments without a zero
     T* to = packed + (int64_t)blockIdx.x * kt * (64 * N) + lane * N;
     bool pack = PACK && blockIdx.y == 0;
@@ -287,7 +290,7 @@ __global__ __launch_bounds__(64 * WAVES) void shrink_kernel(const T* __restrict_
                 if (__shfl(mine, lane & 15) == id) {
                     if constexpr (!SPLIT) {
 #pragma unroll
-                        for (int r = 0; r < RT; ++r) __builtin_memcpy(t.f + at * t.ld + r * 16 + (lane >> 4) * 4, v[r], 16);
+                        for (int r = 0; r < RT; ++r) __builtin_memcpy(t.f + (blockIdx.z * n + at) * t.ld + r * 16 + (lane >> 4) * 4, v[r], 16);
                     } else {
                         if (t.back && lane < 16) t.back[at] = down;
 #pragma unroll
@@ -384,7 +387,12 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_rows_kernel(const T* __res
         for (int p = 0; p * N < rank; ++p) {
             const V bv = load_piece(bp + ((p >> 2) * 64 + (p & 3) * 16) * N);
 #pragma unroll
-            for (int j = 0; j < N; ++j) d = fmaf(tp[p * N + j], (float)bv[j], d);
+            for (int j = 0; j < N; ++j) {
+                float tv = tp[p * N + j];
+#pragma unroll
+                for (int q = 1; q < FEW_PARTS; ++q) tv += tp[(int64_t)q * n * ldt + p * N + j];
+                d = fmaf(tv, (float)bv[j], d);
+            }
         }
     }
     __syncthreads();
@@ -700,7 +708,7 @@ void adapter_forward(const AdapterArgs& g) {
         if (g.ids) {
             t.ld = std::max(s.rk * DEPTH<T>, s.rt * 16);
             if (few) {
-                t.f = scratch_f32("adapter_t", n * t.ld);
+                t.f = scratch_f32("adapter_t", FEW_PARTS * n * t.ld);
             } else {
                 perm = (int32_t*)scratch_bytes("adapter_rows", n * 4);
                 int bits = 1;
@@ -726,12 +734,15 @@ void adapter_forward(const AdapterArgs& g) {
             }
         }
         const int64_t row_tiles = (n + 15) / 16;
-        // one row tile is read as it is: its 16-row loads cost less than another launch
-        T* packed = split_gemm || n <= 16 ? nullptr : (T*)scratch_bytes("adapter_x", row_tiles * s.kt * 1024);
+        // without adapters one row tile is read as it is: its 16-row loads cost less than another launch
+        T* packed = split_gemm || (n <= 16 && !g.ids) ? nullptr : (T*)scratch_bytes("adapter_x", row_tiles * s.kt * 1024);
+        // few row tiles: several blocks each, for the turns of different adapters and parts of the sum
+        const unsigned spare = (unsigned)std::max<int64_t>(1, std::min<int64_t>(16, 2 * cus / row_tiles));
+        const unsigned turns = g.ids ? few ? 16 : spare : 1, sums = few ? FEW_PARTS : g.ids ? 1 : std::min(spare, 4u);
         auto shrink = [&](auto rt, auto waves, auto split, auto pack) {
             constexpr int RT = decltype(rt)::value, W = decltype(waves)::value;
             RVX_LAUNCH("adapter_shrink", (shrink_kernel<T, RT, W, decltype(split)::value, decltype(pack)::value>),
-                       dim3((unsigned)row_tiles, few && RT ? 16 : 1), dim3(64 * W), 0, x, s.in, n, (const int32_t*)perm,
+                       dim3((unsigned)row_tiles, turns, sums), dim3(64 * W), 0, x, s.in, n, (const int32_t*)perm,
                        (const T*)g.a, s.a_slot, s.kt, g.ids, g.slot, s.slots, t, packed);
         };
         auto by_rank = [&](auto waves, auto split, auto pack) {
@@ -742,11 +753,14 @@ void adapter_forward(const AdapterArgs& g) {
             else shrink(integral_constant<int, 8>{}, integral_constant<int, 8>{}, split, pack);
         };
         if (few) {
-            if (packed) by_rank(integral_constant<int, 16>{}, std::false_type{}, std::true_type{});
-            else if (g.ids) by_rank(integral_constant<int, 16>{}, std::false_type{}, std::false_type{});
+            if (packed) by_rank(integral_constant<int, 8>{}, std::false_type{}, std::true_type{});
         } else {
-            if (packed) by_rank(integral_constant<int, 8>{}, std::true_type{}, std::true_type{});
-            else if (g.ids) by_rank(integral_constant<int, 8>{}, std::true_type{}, std::false_type{});
+            auto many = [&](auto waves) {
+                if (packed) by_rank(waves, std::true_type{}, std::true_type{});
+                else if (g.ids) by_rank(waves, std::true_type{}, std::false_type{});
+            };
+            if (row_tiles < cus) many(integral_constant<int, 16>{});
+            else many(integral_constant<int, 8>{});
         }
         if (few) {
             auto go = [&](auto mt) {
@@ -754,7 +768,8 @@ void adapter_forward(const AdapterArgs& g) {
                 RVX_LAUNCH("adapter_few_rows", (few_rows_kernel<T, MT>), dim3(s.nt), dim3(64 * FEW_WAVES), 0,
                            packed ? (const T*)packed : x, s.in, (int)n, w, s.kt, bias, b, s.b_slot, s.rk, g.ids, g.slot, s.slots, (const float*)t.f, t.ld, s.out, y);
             };
-            if (n <= 16) go(integral_constant<int, 0>{});
+            if (!packed) go(integral_constant<int, 0>{});
+            else if (n <= 16) go(integral_constant<int, 1>{});
             else if (n <= 32) go(integral_constant<int, 2>{});
             else go(integral_constant<int, 4>{});
             return;
@@ -789,10 +804,10 @@ void adapter_forward(const AdapterArgs& g) {
         }
         if (tiles(256, 256) >= cus)
             go(integral_constant<int, 256>{}, integral_constant<int, 256>{}, integral_constant<int, 2>{},
-               integral_constant<int, 4>{}, integral_constant<int, 4>{}, std::false_type{});
+               integral_constant<int, 4>{}, integral_constant<int, 5>{}, std::false_type{});
         else if (tiles(128, 128) >= cus)
             go(integral_constant<int, 128>{}, integral_constant<int, 128>{}, integral_constant<int, 2>{},
-               integral_constant<int, 2>{}, integral_constant<int, 4>{}, std::false_type{});
+               integral_constant<int, 2>{}, integral_constant<int, 8>{}, std::false_type{});
         else
             go(integral_constant<int, 64>{}, integral_constant<int, 64>{}, integral_constant<int, 2>{},
                integral_constant<int, 2>{}, integral_constant<int, 8>{}, std::false_type{});
