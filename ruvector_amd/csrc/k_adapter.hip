@@ -178,6 +178,7 @@ struct Mid {
     float* f;
     T *hi, *lo;
     float* back;
+    int32_t* eff;  // few rows: a row's adapter and its rank, id * 256 + rank, -1 = none
     int ld;
 };
 
@@ -208,6 +209,8 @@ __global__ __launch_bounds__(64 * WAVES) void shrink_kernel(const T* __restrict_
     const int64_t place = min(row0 + (lane & 15), n - 1);
     const int64_t my_row = perm ? perm[place] : place;
     const int mine = RT && lane < 16 && row0 + lane < n ? adapter_of(ids, slot, slots, my_row, n) : -1;
+    if (RT && !SPLIT && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x < 16 && row0 + lane < n)
+        t.eff[row0 + lane] = mine < 0 ? -1 : mine * 256 + slot[mine].rank;
     unsigned long long todo = __ballot(mine >= 0);
     const T* xp = x + my_row * in;
     // several blocks may share the sum (gridDim.z): each then writes a part of t of its own
@@ -330,8 +333,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_rows_kernel(const T* __res
                                                                  const T* __restrict__ w, int kt,
                                                                  const T* __restrict__ bias, const T* __restrict__ b,
                                                                  int64_t b_slot, int rk,
-                                                                 const int32_t* __restrict__ ids,
-                                                                 const AdapterSlot* __restrict__ slot, int slots,
+                                                                 const int32_t* __restrict__ eff,
                                                                  const float* __restrict__ t, int ldt, int out,
                                                                  T* __restrict__ y) {
     using V = typename Mma<T>::V;
@@ -342,8 +344,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_rows_kernel(const T* __res
     // this thread's output: o = (row tile, row, output), one each (16 rows: of the first 256 threads)
     const int o = threadIdx.x, row = o >> 4, c = o & 15, col = out_of(nt, c);
     const bool there = o < MT * 256 && row < n && col < out;
-    const int id = there ? adapter_of(ids, slot, slots, row, n) : -1;
-    const int rank = id >= 0 ? slot[id].rank : 0;
+    const int who = there && eff ? eff[row] : -1;
     const int per = (kt / 2 + FEW_WAVES - 1) / FEW_WAVES * 2, k0 = min(kt, wave * per), k1 = min(kt, k0 + per);
     const T* wp = w + (int64_t)nt * kt * (64 * N) + lane * N;
     const T* xp[MT];  // rows past n are not there: their lanes read the last one, or the last tile's
@@ -381,7 +382,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_rows_kernel(const T* __res
     for (int m = 0; m < MT; ++m) red[wave][m][lane] = acc[m];
     // B's row of this output: the piece of ranks p N .. is lane (p % 4) * 16 + c of fragment p / 4
     float d = 0.0f;
-    if (id >= 0) {
+    if (who >= 0) {
+        const int id = who >> 8, rank = who & 255;
         const T* bp = b + id * b_slot + (int64_t)nt * rk * (64 * N) + c * N;
         const float* tp = t + (int64_t)row * ldt;
         for (int p = 0; p * N < rank; ++p) {
@@ -406,17 +408,19 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_rows_kernel(const T* __res
 }
 
 // ---------------------------------------------------------------- many rows
-// A block: BM rows (of the permutation) x BN outputs; WM x WN waves; the sum in stages one fragment
-// deep, NS of which are in LDS or on their way to it (copied there without registers). While a stage is
-// multiplied from registers, the next one is read into others. Behind a stage's one barrier everybody
-// has read it, so its place is free for stage s + NS, and has the next: the copies of NS - 2 stages
-// more may still be on their way, which is what hides their latency.
-template <int BM, int BN, int WM, int WN, int NS>
+// A block: BM rows (of the permutation) x BN outputs; WM x WN waves; the sum in stages KF fragments
+// deep, NS of which are in LDS or on their way to it (copied there without registers).
+// KF == 1, large tiles: while a stage is multiplied from registers, the next one is read into others.
+// Behind a stage's one barrier everybody has read it, so its place is free for stage s + NS, and has
+// the next: the copies of NS - 2 stages more may still be on their way, which hides their latency.
+// KF > 1, small tiles: a fragment is a few products only, so a barrier serves KF of them; behind it
+// stage s has arrived and s - 1 is read, whose place the copies of s + NS - 1 take.
+template <int BM, int BN, int WM, int WN, int NS, int KF>
 struct TileCfg {
     static constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
     static constexpr int XF = BM / 16, WF = BN / 16;          // 1-KiB fragments of a stage
-    static constexpr int XP = XF / WAVES, WP = WF / WAVES;    // copied by each wave
-    static constexpr int STAGE = (XF + WF) * 1024;
+    static constexpr int XP = XF / WAVES, WP = WF / WAVES;    // copied by each wave, of each fragment's depth
+    static constexpr int STAGE = (XF + WF) * KF * 1024;
     static_assert(XF % WAVES == 0 && WF % WAVES == 0 && TN % 2 == 0);
 };
 
@@ -453,7 +457,7 @@ __device__ __forceinline__ void spread() {
 }
 
 // ADD: y is there already (f32), the adapters' part is added to it.
-template <class T, int BM, int BN, int WM, int WN, int NS, bool ADD>
+template <class T, int BM, int BN, int WM, int WN, int NS, int KF, bool ADD>
 __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const T* __restrict__ x, int64_t n,
                                                            const T* __restrict__ w, int kt, int nts,
                                                            const T* __restrict__ bias, const T* __restrict__ b,
@@ -461,7 +465,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const T* __restrict_
                                                            const int32_t* __restrict__ perm,
                                                            const AdapterSlot* __restrict__ slot, int slots, Mid<T> t,
                                                            int out, int tiles_m, int tiles_n, T* y) {
-    using Cf = TileCfg<BM, BN, WM, WN, NS>;
+    using Cf = TileCfg<BM, BN, WM, WN, NS, KF>;
     using V = typename Mma<T>::V;
     constexpr int N = PIECE<T>, TM = Cf::TM, TN = Cf::TN, MMA = sizeof(T) == 2 ? 1 : 4;
     __shared__ __align__(16) unsigned char lds[ADD ? 16 : NS * Cf::STAGE];
@@ -497,23 +501,28 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const T* __restrict_
             xs[j] = x + min(row0 / 16 + wave * Cf::XP + j, (n - 1) / 16) * kt * (64 * N);
 #pragma unroll
         for (int j = 0; j < Cf::WP; ++j) ws[j] = w + (int64_t)min(nt0 + wave * Cf::WP + j, nts - 1) * kt * (64 * N);
-        auto fill = [&](int s, int buf) {
-            unsigned char* base = lds + buf * Cf::STAGE;
+        // fragment k of the sum, the f-th of its stage: x's tiles, then W's
+        auto copy = [&](int k, int buf, int f) {
+            unsigned char* base = lds + buf * Cf::STAGE + f * (Cf::XF + Cf::WF) * 1024;
 #pragma unroll
             for (int j = 0; j < Cf::XP; ++j)
                 __builtin_amdgcn_global_load_lds(
-                    (const void*)(xs[j] + (int64_t)s * (64 * N) + lane * N),
+                    (const void*)(xs[j] + (int64_t)k * (64 * N) + lane * N),
                     (__attribute__((address_space(3))) void*)(base + (wave * Cf::XP + j) * 1024), 16, 0, 0);
 #pragma unroll
             for (int j = 0; j < Cf::WP; ++j)
                 __builtin_amdgcn_global_load_lds(
-                    (const void*)(ws[j] + (int64_t)s * (64 * N) + lane * N),
+                    (const void*)(ws[j] + (int64_t)k * (64 * N) + lane * N),
                     (__attribute__((address_space(3))) void*)(base + (Cf::XF + wave * Cf::WP + j) * 1024), 16, 0, 0);
         };
+        auto fill = [&](int s, int buf) {  // past the end: copies of the last fragment, which nobody reads
+#pragma unroll
+            for (int f = 0; f < KF; ++f) copy(min(s * KF + f, kt - 1), buf, f);
+        };
         V xv[2][TM], wv[2][TN];
-        auto read = [&](auto to, int buf) {
+        auto read = [&](auto to, int buf, int f) {
             constexpr int h = decltype(to)::value;
-            const unsigned char* base = lds + buf * Cf::STAGE + lane * 16;
+            const unsigned char* base = lds + buf * Cf::STAGE + f * (Cf::XF + Cf::WF) * 1024 + lane * 16;
 #pragma unroll
             for (int j = 0; j < TN; ++j) wv[h][j] = *(const V*)(base + (Cf::XF + wn * TN + j) * 1024);
 #pragma unroll
@@ -527,36 +536,61 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const T* __restrict_
                 for (int j = 0; j < TN; ++j) acc[i][j] = Mma<T>::run(wv[h][j], xv[h][i], acc[i][j]);
         };
         constexpr int COPIES = Cf::XP + Cf::WP;
-        for (int s = 0; s < NS && s < kt; ++s) fill(s, s);
-        wait_and_meet<0>();
-        read(std::integral_constant<int, 0>{}, 0);
-        int s = 0, buf = 0;
-        auto step = [&](auto at, bool full) {  // stage s is in registers, or on its way from LDS
-            constexpr int h = decltype(at)::value;
-            const int next = buf + 1 == NS ? 0 : buf + 1;
-            if (full) {
-                wait_and_meet<(NS - 2) * COPIES>();
-                fill(s + NS, buf);
-                read(std::integral_constant<int, 1 - h>{}, next);
-                multiply(at);
-                spread<TM + TN, COPIES, TM * TN * MMA>();
-                __builtin_amdgcn_sched_barrier(0);
-            } else {
-                wait_and_meet<0>();
-                if (s + NS < kt) fill(s + NS, buf);
-                if (s + 1 < kt) read(std::integral_constant<int, 1 - h>{}, next);
-                multiply(at);
+        using std::integral_constant;
+        if constexpr (KF > 1) {
+            const int stages = (kt + KF - 1) / KF;
+#pragma unroll
+            for (int s = 0; s < NS - 1; ++s) fill(s, s);  // as many as are counted below, there or not
+            int buf = 0, last = NS - 1;
+            for (int s = 0; s < stages; ++s) {
+                wait_and_meet<(NS - 2) * COPIES * KF>();
+                fill(s + NS - 1, last);
+                const int depth = min(KF, kt - s * KF);  // even
+                read(integral_constant<int, 0>{}, buf, 0);
+#pragma unroll
+                for (int f = 0; f < KF; f += 2) {
+                    if (f >= depth) break;
+                    read(integral_constant<int, 1>{}, buf, f + 1);
+                    multiply(integral_constant<int, 0>{});
+                    if (f + 2 < depth) read(integral_constant<int, 0>{}, buf, f + 2);
+                    multiply(integral_constant<int, 1>{});
+                }
+                last = buf;
+                buf = buf + 1 == NS ? 0 : buf + 1;
             }
-            buf = next;
-            ++s;
-        };
-        for (; s + 1 + NS < kt;) {  // kt is even
-            step(std::integral_constant<int, 0>{}, true);
-            step(std::integral_constant<int, 1>{}, true);
-        }
-        for (; s < kt;) {
-            step(std::integral_constant<int, 0>{}, false);
-            step(std::integral_constant<int, 1>{}, false);
+            __builtin_amdgcn_s_waitcnt(0xf << 8 | 7 << 4);  // vmcnt 0: no copy outlives the loop
+        } else {
+            for (int s = 0; s < NS && s < kt; ++s) fill(s, s);
+            wait_and_meet<0>();
+            read(integral_constant<int, 0>{}, 0, 0);
+            int s = 0, buf = 0;
+            auto step = [&](auto at, bool full) {  // stage s is in registers, or on its way from LDS
+                constexpr int h = decltype(at)::value;
+                const int next = buf + 1 == NS ? 0 : buf + 1;
+                if (full) {
+                    wait_and_meet<(NS - 2) * COPIES>();
+                    fill(s + NS, buf);
+                    read(integral_constant<int, 1 - h>{}, next, 0);
+                    multiply(at);
+                    spread<TM + TN, COPIES, TM * TN * MMA>();
+                    __builtin_amdgcn_sched_barrier(0);
+                } else {
+                    wait_and_meet<0>();
+                    if (s + NS < kt) fill(s + NS, buf);
+                    if (s + 1 < kt) read(integral_constant<int, 1 - h>{}, next, 0);
+                    multiply(at);
+                }
+                buf = next;
+                ++s;
+            };
+            for (; s + 1 + NS < kt;) {  // kt is even
+                step(integral_constant<int, 0>{}, true);
+                step(integral_constant<int, 1>{}, true);
+            }
+            for (; s < kt;) {
+                step(integral_constant<int, 0>{}, false);
+                step(integral_constant<int, 1>{}, false);
+            }
         }
     }
 
@@ -708,7 +742,8 @@ void adapter_forward(const AdapterArgs& g) {
         if (g.ids) {
             t.ld = std::max(s.rk * DEPTH<T>, s.rt * 16);
             if (few) {
-                t.f = scratch_f32("adapter_t", FEW_PARTS * n * t.ld);
+                t.f = scratch_f32("adapter_t", FEW_PARTS * n * t.ld + n);
+                t.eff = (int32_t*)(t.f + FEW_PARTS * n * t.ld);
             } else {
                 perm = (int32_t*)scratch_bytes("adapter_rows", n * 4);
                 int bits = 1;
@@ -766,7 +801,7 @@ void adapter_forward(const AdapterArgs& g) {
             auto go = [&](auto mt) {
                 constexpr int MT = decltype(mt)::value;
                 RVX_LAUNCH("adapter_few_rows", (few_rows_kernel<T, MT>), dim3(s.nt), dim3(64 * FEW_WAVES), 0,
-                           packed ? (const T*)packed : x, s.in, (int)n, w, s.kt, bias, b, s.b_slot, s.rk, g.ids, g.slot, s.slots, (const float*)t.f, t.ld, s.out, y);
+                           packed ? (const T*)packed : x, s.in, (int)n, w, s.kt, bias, b, s.b_slot, s.rk, (const int32_t*)t.eff, (const float*)t.f, t.ld, s.out, y);
             };
             if (!packed) go(integral_constant<int, 0>{});
             else if (n <= 16) go(integral_constant<int, 1>{});
@@ -774,11 +809,12 @@ void adapter_forward(const AdapterArgs& g) {
             else go(integral_constant<int, 4>{});
             return;
         }
-        auto go = [&](auto bm, auto bn, auto wm, auto wn, auto ns, auto add) {
+        auto go = [&](auto bm, auto bn, auto wm, auto wn, auto ns, auto kf, auto add) {
             constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WM = decltype(wm)::value,
                           WN = decltype(wn)::value, NS = decltype(ns)::value;
             const int tm = (int)((n + BM - 1) / BM), tn = (s.out + BN - 1) / BN;
-            RVX_LAUNCH("adapter_tile", (tile_kernel<T, BM, BN, WM, WN, NS, decltype(add)::value>), dim3((unsigned)(tm * tn)),
+            RVX_LAUNCH("adapter_tile", (tile_kernel<T, BM, BN, WM, WN, NS, decltype(kf)::value, decltype(add)::value>),
+                       dim3((unsigned)(tm * tn)),
                        dim3(64 * WM * WN), 0, (const T*)packed, n, w, s.kt, s.nt, bias, b, s.b_slot, s.rk, g.ids, (const int32_t*)perm,
                        g.slot, s.slots, t, s.out, tm, tn, y);
         };
@@ -798,19 +834,19 @@ void adapter_forward(const AdapterArgs& g) {
                 gemm_nt_h2(n, s.out, op, op.Bh, nullptr, nullptr, scale, op.b_inv, ep, y, s.out, "adapter_gemm");
                 if (g.ids)
                     go(integral_constant<int, 64>{}, integral_constant<int, 64>{}, integral_constant<int, 2>{},
-                       integral_constant<int, 2>{}, integral_constant<int, 2>{}, std::true_type{});
+                       integral_constant<int, 2>{}, integral_constant<int, 2>{}, integral_constant<int, 1>{}, std::true_type{});
                 return;
             }
         }
         if (tiles(256, 256) >= cus)
             go(integral_constant<int, 256>{}, integral_constant<int, 256>{}, integral_constant<int, 2>{},
-               integral_constant<int, 4>{}, integral_constant<int, 5>{}, std::false_type{});
+               integral_constant<int, 4>{}, integral_constant<int, 4>{}, integral_constant<int, 1>{}, std::false_type{});
         else if (tiles(128, 128) >= cus)
             go(integral_constant<int, 128>{}, integral_constant<int, 128>{}, integral_constant<int, 2>{},
-               integral_constant<int, 2>{}, integral_constant<int, 8>{}, std::false_type{});
+               integral_constant<int, 2>{}, integral_constant<int, 4>{}, integral_constant<int, 2>{}, std::false_type{});
         else
             go(integral_constant<int, 64>{}, integral_constant<int, 64>{}, integral_constant<int, 2>{},
-               integral_constant<int, 2>{}, integral_constant<int, 8>{}, std::false_type{});
+               integral_constant<int, 2>{}, integral_constant<int, 4>{}, integral_constant<int, 2>{}, std::false_type{});
     });
 }
 
