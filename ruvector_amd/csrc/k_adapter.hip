@@ -16,7 +16,6 @@
 // are interleaved by pieces (`in_of`): a row's two pieces of one lane are neighbours, and the loads of
 // a pair touch whole 128-byte lines of x.
 #include "adapter.hpp"
-#include "kernels.hpp"
 
 namespace rvx {
 namespace {
@@ -88,17 +87,6 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ src, in
 #pragma unroll
     for (int j = 0; j < N; ++j) v[j] = row < rows && col + j < cols ? src[(int64_t)row * cols + col + j] : (T)0.0f;
     __builtin_memcpy(dst + p * N, v, 16);
-}
-
-// rows of x with zeros behind them, up to whole pairs of fragments
-template <class T>
-__global__ __launch_bounds__(256) void pad_kernel(const T* __restrict__ x, int64_t n, int in, int ld, T* __restrict__ out) {
-    const int64_t total = n * ld;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / ld;
-        const int c = (int)(i - r * ld);
-        out[i] = c < in ? x[r * in + c] : (T)0.0f;
-    }
 }
 
 __device__ __forceinline__ int adapter_of(const int32_t* ids, const AdapterSlot* slot, int slots, int64_t row, int64_t n) {
@@ -322,6 +310,58 @@ __global__ __launch_bounds__(64 * WAVES) void shrink_kernel(const T* __restrict_
     }
 }
 
+// ---------------------------------------------------------------- f32 as two halves
+// f32 products of many rows run on the f16 matrix instructions, 16 times the f32 ones' rate: each row
+// of x and of W is scaled by a power of two to a largest value in [2^14, 2^15) and split into hi + lo,
+// 22 bits of the row's largest values and 2^-39 of them at least of the others, and three products
+// hi hi + hi lo + lo hi give x w within about 2^-22. Fragment q of hi lies beside that of lo. inv: 1 /
+// scale. One wave a row.
+template <bool WEIGHT>
+__global__ __launch_bounds__(1024) void split_kernel(const float* __restrict__ x, int in, int64_t rows,
+                                                    const int32_t* __restrict__ perm, int ktq,
+                                                    _Float16* __restrict__ out, float* __restrict__ inv) {
+    const int lane = threadIdx.x & 63, m = threadIdx.x >> 6;
+    const int64_t place = WEIGHT ? out_of(blockIdx.x, m) : (int64_t)blockIdx.x * 16 + m;
+    const bool there = place < rows;
+    const float* row = x + (there ? perm ? perm[place] : place : 0) * in;
+    auto piece = [&](int c, float (&v)[8]) {
+        if (there && c + 8 <= in) __builtin_memcpy(v, row + c, 32);
+        else
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = there && c + j < in ? row[c + j] : 0.0f;
+    };
+    float most = 0.0f;
+    const int pieces = ktq * 4;
+#pragma unroll 4
+    for (int p = lane; p < pieces; p += 64) {
+        float v[8];
+        piece(p * 8, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(v[j]));
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
+    const float scale = h2_scale_dev(most);
+    if (there && lane == 0) inv[place] = 1.0f / scale;
+#pragma unroll 2
+    for (int p = lane; p < pieces; p += 64) {
+        float v[8];
+        piece(p * 8, v);
+        f16x8 hi, lo;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float s = v[j] * scale;
+            hi[j] = (_Float16)s;
+            lo[j] = (_Float16)(s - (float)hi[j]);
+        }
+        // the inverse of in_of: 8 pieces a pair of fragments, two by two of a lane
+        const int q = (p >> 3) * 2 + (p & 1), to = ((p & 7) >> 1) * 16 + m;
+        _Float16* o = out + (((int64_t)blockIdx.x * ktq + q) * 2) * 512 + to * 8;
+        __builtin_memcpy(o, &hi, 16);
+        __builtin_memcpy(o + 512, &lo, 16);
+    }
+}
+
 // ---------------------------------------------------------------- few rows
 // A block: a fragment tile's 16 outputs for all (<= 16 MT) rows; its waves split the sum and join in
 // LDS. Bound by reading W once.
@@ -456,10 +496,11 @@ __device__ __forceinline__ void spread() {
 #endif
 }
 
-// ADD: y is there already (f32), the adapters' part is added to it.
-template <class T, int BM, int BN, int WM, int WN, int NS, int KF, bool ADD>
-__global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const T* __restrict__ x, int64_t n,
-                                                           const T* __restrict__ w, int kt, int nts,
+// P: the products' type; _Float16 with T = float: hi and lo fragments in turn, KF = 2.
+template <class T, class P, int BM, int BN, int WM, int WN, int NS, int KF>
+__global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const P* __restrict__ x, const float* __restrict__ x_inv,
+                                                           int64_t n, const P* __restrict__ w,
+                                                           const float* __restrict__ w_inv, int kt, int nts,
                                                            const T* __restrict__ bias, const T* __restrict__ b,
                                                            int64_t b_slot, int rk, const int32_t* __restrict__ ids,
                                                            const int32_t* __restrict__ perm,
@@ -467,8 +508,11 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const T* __restrict_
                                                            int out, int tiles_m, int tiles_n, T* y) {
     using Cf = TileCfg<BM, BN, WM, WN, NS, KF>;
     using V = typename Mma<T>::V;
-    constexpr int N = PIECE<T>, TM = Cf::TM, TN = Cf::TN, MMA = sizeof(T) == 2 ? 1 : 4;
-    __shared__ __align__(16) unsigned char lds[ADD ? 16 : NS * Cf::STAGE];
+    using PV = typename Mma<P>::V;
+    constexpr bool HALVES = !__is_same(T, P);
+    static_assert(!HALVES || KF == 2);
+    constexpr int N = PIECE<T>, TM = Cf::TM, TN = Cf::TN;
+    __shared__ __align__(16) unsigned char lds[NS * Cf::STAGE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave - wm * WN;
     // Blocks go to the 8 XCDs in turn: block i of XCD d is the i-th tile of the d-th part, so that an
@@ -489,51 +533,52 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const T* __restrict_
         return perm ? perm[p] : p;
     };
     f32x4 acc[TM][TN];
-    if constexpr (!ADD) {
+    {
+        constexpr int UNIT = 64 * PIECE<P>;  // elements of a fragment
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
             for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-        const T* xs[Cf::XP];
-        const T* ws[Cf::WP];
+        const P* xs[Cf::XP];
+        const P* ws[Cf::WP];
 #pragma unroll
         for (int j = 0; j < Cf::XP; ++j)
-            xs[j] = x + min(row0 / 16 + wave * Cf::XP + j, (n - 1) / 16) * kt * (64 * N);
+            xs[j] = x + min(row0 / 16 + wave * Cf::XP + j, (n - 1) / 16) * kt * UNIT;
 #pragma unroll
-        for (int j = 0; j < Cf::WP; ++j) ws[j] = w + (int64_t)min(nt0 + wave * Cf::WP + j, nts - 1) * kt * (64 * N);
+        for (int j = 0; j < Cf::WP; ++j) ws[j] = w + (int64_t)min(nt0 + wave * Cf::WP + j, nts - 1) * kt * UNIT;
         // fragment k of the sum, the f-th of its stage: x's tiles, then W's
         auto copy = [&](int k, int buf, int f) {
             unsigned char* base = lds + buf * Cf::STAGE + f * (Cf::XF + Cf::WF) * 1024;
 #pragma unroll
             for (int j = 0; j < Cf::XP; ++j)
                 __builtin_amdgcn_global_load_lds(
-                    (const void*)(xs[j] + (int64_t)k * (64 * N) + lane * N),
+                    (const void*)(xs[j] + (int64_t)k * UNIT + lane * PIECE<P>),
                     (__attribute__((address_space(3))) void*)(base + (wave * Cf::XP + j) * 1024), 16, 0, 0);
 #pragma unroll
             for (int j = 0; j < Cf::WP; ++j)
                 __builtin_amdgcn_global_load_lds(
-                    (const void*)(ws[j] + (int64_t)k * (64 * N) + lane * N),
+                    (const void*)(ws[j] + (int64_t)k * UNIT + lane * PIECE<P>),
                     (__attribute__((address_space(3))) void*)(base + (Cf::XF + wave * Cf::WP + j) * 1024), 16, 0, 0);
         };
         auto fill = [&](int s, int buf) {  // past the end: copies of the last fragment, which nobody reads
 #pragma unroll
             for (int f = 0; f < KF; ++f) copy(min(s * KF + f, kt - 1), buf, f);
         };
-        V xv[2][TM], wv[2][TN];
+        PV xv[2][TM], wv[2][TN];
         auto read = [&](auto to, int buf, int f) {
             constexpr int h = decltype(to)::value;
             const unsigned char* base = lds + buf * Cf::STAGE + f * (Cf::XF + Cf::WF) * 1024 + lane * 16;
 #pragma unroll
-            for (int j = 0; j < TN; ++j) wv[h][j] = *(const V*)(base + (Cf::XF + wn * TN + j) * 1024);
+            for (int j = 0; j < TN; ++j) wv[h][j] = *(const PV*)(base + (Cf::XF + wn * TN + j) * 1024);
 #pragma unroll
-            for (int i = 0; i < TM; ++i) xv[h][i] = *(const V*)(base + (wm * TM + i) * 1024);
+            for (int i = 0; i < TM; ++i) xv[h][i] = *(const PV*)(base + (wm * TM + i) * 1024);
         };
-        auto multiply = [&](auto from) {
-            constexpr int h = decltype(from)::value;
+        auto multiply = [&](auto from, auto other) {
+            constexpr int h = decltype(from)::value, o = decltype(other)::value;
 #pragma unroll
             for (int i = 0; i < TM; ++i)
 #pragma unroll
-                for (int j = 0; j < TN; ++j) acc[i][j] = Mma<T>::run(wv[h][j], xv[h][i], acc[i][j]);
+                for (int j = 0; j < TN; ++j) acc[i][j] = Mma<P>::run(wv[h][j], xv[o][i], acc[i][j]);
         };
         constexpr int COPIES = Cf::XP + Cf::WP;
         using std::integral_constant;
@@ -551,9 +596,14 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const T* __restrict_
                 for (int f = 0; f < KF; f += 2) {
                     if (f >= depth) break;
                     read(integral_constant<int, 1>{}, buf, f + 1);
-                    multiply(integral_constant<int, 0>{});
+                    multiply(integral_constant<int, 0>{}, integral_constant<int, 0>{});
                     if (f + 2 < depth) read(integral_constant<int, 0>{}, buf, f + 2);
-                    multiply(integral_constant<int, 1>{});
+                    if constexpr (HALVES) {
+                        multiply(integral_constant<int, 0>{}, integral_constant<int, 1>{});
+                        multiply(integral_constant<int, 1>{}, integral_constant<int, 0>{});
+                    } else {
+                        multiply(integral_constant<int, 1>{}, integral_constant<int, 1>{});
+                    }
                 }
                 last = buf;
                 buf = buf + 1 == NS ? 0 : buf + 1;
@@ -571,14 +621,14 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const T* __restrict_
                     wait_and_meet<(NS - 2) * COPIES>();
                     fill(s + NS, buf);
                     read(integral_constant<int, 1 - h>{}, next, 0);
-                    multiply(at);
-                    spread<TM + TN, COPIES, TM * TN * MMA>();
+                    multiply(at, at);
+                    spread<TM + TN, COPIES, TM * TN>();
                     __builtin_amdgcn_sched_barrier(0);
                 } else {
                     wait_and_meet<0>();
                     if (s + NS < kt) fill(s + NS, buf);
                     if (s + 1 < kt) read(integral_constant<int, 1 - h>{}, next, 0);
-                    multiply(at);
+                    multiply(at, at);
                 }
                 buf = next;
                 ++s;
@@ -605,16 +655,18 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const T* __restrict_
         if (place >= n) row[i] = -1;
     }
     const int col0 = ntw * 16 + (lane >> 4) * 8;  // of the pair j, j + 1: col0 + j * 16 ..
-    if constexpr (ADD) {
+    if constexpr (HALVES) {
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
+        for (int i = 0; i < TM; ++i) {
+            const float xi = row[i] >= 0 ? x_inv[row0 + (wm * TM + i) * 16 + (lane & 15)] : 0.0f;
 #pragma unroll
             for (int j = 0; j < TN; ++j)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int col = col0 + (j >> 1) * 32 + (j & 1) * 4 + r;
-                    acc[i][j][r] = row[i] >= 0 && col < out ? (float)y[row[i] * out + col] : 0.0f;
+                    acc[i][j][r] *= xi * (col < out ? w_inv[col] : 0.0f);
                 }
+        }
     }
     if (ids) {
         float back[TM];
@@ -665,7 +717,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const T* __restrict_
         const int col = col0 + j * 16;
         float bs[8];
 #pragma unroll
-        for (int r = 0; r < 8; ++r) bs[r] = !ADD && bias && col + r < out ? (float)bias[col + r] : 0.0f;
+        for (int r = 0; r < 8; ++r) bs[r] = bias && col + r < out ? (float)bias[col + r] : 0.0f;
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
             T v[8];
@@ -682,6 +734,8 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const T* __restrict_
 }
 
 }  // namespace
+
+static int split_frags(int in) { return (in + 63) / 64 * 2; }  // 32 deep, an even number
 
 AdapterShape adapter_shape(int32_t dtype, int32_t in, int32_t out, int32_t max_rank, int32_t slots) {
     const int piece = 16 / dtype_size(dtype), depth = 4 * piece;
@@ -706,25 +760,12 @@ void adapter_pack(int32_t dtype, const void* src, int rows, int cols, int tiles,
     });
 }
 
-template <class T>
-static void pad_rows(const T* x, int64_t n, int in, int ld, T* out) {
-    RVX_LAUNCH("adapter_pad", pad_kernel<T>,
-               dim3((unsigned)std::min<int64_t>((n * ld + 255) / 256, 16LL * device().num_cus)), dim3(256), 0, x, n, in, ld,
-               out);
-}
-
 int64_t adapter_split_bytes(const AdapterShape& s) {
-    const int64_t k = s.kt * DEPTH<float>;
-    return s.dtype == RVX_DTYPE_F32 ? 4 * k * s.out : 0;
+    return s.dtype == RVX_DTYPE_F32 ? (int64_t)s.nt * split_frags(s.in) * 2048 : 0;
 }
-void adapter_split(const AdapterShape& s, const float* w, void* planes, float* inv) {
-    const int k = s.kt * DEPTH<float>;
-    if (k != s.in) {
-        float* padded = scratch_f32("adapter_x", (int64_t)s.out * k);
-        pad_rows<float>(w, s.out, s.in, k, padded);
-        w = padded;
-    }
-    split_h2_rows(w, nullptr, s.out, k, (_Float16*)planes, nullptr, inv);
+void adapter_split(const AdapterShape& s, const float* w, void* halves, float* inv) {
+    RVX_LAUNCH("adapter_split", split_kernel<true>, dim3((unsigned)s.nt), dim3(1024), 0, w, s.in, (int64_t)s.out,
+               (const int32_t*)nullptr, split_frags(s.in), (_Float16*)halves, inv);
 }
 
 void adapter_forward(const AdapterArgs& g) {
@@ -756,21 +797,11 @@ void adapter_forward(const AdapterArgs& g) {
                 t.back = __is_same(T, _Float16) ? (float*)(t.lo + plane) : nullptr;
             }
         }
-        // f32 through the split-f16 product: see below
-        bool split_gemm = false;
-        int ldx = s.kt * DEPTH<T>;
-        GemmOperand op{};
+        constexpr bool F32 = __is_same(T, float);
         auto tiles = [&](int64_t bm, int64_t bn) { return (n + bm - 1) / bm * ((s.out + bn - 1) / bn); };
-        if constexpr (__is_same(T, float)) {
-            if (g.w_split && tiles(128, 128) >= cus) {
-                op = GemmOperand{x, ldx, nullptr, ldx, ldx};
-                op.Bh = (const _Float16*)g.w_split, op.Bh_plane = (int64_t)s.out * ldx, op.b_inv = g.w_inv;
-                split_gemm = gemm_h2_ok(n, s.out, op, nullptr);
-            }
-        }
         const int64_t row_tiles = (n + 15) / 16;
         // without adapters one row tile is read as it is: its 16-row loads cost less than another launch
-        T* packed = split_gemm || (n <= 16 && !g.ids) ? nullptr : (T*)scratch_bytes("adapter_x", row_tiles * s.kt * 1024);
+        T* packed = (F32 && !few) || (n <= 16 && !g.ids) ? nullptr : (T*)scratch_bytes("adapter_x", row_tiles * s.kt * 1024);
         // few row tiles: several blocks each, for the turns of different adapters and parts of the sum
         const unsigned spare = (unsigned)std::max<int64_t>(1, std::min<int64_t>(16, 2 * cus / row_tiles));
         const unsigned turns = g.ids ? few ? 16 : spare : 1, sums = few ? FEW_PARTS : g.ids ? 1 : std::min(spare, 4u);
@@ -809,44 +840,36 @@ void adapter_forward(const AdapterArgs& g) {
             else go(integral_constant<int, 4>{});
             return;
         }
-        auto go = [&](auto bm, auto bn, auto wm, auto wn, auto ns, auto kf, auto add) {
+        auto go = [&](auto zero_p, const void* xp, const float* x_inv, const void* wp, int frags, auto bm, auto bn, auto wm,
+                      auto wn, auto ns, auto kf) {
+            using P = decltype(zero_p);
             constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WM = decltype(wm)::value,
                           WN = decltype(wn)::value, NS = decltype(ns)::value;
             const int tm = (int)((n + BM - 1) / BM), tn = (s.out + BN - 1) / BN;
-            RVX_LAUNCH("adapter_tile", (tile_kernel<T, BM, BN, WM, WN, NS, decltype(kf)::value, decltype(add)::value>),
-                       dim3((unsigned)(tm * tn)),
-                       dim3(64 * WM * WN), 0, (const T*)packed, n, w, s.kt, s.nt, bias, b, s.b_slot, s.rk, g.ids, (const int32_t*)perm,
-                       g.slot, s.slots, t, s.out, tm, tn, y);
+            RVX_LAUNCH("adapter_tile", (tile_kernel<T, P, BM, BN, WM, WN, NS, decltype(kf)::value>), dim3((unsigned)(tm * tn)),
+                       dim3(64 * WM * WN), 0, (const P*)xp, x_inv, n, (const P*)wp, g.w_inv, frags, s.nt, bias, b, s.b_slot,
+                       s.rk, g.ids, (const int32_t*)perm, g.slot, s.slots, t, s.out, tm, tn, y);
         };
-        if constexpr (__is_same(T, float)) {
-            // The framework's split-f16 product has about twice the rate of f32 matrix instructions; it
-            // takes its operands row-major and knows no adapters, so their part is added to y.
-            if (split_gemm) {
-                if (ldx != s.in) {
-                    float* padded = scratch_f32("adapter_x", n * ldx);
-                    pad_rows<float>(x, n, s.in, ldx, padded);
-                    op.A = padded;
-                }
-                GemmEpilogue ep;
-                ep.bias0 = bias;
-                float* scale = scratch_f32("gemm_auto_scale", n);
-                row_scale_h2(op.A, ldx, ldx, nullptr, 0, 0, n, scale);
-                gemm_nt_h2(n, s.out, op, op.Bh, nullptr, nullptr, scale, op.b_inv, ep, y, s.out, "adapter_gemm");
-                if (g.ids)
-                    go(integral_constant<int, 64>{}, integral_constant<int, 64>{}, integral_constant<int, 2>{},
-                       integral_constant<int, 2>{}, integral_constant<int, 2>{}, integral_constant<int, 1>{}, std::true_type{});
-                return;
-            }
+        constexpr integral_constant<int, 2> I2{};
+        constexpr integral_constant<int, 4> I4{};
+        constexpr integral_constant<int, 64> I64{};
+        constexpr integral_constant<int, 128> I128{};
+        constexpr integral_constant<int, 256> I256{};
+        if constexpr (F32) {
+            const int ktq = split_frags(s.in);
+            const int64_t bytes = row_tiles * ktq * 2048;
+            auto* halves = (char*)scratch_bytes("adapter_x", bytes + n * 4);
+            auto* x_inv = (float*)(halves + bytes);
+            RVX_LAUNCH("adapter_split", split_kernel<false>, dim3((unsigned)row_tiles), dim3(1024), 0, x, s.in, n,
+                       (const int32_t*)perm, ktq, (_Float16*)halves, x_inv);
+            if (tiles(128, 128) >= cus) go(_Float16{}, halves, x_inv, g.w_split, 2 * ktq, I128, I128, I2, I2, I4, I2);
+            else go(_Float16{}, halves, x_inv, g.w_split, 2 * ktq, I64, I64, I2, I2, I4, I2);
+        } else {
+            if (tiles(256, 256) >= cus)
+                go(T{}, packed, nullptr, w, s.kt, I256, I256, I2, I4, I4, integral_constant<int, 1>{});
+            else if (tiles(128, 128) >= cus) go(T{}, packed, nullptr, w, s.kt, I128, I128, I2, I2, I4, I2);
+            else go(T{}, packed, nullptr, w, s.kt, I64, I64, I2, I2, I4, I2);
         }
-        if (tiles(256, 256) >= cus)
-            go(integral_constant<int, 256>{}, integral_constant<int, 256>{}, integral_constant<int, 2>{},
-               integral_constant<int, 4>{}, integral_constant<int, 4>{}, integral_constant<int, 1>{}, std::false_type{});
-        else if (tiles(128, 128) >= cus)
-            go(integral_constant<int, 128>{}, integral_constant<int, 128>{}, integral_constant<int, 2>{},
-               integral_constant<int, 2>{}, integral_constant<int, 4>{}, integral_constant<int, 2>{}, std::false_type{});
-        else
-            go(integral_constant<int, 64>{}, integral_constant<int, 64>{}, integral_constant<int, 2>{},
-               integral_constant<int, 2>{}, integral_constant<int, 4>{}, integral_constant<int, 2>{}, std::false_type{});
     });
 }
 
