@@ -9,6 +9,36 @@
 namespace rvx {
 namespace {
 
+// N values of S as one vector (kept packed: arrays of 16-bit values are spread over registers)
+template <class S, int N>
+struct Pack {
+    typedef S V __attribute__((ext_vector_type(N)));
+};
+template <class S, int N>
+using PackOf = typename Pack<S, N>::V;
+
+// Columns past dim hold anything. No lane branches, so that the loads of many rows go out together: a
+// lane past the last whole vector reads the last N columns and shifts its own into place.
+template <class S, int N>
+__device__ __forceinline__ PackOf<S, N> get_vec(const S* row, int c, int dim) {
+    PackOf<S, N> v;
+    if (dim < N) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = i < dim ? row[i] : (S)0.0f;  // (one vector: c is 0 or past dim)
+        return v;
+    }
+    const int from = min(c, dim - N), shift = c - from;
+    __builtin_memcpy(&v, row + from, sizeof(v));
+    if (dim % N) {
+#pragma unroll
+        for (int st = N / 2; st > 0; st >>= 1)
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (i + st < N) v[i] = shift & st ? v[i + st] : v[i];
+    }
+    return v;
+}
+
 // ---------------------------------------------------------------- forward
 constexpr int EF_U = 4;  // 16-byte chunks per lane
 
@@ -31,28 +61,25 @@ __global__ __launch_bounds__(256) void embed_forward_kernel(const T* __restrict_
         col[u] = (x - q * cpr) * N;
         id[u] = row[u] < n ? ids[row[u]] : -1;
     }
-    Vec16<T> v[EF_U];
+    PackOf<T, N> v[EF_U];
 #pragma unroll
     for (int u = 0; u < EF_U; ++u) {
         const bool there = id[u] >= 0 && id[u] < rows;
-        const T* p = table + id[u] * dim + col[u];
-        if (there && col[u] + N <= (uint32_t)dim) v[u] = load16(p);
-        else
-#pragma unroll
-            for (int j = 0; j < N; ++j) v[u].v[j] = there && col[u] + j < (uint32_t)dim ? p[j] : (T)0.0f;
+        v[u] = get_vec<T, N>(table + (there ? id[u] : 0) * dim, col[u], dim);
+        if (!there) v[u] = (T)0.0f;
     }
 #pragma unroll
     for (int u = 0; u < EF_U; ++u) {
         if (row[u] >= n) continue;
-        Vec16<T> r;
+        PackOf<T, N> r;
 #pragma unroll
-        for (int j = 0; j < N; ++j) r.v[j] = (T)((float)v[u].v[j] * scale);
+        for (int j = 0; j < N; ++j) r[j] = (T)((float)v[u][j] * scale);
         T* o = out + row[u] * dim + col[u];
-        if (col[u] + N <= (uint32_t)dim) store16(o, r);
+        if (col[u] + N <= (uint32_t)dim) __builtin_memcpy(o, &r, 16);
         else
 #pragma unroll
             for (int j = 0; j < N; ++j)
-                if (col[u] + j < (uint32_t)dim) o[j] = r.v[j];
+                if (col[u] + j < (uint32_t)dim) o[j] = r[j];
     }
 }
 
@@ -67,6 +94,19 @@ constexpr int SORT_MAX_BITS = 11, SORT_BINS = 1 << SORT_MAX_BITS;
 __device__ __forceinline__ uint32_t sort_key(const int64_t* ids, int64_t i, uint32_t rows) {
     const int64_t id = ids[i];
     return id >= 0 && id < (int64_t)rows ? (uint32_t)id : rows;
+}
+
+// the block-th of `blocks` blocks' share of setting bytes (an even number of them) to 0
+__device__ __forceinline__ void zero_bytes(unsigned char* p, int64_t bytes, int block, int blocks) {
+    const int64_t step = (int64_t)blocks * blockDim.x * 16;
+    const uint4 z = {0, 0, 0, 0};
+    int64_t b = ((int64_t)block * blockDim.x + threadIdx.x) * 16;
+    for (; b + 3 * step + 16 <= bytes; b += 4 * step)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) __builtin_memcpy(p + b + u * step, &z, 16);
+    for (; b + 16 <= bytes; b += step) __builtin_memcpy(p + b, &z, 16);
+    if (b < bytes)
+        for (; b < bytes; b += 2) *(uint16_t*)(p + b) = 0;
 }
 
 // counts[tile][digit]; clear: nullable, words to set to 0
@@ -192,6 +232,90 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_move_kernel(const int64_t* 
     }
 }
 
+// Up to SMALL_SORT positions: one block sorts them in LDS, in one launch; the other blocks meanwhile
+// set `clear` (nullable) to zeros.
+constexpr int SMALL_SORT = 8192, SMALL_BITS = 9, SMALL_THREADS = 1024, SMALL_WAVES = SMALL_THREADS / 64;
+
+__global__ __launch_bounds__(SMALL_THREADS) void sort_small_kernel(const int64_t* __restrict__ ids, int n, uint32_t rows,
+                                                                  int passes, int bits, uint32_t* __restrict__ key_out,
+                                                                  uint32_t* __restrict__ pos_out, unsigned char* clear,
+                                                                  int64_t clear_bytes) {
+    __shared__ uint32_t key[2][SMALL_SORT];
+    __shared__ uint16_t pos[2][SMALL_SORT];
+    __shared__ uint32_t mine[SMALL_WAVES][1 << SMALL_BITS];
+    __shared__ uint32_t sums[(1 << SMALL_BITS) / 64];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    if (blockIdx.x > 0) {
+        zero_bytes(clear, clear_bytes, blockIdx.x - 1, gridDim.x - 1);
+        return;
+    }
+    for (int i = t; i < n; i += SMALL_THREADS) {
+        key[0][i] = sort_key(ids, i, rows);
+        pos[0][i] = (uint16_t)i;
+    }
+    const int bins = 1 << bits, chunk = (n + SMALL_THREADS - 1) / SMALL_THREADS * 64;  // a wave's elements, in order
+    const int lo = wave * chunk, hi = min(n, lo + chunk);
+    for (int p = 0; p < passes; ++p) {
+        const int in = p & 1, shift = p * bits;
+        for (int i = t; i < SMALL_WAVES << bits; i += SMALL_THREADS) mine[i >> bits][i & (bins - 1)] = 0;
+        __syncthreads();
+        for (int i = lo + lane; i < hi; i += 64) atomicAdd(&mine[wave][(key[in][i] >> shift) & (bins - 1)], 1u);
+        __syncthreads();
+        // a digit's places: those of smaller digits, then of this one wave by wave
+        uint32_t count[SMALL_WAVES], total = 0;
+        if (t < bins)
+#pragma unroll
+            for (int w = 0; w < SMALL_WAVES; ++w) count[w] = mine[w][t];
+        if (t < bins)
+#pragma unroll
+            for (int w = 0; w < SMALL_WAVES; ++w) total += count[w];
+        uint32_t scan = total;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t v = __shfl_up(scan, o);
+            scan += lane >= o ? v : 0;
+        }
+        if (lane == 63 && wave < (1 << SMALL_BITS) / 64) sums[wave] = scan;
+        __syncthreads();
+        if (t < bins) {
+            uint32_t from = scan - total;
+            for (int w = 0; w < wave; ++w) from += sums[w];
+#pragma unroll
+            for (int w = 0; w < SMALL_WAVES; ++w) {
+                mine[w][t] = from;
+                from += count[w];
+            }
+        }
+        __syncthreads();
+        for (int i0 = lo; i0 < hi; i0 += 64) {
+            const int i = i0 + lane;
+            const bool there = i < hi;
+            const uint32_t k = there ? key[in][i] : 0, d = (k >> shift) & (bins - 1);
+            unsigned long long same = __ballot(there);
+            for (int b = 0; b < bits; ++b) {
+                const unsigned long long m = __ballot((d >> b) & 1);
+                same &= (d >> b) & 1 ? m : ~m;
+            }
+            const int before = __popcll(same & ((1ull << lane) - 1));
+            uint32_t to = 0;
+            if (there) to = mine[wave][d] + before;
+            __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");
+            if (there && before == 0) mine[wave][d] = to + __popcll(same);
+            __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");
+            if (there) {
+                if (p + 1 < passes) {
+                    key[1 - in][to] = k;
+                    pos[1 - in][to] = pos[in][i];
+                } else {
+                    key_out[to] = k;
+                    pos_out[to] = pos[in][i];
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
 // ---------------------------------------------------------------- sums over groups
 // An id's entries are a run of the sorted order. A run of fewer than LONG entries is summed by one
 // wave per slab of columns, in order. A longer one is cut where the order is, into groups of GROUP
@@ -201,25 +325,11 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_move_kernel(const int64_t* 
 // of its group.) Groups and order depend on the sorted ids alone.
 constexpr int GROUP = 64, LONG = 63;
 
-// N values of S as one vector (kept packed: arrays of 16-bit values are spread over registers)
-template <class S, int N>
-struct Pack {
-    typedef S V __attribute__((ext_vector_type(N)));
-};
-template <class S, int N>
-using PackOf = typename Pack<S, N>::V;
-
 // A wave's columns of a row: V vectors of N columns a lane, vector q at (q * 64 + lane) * N.
 template <class S, int N, int V>
 __device__ __forceinline__ void get_cols(const S* row, PackOf<S, N> (&v)[V], int col, int dim) {
 #pragma unroll
-    for (int q = 0; q < V; ++q) {
-        const int c = col + q * 64 * N;
-        if (c + N <= dim) __builtin_memcpy(&v[q], row + c, sizeof(S) * N);
-        else
-#pragma unroll
-            for (int i = 0; i < N; ++i) v[q][i] = c + i < dim ? row[c + i] : (S)0.0f;
-    }
+    for (int q = 0; q < V; ++q) v[q] = get_vec<S, N>(row, col + q * 64 * N, dim);
 }
 template <class S, int N, int V>
 __device__ __forceinline__ void put_cols(S* row, const PackOf<S, N> (&v)[V], int col, int dim) {
@@ -306,7 +416,7 @@ __global__ __launch_bounds__(64) void embed_groups_kernel(const T* __restrict__ 
     const int col = blockIdx.y * 64 * N + lane * N;
     auto sum = [&](int from, int count, float* out) {
         PackOf<float, N> acc[1] = {};
-        add_rows<16, T, N, 1>(acc, count, col, dim, [&](int j) {
+        add_rows<32, T, N, 1>(acc, count, col, dim, [&](int j) {
             return grad_out + (int64_t)(uint32_t)__builtin_amdgcn_readlane(at.pos, from + j) * dim;
         });
         put_cols<float, N, 1>(out + g * dim, acc, col, dim);
@@ -386,7 +496,8 @@ __global__ __launch_bounds__(64) void embed_long_kernel(int dim, const uint32_t*
 
 // One wave per (sorted entry, slab): the first entry of an id sums the id's run into its row. Bound
 // by HBM: a wave takes up to 4 vectors a lane, so that a row's bytes are all in flight at once.
-template <class T, class S, int V>
+// UP: 4 times as many rows of a run in flight; costs occupancy.
+template <class T, class S, int V, bool UP>
 __global__ __launch_bounds__(256) void embed_rows_kernel(const T* __restrict__ grad_out, int dim, int64_t begin,
                                                         const uint32_t* __restrict__ key,
                                                         const uint32_t* __restrict__ pos, int64_t n, uint32_t rows,
@@ -409,7 +520,7 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const T* __restrict__ g
     PackOf<S, N> old[V] = {};
     if (add) get_cols<S, N, V>(row, old, col, dim);  // does not wait for the sum
     PackOf<float, N> acc[V] = {};
-    add_rows<V == 1 ? 8 : V == 2 ? 4 : 2, T, N, V>(acc, run, col, dim, [&](int j) {
+    add_rows<(V == 1 ? 8 : V == 2 ? 4 : 2) * (UP ? 4 : 1), T, N, V>(acc, run, col, dim, [&](int j) {
         return grad_out + (int64_t)(uint32_t)__builtin_amdgcn_readlane(near_pos, j + 1) * dim;
     });
     finish_row<S, N, V>(row, acc, old, col, dim, scale);
@@ -473,15 +584,7 @@ __global__ __launch_bounds__(256) void embed_zero_rows_kernel(unsigned char* tab
 }
 // The whole table: zeros.
 __global__ __launch_bounds__(256) void embed_zero_kernel(unsigned char* table, int64_t bytes) {
-    const int64_t step = (int64_t)gridDim.x * 256 * 16;
-    const uint4 z = {0, 0, 0, 0};
-    int64_t b = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 16;
-    for (; b + 3 * step + 16 <= bytes; b += 4 * step)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) __builtin_memcpy(table + b + u * step, &z, 16);
-    for (; b + 16 <= bytes; b += step) __builtin_memcpy(table + b, &z, 16);
-    if (b < bytes)
-        for (; b < bytes; b += 2) *(uint16_t*)(table + b) = 0;
+    zero_bytes(table, bytes, blockIdx.x, gridDim.x);
 }
 
 }  // namespace
@@ -509,8 +612,8 @@ void embedding_forward(int32_t dtype, const void* table, int64_t rows, int dim, 
 void embedding_backward(int32_t dtype, const void* grad_out, const int64_t* ids, int64_t n, int64_t rows, int dim,
                         float scale, bool accumulate, int32_t table_dtype, void* grad_table) {
     const int64_t table_bytes = rows * dim * dtype_size(table_dtype);
-    auto zero_table = [&](int per_cu) {
-        const int64_t blocks = std::min<int64_t>((table_bytes + 4095) / 4096, (int64_t)per_cu * device().num_cus);
+    auto zero_table = [&] {
+        const int64_t blocks = std::min<int64_t>((table_bytes + 4095) / 4096, 8LL * device().num_cus);
         RVX_LAUNCH("embedding_zero", embed_zero_kernel, dim3((unsigned)blocks), dim3(256), 0, (unsigned char*)grad_table,
                    table_bytes);
     };
@@ -518,7 +621,7 @@ void embedding_backward(int32_t dtype, const void* grad_out, const int64_t* ids,
         with_dtype(dtype, [&](auto t) { with_dtype(table_dtype, [&](auto s) { f(t, s); }); });
     };
     if (n <= SCAN_MAX) {
-        if (!accumulate) zero_table(8);
+        if (!accumulate) zero_table();
         if (n == 0) return;
         typed([&](auto t, auto s) {
             using T = decltype(t);
@@ -533,59 +636,66 @@ void embedding_backward(int32_t dtype, const void* grad_out, const int64_t* ids,
     // digits of equal width, as few as SORT_MAX_BITS allows; the key `rows` stands for absent ids
     int key_bits = 1;
     while (((int64_t)1 << key_bits) <= rows) ++key_bits;
-    const int passes = (key_bits + SORT_MAX_BITS - 1) / SORT_MAX_BITS;
-    const int bits = std::max(2, (key_bits + passes - 1) / passes);  // at least the 4 digits of a thread
-    int64_t tile = (n + SORT_TILES - 1) / SORT_TILES;
-    tile = (tile + SORT_STEP - 1) / SORT_STEP * SORT_STEP;
-    const int tiles = (int)((n + tile - 1) / tile);
-    auto* counts = (uint32_t*)scratch_bytes("embed_counts", ((int64_t)SORT_TILES << bits) * 4);
     auto* sorted = (uint32_t*)scratch_bytes("embed_sorted", n * 16);  // key, pos and their other halves
     uint32_t *key[2] = {sorted, sorted + 2 * n}, *pos[2] = {sorted + n, sorted + 3 * n};
+    const uint32_t *sk, *sp;
     const int64_t groups = (n + GROUP - 1) / GROUP, span_count = n / (GROUP * GROUP);
     float* heads = scratch_f32("embed_partial", (2 * groups + span_count) * dim);
     float *tails = heads + groups * dim, *spans = tails + groups * dim;
+    // A small table's dense gradient is set to zeros before the sums; of a large one only the rows
+    // without an id, beside the sums.
+    const bool beside = !accumulate && table_bytes >= ZERO_BESIDE_BYTES;
     const int64_t words = (rows + 3) / 4;
-    auto* present = accumulate ? nullptr : (uint32_t*)scratch_bytes("embed_present", words * 4);  // a byte a row
-    for (int p = 0; p < passes; ++p) {
-        const int in = (p + 1) & 1, out = p & 1, shift = p * bits;
-        if (p == 0) {
-            RVX_LAUNCH("embedding_count", sort_count_kernel<true>, dim3(tiles), dim3(SORT_THREADS), 0, ids,
-                       (const uint32_t*)nullptr, n, (uint32_t)rows, tile, bits, shift, counts, present, words);
-            RVX_LAUNCH("embedding_sort", sort_move_kernel<true>, dim3(tiles), dim3(SORT_THREADS), 0, ids,
-                       (const uint32_t*)nullptr, (const uint32_t*)nullptr, n, (uint32_t)rows, tile, tiles, bits, shift,
-                       (const uint32_t*)counts, key[out], pos[out]);
-        } else {
-            RVX_LAUNCH("embedding_count", sort_count_kernel<false>, dim3(tiles), dim3(SORT_THREADS), 0,
-                       (const int64_t*)nullptr, (const uint32_t*)key[in], n, (uint32_t)rows, tile, bits, shift, counts, nullptr, (int64_t)0);
-            RVX_LAUNCH("embedding_sort", sort_move_kernel<false>, dim3(tiles), dim3(SORT_THREADS), 0,
-                       (const int64_t*)nullptr, (const uint32_t*)key[in], (const uint32_t*)pos[in], n, (uint32_t)rows, tile,
-                       tiles, bits, shift, (const uint32_t*)counts, key[out], pos[out]);
+    auto* present = beside ? (uint32_t*)scratch_bytes("embed_present", words * 4) : nullptr;  // a byte a row
+    if (n <= SMALL_SORT) {
+        const int passes = (key_bits + SMALL_BITS - 1) / SMALL_BITS, bits = (key_bits + passes - 1) / passes;
+        unsigned char* clear = beside ? (unsigned char*)present : accumulate ? nullptr : (unsigned char*)grad_table;
+        const int64_t bytes = beside ? words * 4 : accumulate ? 0 : table_bytes;
+        const int64_t blocks = std::min<int64_t>((bytes + 16383) / 16384, 2LL * device().num_cus);
+        RVX_LAUNCH("embedding_sort", sort_small_kernel, dim3((unsigned)(1 + blocks)), dim3(SMALL_THREADS), 0, ids, (int)n,
+                   (uint32_t)rows, passes, bits, key[0], pos[0], clear, bytes);
+        sk = key[0], sp = pos[0];
+    } else {
+        const int passes = (key_bits + SORT_MAX_BITS - 1) / SORT_MAX_BITS;
+        const int bits = std::max(2, (key_bits + passes - 1) / passes);  // at least the 4 digits of a thread
+        int64_t tile = (n + SORT_TILES - 1) / SORT_TILES;
+        tile = (tile + SORT_STEP - 1) / SORT_STEP * SORT_STEP;
+        const int tiles = (int)((n + tile - 1) / tile);
+        auto* counts = (uint32_t*)scratch_bytes("embed_counts", ((int64_t)SORT_TILES << bits) * 4);
+        for (int p = 0; p < passes; ++p) {
+            const int in = (p + 1) & 1, out = p & 1, shift = p * bits;
+            if (p == 0) {
+                RVX_LAUNCH("embedding_count", sort_count_kernel<true>, dim3(tiles), dim3(SORT_THREADS), 0, ids,
+                           (const uint32_t*)nullptr, n, (uint32_t)rows, tile, bits, shift, counts, present, words);
+                RVX_LAUNCH("embedding_sort", sort_move_kernel<true>, dim3(tiles), dim3(SORT_THREADS), 0, ids,
+                           (const uint32_t*)nullptr, (const uint32_t*)nullptr, n, (uint32_t)rows, tile, tiles, bits, shift,
+                           (const uint32_t*)counts, key[out], pos[out]);
+            } else {
+                RVX_LAUNCH("embedding_count", sort_count_kernel<false>, dim3(tiles), dim3(SORT_THREADS), 0,
+                           (const int64_t*)nullptr, (const uint32_t*)key[in], n, (uint32_t)rows, tile, bits, shift, counts,
+                           nullptr, (int64_t)0);
+                RVX_LAUNCH("embedding_sort", sort_move_kernel<false>, dim3(tiles), dim3(SORT_THREADS), 0,
+                           (const int64_t*)nullptr, (const uint32_t*)key[in], (const uint32_t*)pos[in], n, (uint32_t)rows,
+                           tile, tiles, bits, shift, (const uint32_t*)counts, key[out], pos[out]);
+            }
         }
+        sk = key[(passes + 1) & 1], sp = pos[(passes + 1) & 1];
+        if (!accumulate && !beside) zero_table();
     }
-    const uint32_t *sk = key[(passes + 1) & 1], *sp = pos[(passes + 1) & 1];
-    // The dense gradient's zeros are written on a second stream beside the sums: the two write
-    // different rows. Small tables are not worth the events.
     hipEvent_t zeroed = nullptr;
-    if (!accumulate) {
-        auto zero_rows = [&](int per_cu) {
-            const int64_t blocks = std::min<int64_t>((rows + 255) / 256, (int64_t)per_cu * device().num_cus);
-            RVX_LAUNCH("embedding_zero", embed_zero_rows_kernel, dim3((unsigned)blocks), dim3(256), 0,
-                       (unsigned char*)grad_table, rows, table_bytes / rows, (const unsigned char*)present);
-        };
+    if (beside) {  // on a second stream: the two write different rows
         RVX_LAUNCH("embedding_mark", embed_mark_kernel,
                    dim3((unsigned)std::min<int64_t>((n + 255) / 256, 4LL * device().num_cus)), dim3(256), 0, sk, n,
                    (uint32_t)rows, (unsigned char*)present);
-        if (table_bytes >= ZERO_BESIDE_BYTES) {
-            hipEvent_t* ev = pipeline_events(2);
-            RVX_HIP(hipEventRecord(ev[0], stream()));
-            RVX_HIP(hipStreamWaitEvent(device().aux, ev[0], 0));
-            StreamScope on(device().aux);
-            zero_rows(ZERO_BESIDE_BLOCKS);
-            zeroed = ev[1];
-            RVX_HIP(hipEventRecord(zeroed, device().aux));
-        } else {
-            zero_rows(8);
-        }
+        hipEvent_t* ev = pipeline_events(2);
+        RVX_HIP(hipEventRecord(ev[0], stream()));
+        RVX_HIP(hipStreamWaitEvent(device().aux, ev[0], 0));
+        StreamScope on(device().aux);
+        const int64_t blocks = std::min<int64_t>((rows + 255) / 256, (int64_t)ZERO_BESIDE_BLOCKS * device().num_cus);
+        RVX_LAUNCH("embedding_zero", embed_zero_rows_kernel, dim3((unsigned)blocks), dim3(256), 0, (unsigned char*)grad_table,
+                   rows, table_bytes / rows, (const unsigned char*)present);
+        zeroed = ev[1];
+        RVX_HIP(hipEventRecord(zeroed, device().aux));
     }
     typed([&](auto t, auto s) {
         using T = decltype(t);
@@ -601,17 +711,22 @@ void embedding_backward(int32_t dtype, const void* grad_out, const int64_t* ids,
                    (uint32_t)rows, (const float*)heads, (const float*)tails, (const float*)spans, scale, accumulate,
                    (S*)grad_table);
         const int slabs = (vecs + 3) / 4, per = (vecs + slabs - 1) / slabs;
-        auto go = [&](auto v) {
+        auto go = [&](auto v, auto up) {
             constexpr int64_t SLICE = (int64_t)1 << 24;  // entries of one launch: at most 2^30 threads
             for (int64_t i = 0; i < n; i += SLICE)
-                RVX_LAUNCH("embedding_backward", (embed_rows_kernel<T, S, decltype(v)::value>),
+                RVX_LAUNCH("embedding_backward", (embed_rows_kernel<T, S, decltype(v)::value, decltype(up)::value>),
                            dim3((unsigned)((std::min(SLICE, n - i) + 3) / 4), slabs), dim3(256), 0, (const T*)grad_out, dim, i,
                            sk, sp, n, (uint32_t)rows, scale, accumulate, (S*)grad_table);
         };
-        if (per == 1) go(std::integral_constant<int, 1>{});
-        else if (per == 2) go(std::integral_constant<int, 2>{});
-        else if (per == 3) go(std::integral_constant<int, 3>{});
-        else go(std::integral_constant<int, 4>{});
+        auto by_width = [&](auto up) {
+        if (per == 1) go(std::integral_constant<int, 1>{}, up);
+        else if (per == 2) go(std::integral_constant<int, 2>{}, up);
+        else if (per == 3) go(std::integral_constant<int, 3>{}, up);
+        else go(std::integral_constant<int, 4>{}, up);
+        };
+        // few waves: the latency of long runs counts, else the waves that hide it do
+        if (n * slabs <= 32LL * device().num_cus) by_width(std::true_type{});
+        else by_width(std::false_type{});
     });
     if (zeroed) RVX_HIP(hipStreamWaitEvent(stream(), zeroed, 0));
 }

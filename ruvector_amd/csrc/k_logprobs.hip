@@ -485,13 +485,19 @@ __global__ __launch_bounds__(256) void logprobs_backward_kernel(
     const T* x = scores + row * ld;
     T* g = grad + row * ld_grad;
     Vec16<T> v[U];
+    const bool whole = at + 64 * N * U <= c;
+    if (whole) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int64_t p = at + (u * 64 + lane) * N;
-        if (p + N <= c) v[u] = load16(x + p);
-        else
+        for (int u = 0; u < U; ++u) v[u] = load16(x + at + (u * 64 + lane) * N);
+    } else {
 #pragma unroll
-            for (int j = 0; j < N; ++j) v[u].v[j] = p + j < c ? x[p + j] : (T)0.0f;
+        for (int u = 0; u < U; ++u) {
+            const int64_t p = at + (u * 64 + lane) * N;
+            if (p + N <= c) v[u] = load16(x + p);
+            else
+#pragma unroll
+                for (int j = 0; j < N; ++j) v[u].v[j] = p + j < c ? x[p + j] : (T)0.0f;
+        }
     }
     int64_t target = targets ? targets[row] : -1;
     if (target >= c) target = -1;
@@ -519,7 +525,7 @@ __global__ __launch_bounds__(256) void logprobs_backward_kernel(
         Vec16<T> o;
 #pragma unroll
         for (int j = 0; j < N; ++j) o.v[j] = (T)d[j];
-        if (p + N <= c) store16(g + p, o);
+        if (whole || p + N <= c) store16(g + p, o);
         else
 #pragma unroll
             for (int j = 0; j < N; ++j)
