@@ -19,10 +19,11 @@ void with_dtype(int32_t dtype, F&& f) {  // f(T{}) for the element type T of `dt
 
 // 16 bytes of T at any element address: rows of an odd width start at odd elements, and gfx950
 // takes vector loads and stores at any address.
+// (A vector type: arrays of 16-bit values would be spread over a register each.)
 template <class T>
 struct Vec16 {
     static constexpr int N = 16 / (int)sizeof(T);
-    T v[N];
+    T v __attribute__((ext_vector_type(N)));
 };
 template <class T>
 __device__ __forceinline__ Vec16<T> load16(const T* p) {

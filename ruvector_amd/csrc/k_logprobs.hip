@@ -161,6 +161,16 @@ struct Best {
                                                      __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0))] = key;
         waiting += __popcll(mask);
     }
+    // One score a lane; most hold no lane's candidate, which one comparison shows.
+    __device__ __forceinline__ void offer_score(float x, uint32_t id) {
+        const bool may = x >= tau_score && x > -INFINITY;
+        if (__any(may)) offer(key_of(x, id), may);
+    }
+    // Waiting keys are merged once they are worth it: a late tau lets more scores through.
+    __device__ __forceinline__ void settle() {
+        const int worth = k <= 32 ? 32 : 64;
+        while (waiting >= worth) flush();
+    }
 };
 
 struct Part {  // what one block found of one row
@@ -194,24 +204,38 @@ __device__ __forceinline__ void write_top(u64 list, int k, int64_t row, const St
 // ---------------------------------------------------------------- one pass
 constexpr int LP_U = 2, LP_WAVES = 4;  // 16-byte loads per lane and step; waves per block
 
+// A wave's elements of one step, 16 bytes a lane and load. In a row's last step a lane whose piece
+// would pass the end takes the row's last piece, and drops what is not its own: no lane branches.
 template <class T>
-struct Step {  // a wave's elements of one step, lane by lane 16 bytes
+struct Step {
     static constexpr int N = Vec16<T>::N, SIZE = 64 * N * LP_U;
     Vec16<T> v[LP_U];
-    __device__ __forceinline__ void load(const T* x, int64_t at, int64_t hi) {  // past hi: masked
-        const int lane = threadIdx.x & 63;
-        if (at + SIZE <= hi) {
+    static __device__ __forceinline__ int place(int u, int64_t left) {  // the piece's begin, from the step's on
+        const int p = (u * 64 + (threadIdx.x & 63)) * N;
+        return left >= SIZE ? p : (int)min((int64_t)p, left - N);
+    }
+    __device__ __forceinline__ void load(const T* x, int64_t at, int64_t hi) {
+        if (hi < N) {  // a row shorter than a piece: every lane holds it
 #pragma unroll
-            for (int u = 0; u < LP_U; ++u) v[u] = load16(x + at + (u * 64 + lane) * N);
-        } else {
+            for (int u = 0; u < LP_U; ++u)
 #pragma unroll
-            for (int u = 0; u < LP_U; ++u) {
-                const int64_t p = at + (u * 64 + lane) * N;
-                if (p + N <= hi) v[u] = load16(x + p);
-                else
+                for (int j = 0; j < N; ++j) v[u].v[j] = j >= N - hi ? x[j - (N - hi)] : (T)-INFINITY;
+            return;
+        }
 #pragma unroll
-                    for (int j = 0; j < N; ++j) v[u].v[j] = p + j < hi ? x[p + j] : (T)-INFINITY;
-            }
+        for (int u = 0; u < LP_U; ++u) v[u] = load16(x + at + place(u, hi - at));
+    }
+    __device__ __forceinline__ void values(float (&f)[LP_U][N], int64_t left) const {
+#pragma unroll
+        for (int u = 0; u < LP_U; ++u)
+#pragma unroll
+            for (int j = 0; j < N; ++j) f[u][j] = (float)v[u].v[j];
+        if (left >= SIZE) return;
+#pragma unroll
+        for (int u = 0; u < LP_U; ++u) {
+            const int drop = (u * 64 + (int)(threadIdx.x & 63)) * N - place(u, left);
+#pragma unroll
+            for (int j = 0; j < N; ++j) f[u][j] = j < drop ? -INFINITY : f[u][j];
         }
     }
 };
@@ -225,11 +249,13 @@ __device__ __attribute__((noinline)) Stat far_stats(const T* x, int64_t lo, int6
     for (int64_t at = lo; at < hi; at += Step<T>::SIZE) {
         Step<T> cur;
         cur.load(x, at, hi);
+        float f[LP_U][N];
+        cur.values(f, hi - at);
 #pragma unroll
         for (int u = 0; u < LP_U; ++u)
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                const float v = (float)cur.v[u].v[j], mn = fmaxf(st.m, v);
+                const float v = f[u][j], mn = fmaxf(st.m, v);
                 const float d = fmaxf((st.m - mn) * c1, FLOOR_U), r = __builtin_amdgcn_exp2f(d);
                 const float y = (v - mn) * c1, ex = __builtin_amdgcn_exp2f(y);
                 st.e = fmaf(r, fmaf(st.s, d, st.e), ex * fmaxf(y, FLOOR_U));
@@ -254,10 +280,7 @@ __device__ __forceinline__ Stat walk(const T* __restrict__ x, int64_t lo, int64_
     if (lo < hi) nxt.load(x, lo, hi);
     for (int64_t at = lo; at < hi; at += SIZE) {
         float v[LP_U][N];
-#pragma unroll
-        for (int u = 0; u < LP_U; ++u)
-#pragma unroll
-            for (int j = 0; j < N; ++j) v[u][j] = (float)nxt.v[u].v[j];
+        nxt.values(v, hi - at);
         if (at + SIZE < hi) nxt.load(x, at + SIZE, hi);  // on its way while this step is worked on
         float cm = -INFINITY;
 #pragma unroll
@@ -311,9 +334,11 @@ __device__ __forceinline__ Stat walk(const T* __restrict__ x, int64_t lo, int64_
 #pragma unroll
                 for (int u = 0; u < LP_U; ++u)
 #pragma unroll
-                    for (int j = 0; j < N; ++j)
-                        before += __popcll(__ballot(v[u][j] > st_score ||
-                                                    (v[u][j] == st_score && (u * 64 + lane) * N + j < t)));
+                    for (int j = 0; j < N; ++j) {
+                        const int place = Step<T>::place(u, hi - at) + j;  // dropped ones are not counted
+                        before += __popcll(__ballot(v[u][j] > st_score || (v[u][j] == st_score && place < t &&
+                                                                           place >= (u * 64 + lane) * N)));
+                    }
             }
         }
         if constexpr (TOP) {
@@ -323,9 +348,8 @@ __device__ __forceinline__ Stat walk(const T* __restrict__ x, int64_t lo, int64_
 #pragma unroll
                 for (int u = 0; u < LP_U; ++u) {
 #pragma unroll
-                    for (int j = 0; j < N; ++j)
-                        best.offer(key_of(v[u][j], (uint32_t)(at + (u * 64 + lane) * N + j)), v[u][j] > -INFINITY);
-                    while (best.waiting >= 64) best.flush();
+                    for (int j = 0; j < N; ++j) best.offer_score(v[u][j], (uint32_t)(at + Step<T>::place(u, hi - at) + j));
+                    best.settle();
                 }
             }
         }
