@@ -36,6 +36,14 @@ __device__ __forceinline__ void store16(T* p, const Vec16<T>& r) {
     __builtin_memcpy(p, &r, 16);
 }
 
+// Between a wave's write and its lanes' reads of LDS: a wave's LDS instructions run in their order, so
+// only the compiler has to keep it. (A fence would also wait for every load on its way.)
+__device__ __forceinline__ void wave_lds_order() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("" ::: "memory");
+}
+
 // ---- argument checks -----------------------------------------------------
 inline void check_dtype(int32_t dtype) {
     RVX_REQUIRE(dtype >= RVX_DTYPE_F32 && dtype <= RVX_DTYPE_BF16, RVX_ERR_INVALID_PARAMETER,

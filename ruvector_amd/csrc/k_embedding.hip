@@ -221,9 +221,9 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_move_kernel(const int64_t* 
             const int before = __popcll(same & ((1ull << lane) - 1));
             uint32_t to = 0;
             if (there) to = mine[wave][d] + before;
-            __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");
+            wave_lds_order();
             if (there && before == 0) mine[wave][d] = to + __popcll(same);
-            __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");
+            wave_lds_order();
             if (there) {
                 key_out[to] = key[u];
                 pos_out[to] = pos[u];
@@ -299,9 +299,9 @@ __global__ __launch_bounds__(SMALL_THREADS) void sort_small_kernel(const int64_t
             const int before = __popcll(same & ((1ull << lane) - 1));
             uint32_t to = 0;
             if (there) to = mine[wave][d] + before;
-            __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");
+            wave_lds_order();
             if (there && before == 0) mine[wave][d] = to + __popcll(same);
-            __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");
+            wave_lds_order();
             if (there) {
                 if (p + 1 < passes) {
                     key[1 - in][to] = k;

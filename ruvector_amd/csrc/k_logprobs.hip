@@ -30,6 +30,13 @@ __device__ __forceinline__ Stat join(const Stat& a, const Stat& b, float c1) {
 }
 
 // ---------------------------------------------------------------- values of other lanes
+// The lane number, hidden from the compiler: masks made from it stay where they are used. (Hoisted
+// out of the loops around, a sort's masks overflow the scalar registers.)
+__device__ __forceinline__ int local_lane() {
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    return lane;
+}
 // x of lane (l ^ ST), without a trip through LDS: rows of 16 lanes are permuted by DPP, rows and
 // halves exchanged by the permlane swaps.
 template <int CTRL>
@@ -38,17 +45,16 @@ __device__ __forceinline__ uint32_t dpp(uint32_t x) {
 }
 template <int ST>
 __device__ __forceinline__ uint32_t lane_xor(uint32_t x) {
-    const int lane = threadIdx.x & 63;
     if constexpr (ST == 1) return dpp<0xB1>(x);             // quad_perm [1,0,3,2]
     else if constexpr (ST == 2) return dpp<0x4E>(x);        // quad_perm [2,3,0,1]
     else if constexpr (ST == 4) return dpp<0x1B>(dpp<0x141>(x));  // mirror of 8 lanes, then of 4: l ^ 7 ^ 3
     else if constexpr (ST == 8) return dpp<0x128>(x);       // rotation of a row by 8
     else if constexpr (ST == 16) {
         const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-        return lane & 16 ? r[0] : r[1];
+        return local_lane() & 16 ? r[0] : r[1];
     } else {
         const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-        return lane & 32 ? r[0] : r[1];
+        return local_lane() & 32 ? r[0] : r[1];
     }
 }
 template <int ST>
@@ -61,30 +67,30 @@ __device__ __forceinline__ u64 lane_xor(u64 x) {
 }
 // One exchange of a bitonic network: the smaller value goes to the lower lane where `up`.
 template <int ST, class K>
-__device__ __forceinline__ K exchange(K x, bool up) {
+__device__ __forceinline__ K exchange(K x, bool up, int lane) {
     const K y = lane_xor<ST>(x);
-    const bool low = ((threadIdx.x & 63) & ST) == 0;
-    return (low == up) == (x < y) ? x : y;
+    return ((lane & ST) == 0) == up == (x < y) ? x : y;
 }
 template <int SIZE, int ST, class K>
-__device__ __forceinline__ K sort_stage(K x) {  // the stage of SIZE: strides ST, ST / 2 .. 1
-    x = exchange<ST>(x, ((threadIdx.x & 63) & SIZE) == 0);
-    if constexpr (ST > 1) x = sort_stage<SIZE, ST / 2>(x);
+__device__ __forceinline__ K sort_stage(K x, int lane) {  // the stage of SIZE: strides ST, ST / 2 .. 1
+    x = exchange<ST>(x, (lane & SIZE) == 0, lane);
+    if constexpr (ST > 1) x = sort_stage<SIZE, ST / 2>(x, lane);
     return x;
 }
 template <class K>
 __device__ __forceinline__ K sort_up(K x) {  // ascending over the 64 lanes
-    x = sort_stage<2, 1>(x);
-    x = sort_stage<4, 2>(x);
-    x = sort_stage<8, 4>(x);
-    x = sort_stage<16, 8>(x);
-    x = sort_stage<32, 16>(x);
-    return sort_stage<64, 32>(x);
+    const int lane = local_lane();
+    x = sort_stage<2, 1>(x, lane);
+    x = sort_stage<4, 2>(x, lane);
+    x = sort_stage<8, 4>(x, lane);
+    x = sort_stage<16, 8>(x, lane);
+    x = sort_stage<32, 16>(x, lane);
+    return sort_stage<64, 32>(x, lane);
 }
 template <int ST = 32>
-__device__ __forceinline__ u64 bitonic_down(u64 x) {  // a bitonic row to descending order
-    x = exchange<ST>(x, false);
-    if constexpr (ST > 1) x = bitonic_down<ST / 2>(x);
+__device__ __forceinline__ u64 bitonic_down(u64 x, int lane) {  // a bitonic row to descending order
+    x = exchange<ST>(x, false, lane);
+    if constexpr (ST > 1) x = bitonic_down<ST / 2>(x, lane);
     return x;
 }
 __device__ __forceinline__ Stat join_lanes(Stat st, float c1) {
@@ -120,18 +126,21 @@ __device__ __forceinline__ u64 lane_value(u64 x, int lane) {  // lane: the same 
            (uint32_t)__builtin_amdgcn_readlane((int)x, lane);
 }
 
-// The 64 best keys a wave has seen, one a lane, best first. Keys above the k-th best wait in LDS;
-// 64 of them at a time are sorted (bitonic, ascending) and merged: max(best, new) of a descending
+// The k best keys a wave has seen, one a lane, best first. Keys above the k-th best wait in LDS until
+// some of them are merged:
+// k <= 8: the list's and the waiting keys each look how many of all are larger: their place. That is
+// 3 instructions a key, a few keys at a time.
+// k > 8: 64 waiting keys are sorted (bitonic, ascending) and merged: max(best, new) of a descending
 // and an ascending row holds the 64 largest as a bitonic row.
 struct Best {
+    static constexpr int ROOM = 192;  // 63 waiting and 64 offered at once (k <= 8: less, and 8 of the list); 64 places
     u64 list = 0, tau = 0;  // tau: no key up to it can be among the k best
     float tau_score = -INFINITY;
     int waiting = 0, k;
-    u64* pend;  // this wave's waiting keys: room for 64 and for what is offered between two flushes
+    u64* pend;
     __device__ Best(u64* p, int kk) : k(kk), pend(p) {}
 
-    __device__ __forceinline__ void take(u64 ascending) {
-        list = bitonic_down(list > ascending ? list : ascending);
+    __device__ __forceinline__ void tighten() {
         const u64 kth = lane_value(list, k - 1);
         if (kth > tau) {
             tau = kth;
@@ -145,13 +154,35 @@ struct Best {
             tau_score = score;
         }
     }
-    __device__ __forceinline__ void flush() {  // the last 64 waiting keys
+    __device__ __forceinline__ void flush() {  // the last waiting keys, as many as go at once
         const int lane = threadIdx.x & 63;
-        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");
-        const int from = max(0, waiting - 64);
-        const u64 x = from + lane < waiting ? pend[from + lane] : 0;
-        waiting = from;
-        if (__any(x > tau)) take(sort_up(x));
+        if (k <= 8) {
+            const int from = max(0, waiting - (64 - k)), total = waiting - from + k;
+            if (lane < k) pend[waiting + lane] = list;
+            wave_lds_order();
+            const u64* all = pend + from;
+            const u64 own = lane < total ? all[lane] : 0;
+            int place = 0;
+#pragma unroll 4
+            for (int j = 0; j < total; ++j) place += all[j] > own ? 1 : 0;
+            const int there = __popcll(__ballot(own != 0));
+            if (own != 0 && place < k) pend[128 + place] = own;
+            wave_lds_order();
+            list = lane < min(k, there) ? pend[128 + lane] : 0;
+            waiting = from;
+            tighten();
+        } else {
+            wave_lds_order();
+            const int from = max(0, waiting - 64);
+            u64 x = from + lane < waiting ? pend[from + lane] : 0;
+            waiting = from;
+            if (!__any(x > tau)) return;
+            take(sort_up(x));
+        }
+    }
+    __device__ __forceinline__ void take(u64 ascending) {
+        list = bitonic_down(list > ascending ? list : ascending, local_lane());
+        tighten();
     }
     __device__ __forceinline__ void offer(u64 key, bool there) {
         const bool in = there && key > tau;
@@ -161,14 +192,9 @@ struct Best {
                                                      __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0))] = key;
         waiting += __popcll(mask);
     }
-    // One score a lane; most hold no lane's candidate, which one comparison shows.
-    __device__ __forceinline__ void offer_score(float x, uint32_t id) {
-        const bool may = x >= tau_score && x > -INFINITY;
-        if (__any(may)) offer(key_of(x, id), may);
-    }
     // Waiting keys are merged once they are worth it: a late tau lets more scores through.
     __device__ __forceinline__ void settle() {
-        const int worth = k <= 32 ? 32 : 64;
+        const int worth = k <= 8 ? 16 : 64;
         while (waiting >= worth) flush();
     }
 };
@@ -244,24 +270,15 @@ struct Step {
 // rows whose largest score is past FAR_SCORE, and for temperatures outside [1e-6, 1e6].
 template <class T>
 __device__ __attribute__((noinline)) Stat far_stats(const T* x, int64_t lo, int64_t hi, float c1) {
-    constexpr int N = Step<T>::N;
     Stat st;
-    for (int64_t at = lo; at < hi; at += Step<T>::SIZE) {
-        Step<T> cur;
-        cur.load(x, at, hi);
-        float f[LP_U][N];
-        cur.values(f, hi - at);
-#pragma unroll
-        for (int u = 0; u < LP_U; ++u)
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const float v = f[u][j], mn = fmaxf(st.m, v);
-                const float d = fmaxf((st.m - mn) * c1, FLOOR_U), r = __builtin_amdgcn_exp2f(d);
-                const float y = (v - mn) * c1, ex = __builtin_amdgcn_exp2f(y);
-                st.e = fmaf(r, fmaf(st.s, d, st.e), ex * fmaxf(y, FLOOR_U));
-                st.s = fmaf(st.s, r, ex);
-                st.m = mn;
-            }
+#pragma unroll 1
+    for (int64_t i = lo + (threadIdx.x & 63); i < hi; i += 64) {
+        const float v = (float)x[i], mn = fmaxf(st.m, v);
+        const float d = fmaxf((st.m - mn) * c1, FLOOR_U), r = __builtin_amdgcn_exp2f(d);
+        const float y = (v - mn) * c1, ex = __builtin_amdgcn_exp2f(y);
+        st.e = fmaf(r, fmaf(st.s, d, st.e), ex * fmaxf(y, FLOOR_U));
+        st.s = fmaf(st.s, r, ex);
+        st.m = mn;
     }
     return st;
 }
@@ -307,11 +324,13 @@ __device__ __forceinline__ Stat walk(const T* __restrict__ x, int64_t lo, int64_
         if constexpr (ENT) {
             if (__any(de != de)) {  // a masked score (0 * -inf) or a NaN
                 de = 0.f;
+                float again = b;  // (hidden: or the 32 values of this path's terms are kept for it)
+                asm volatile("" : "+v"(again));
 #pragma unroll
                 for (int u = 0; u < LP_U; ++u)
 #pragma unroll
                     for (int j = 0; j < N; ++j) {
-                        const float y = fmaf(v[u][j], c1, -b);
+                        const float y = fmaf(v[u][j], c1, -again);
                         de = fmaf(__builtin_amdgcn_exp2f(y), fmaxf(y, FLOOR_U), de);
                     }
             }
@@ -345,10 +364,22 @@ __device__ __forceinline__ Stat walk(const T* __restrict__ x, int64_t lo, int64_
             // the k-th best of the lanes' largest scores of the first step bounds the k-th best score
             if (at == lo) best.bound(__uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(sort_up(cm)), 64 - best.k)));
             if (at == lo || __any(cm > best.tau_score)) {
+                // each lane's candidates as bits, then one of each lane at a time
+                const float from = fmaxf(best.tau_score, -3.402823466e38f);
+                uint32_t bits = 0;
 #pragma unroll
-                for (int u = 0; u < LP_U; ++u) {
+                for (int u = 0; u < LP_U; ++u)
 #pragma unroll
-                    for (int j = 0; j < N; ++j) best.offer_score(v[u][j], (uint32_t)(at + Step<T>::place(u, hi - at) + j));
+                    for (int j = 0; j < N; ++j) bits |= v[u][j] >= from ? 1u << (u * N + j) : 0;
+                while (__any(bits != 0)) {
+                    const bool has = bits != 0;
+                    const int e = has ? __ffs(bits) - 1 : 0;
+                    bits &= bits - 1;
+                    const uint32_t pos = (uint32_t)at + Step<T>::place(e / N, hi - at) + e % N;
+                    float score = v[0][0];
+#pragma unroll
+                    for (int i = 1; i < LP_U * N; ++i) score = e == i ? v[i / N][i % N] : score;
+                    best.offer(key_of(score, pos), has);
                     best.settle();
                 }
             }
@@ -393,7 +424,7 @@ __global__ __launch_bounds__(64 * LP_WAVES) void logprobs_wave_kernel(const T* _
                                                                      int64_t ld, float c1, float inv_t, bool near,
                                                                      const int64_t* __restrict__ targets, int k,
                                                                      LogProbsOut out) {
-    constexpr int ROOM = 64 + 64 * Vec16<T>::N;
+    constexpr int ROOM = Best::ROOM;
     __shared__ u64 pend[TOP ? LP_WAVES * ROOM : 1];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t row = (int64_t)blockIdx.x * LP_WAVES + wave;
@@ -415,9 +446,10 @@ __global__ __launch_bounds__(64 * LP_WAVES) void logprobs_block_kernel(const T* 
                                                                       const int64_t* __restrict__ targets, int k,
                                                                       int splits, int64_t seg_len, Part* parts, u64* keys,
                                                                       LogProbsOut out) {
-    constexpr int ROOM = 64 + 64 * Vec16<T>::N;
+    constexpr int ROOM = Best::ROOM;
     __shared__ u64 pend[TOP ? LP_WAVES * ROOM : 1];
     __shared__ Part found[LP_WAVES];
+    __shared__ u64 lists[TOP ? LP_WAVES : 1][64];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t row = blockIdx.x / splits;
@@ -428,7 +460,7 @@ __global__ __launch_bounds__(64 * LP_WAVES) void logprobs_block_kernel(const T* 
     Best best(TOP ? pend + wave * ROOM : nullptr, k);
     Stat st = walk<T, ENT, RANK, TOP>(x, lo, hi, c1, near, r.target, r.score, before, best);
     if (lane == 0) found[wave] = Part{st.m, st.s, st.e, before};
-    if constexpr (TOP) pend[wave * ROOM + lane] = best.list;
+    if constexpr (TOP) lists[wave][lane] = best.list;
     __syncthreads();
     if (wave) return;
 #pragma unroll
@@ -437,7 +469,7 @@ __global__ __launch_bounds__(64 * LP_WAVES) void logprobs_block_kernel(const T* 
         b.m = found[w].m, b.s = found[w].s, b.e = found[w].e;
         st = join(st, b, c1);
         before += found[w].before;
-        if constexpr (TOP) best.take(pend[w * ROOM + 63 - lane]);
+        if constexpr (TOP) best.take(lists[w][63 - lane]);
     }
     if (!parts) {
         if (lane == 0) write_row(st, before, row, r.score, r.there, inv_t, out);
@@ -455,7 +487,7 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(const T* __restrict__
                                                            float inv_t, const int64_t* __restrict__ targets, int k,
                                                            int splits, const Part* __restrict__ parts,
                                                            const u64* __restrict__ keys, LogProbsOut out) {
-    __shared__ u64 pend[64 + 8 * 64];
+    __shared__ u64 pend[Best::ROOM];
     const int lane = threadIdx.x;
     const int64_t row = blockIdx.x;
     const Row r(scores + row * ld, targets, row, c);
@@ -484,9 +516,11 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(const T* __restrict__
             u64 x[8];
 #pragma unroll
             for (int u = 0; u < 8; ++u) x[u] = i + u * 64 + lane < total ? list[i + u * 64 + lane] : 0;
-#pragma unroll
-            for (int u = 0; u < 8; ++u) best.offer(x[u], x[u] != 0);
-            while (best.waiting >= 64) best.flush();
+            for (int u = 0; u < 8; ++u)
+                if (__any(x[u] > best.tau)) {
+                    best.offer(x[u], x[u] != 0);
+                    best.settle();
+                }
         }
         if (best.waiting) best.flush();
         write_top(best.list, k, row, st, inv_t, out);
@@ -570,7 +604,7 @@ void log_probs(int32_t dtype, const void* scores, int64_t n, int64_t c, int64_t 
         // blocks as give every CU 4: the loads of fewer waves do not hide each other.
         const int cus = device().num_cus;
         const int64_t steps = (c + STEP - 1) / STEP;
-        const bool by_wave = n >= 16LL * cus || steps == 1;
+        const bool by_wave = n >= 8LL * cus || steps == 1;
         int64_t splits = std::max<int64_t>(1, std::min<int64_t>((4LL * cus + n - 1) / n, (steps + LP_WAVES - 1) / LP_WAVES));
         const int64_t seg = (steps + splits * LP_WAVES - 1) / (splits * LP_WAVES) * STEP;
         splits = by_wave ? 1 : (c + seg * LP_WAVES - 1) / (seg * LP_WAVES);
