@@ -86,6 +86,9 @@ rvx_status rvx_device_info(int32_t* num_cus, int64_t* hbm_bytes, char* arch, siz
 typedef struct rvx_buffer rvx_buffer;
 rvx_status rvx_buffer_alloc(int64_t bytes, rvx_buffer** out);
 rvx_status rvx_buffer_free(rvx_buffer* buf);
+/* A DLManagedTensor (DLPack) over the whole buffer: one dimension of bytes, no copy. The memory
+ * lives until both the handle is freed and the tensor's deleter has run. */
+rvx_status rvx_buffer_tensor(rvx_buffer* buf, void** out);
 int64_t    rvx_buffer_bytes(const rvx_buffer* buf);
 void*      rvx_buffer_device_ptr(rvx_buffer* buf);
 rvx_status rvx_buffer_upload(rvx_buffer* buf, const void* src, int64_t bytes, int64_t offset);

@@ -9,7 +9,7 @@ import ctypes as C
 from typing import Optional
 
 from . import _lib as L
-from .device import Buffer, dtype_code
+from .device import Buffer, dtype_code, int32
 
 
 class AdapterError(L.RvxError):
@@ -32,18 +32,19 @@ class AdapterLinear:
         self._h = None
         self.in_features, self.out_features, self.dtype = in_features, out_features, dtype
         self.max_rank, self.max_adapters = max_rank, max_adapters
-        cfg = L.AdapterLinearConfig(in_features, out_features, dtype_code(dtype), max_rank, max_adapters)
+        cfg = L.AdapterLinearConfig(int32(in_features, "in_features"), int32(out_features, "out_features"), dtype_code(dtype),
+                                    int32(max_rank, "max_rank"), int32(max_adapters, "max_adapters"))
         h = C.c_void_p()
         _check("rvx_adapter_linear_create", C.byref(cfg), weight.handle, None if bias is None else bias.handle, C.byref(h))
         self._h = h
 
     def set_adapter(self, slot: int, rank: int, a: Buffer, b: Buffer, scale: float = 1.0) -> None:
         """Slot `slot` gets a [rank][in] and b [out][rank] of the layer's dtype (rank <= max_rank)."""
-        _check("rvx_adapter_linear_set", self._h, int(slot), int(rank), a.handle, b.handle, float(scale))
+        _check("rvx_adapter_linear_set", self._h, int32(slot, "slot"), int32(rank, "rank"), a.handle, b.handle, float(scale))
 
     def clear_adapter(self, slot: int) -> None:
         """Rows of `slot` have no adapter from now on."""
-        _check("rvx_adapter_linear_set", self._h, int(slot), 0, None, None, 1.0)
+        _check("rvx_adapter_linear_set", self._h, int32(slot, "slot"), 0, None, None, 1.0)
 
     def forward_device(self, x: Buffer, n: int, y: Buffer, adapter_ids: Optional[Buffer] = None) -> None:
         """x [n][in] -> y [n][out]; adapter_ids int32 [n], ids without an adapter (-1) get none."""

@@ -11,11 +11,12 @@ namespace {
 
 constexpr int64_t MAX_INDEX = ((int64_t)1 << 31) - 1;
 
-void check_embedding(int32_t dtype, int64_t rows, int32_t dim, int64_t n) {
+void check_embedding(int32_t dtype, int64_t rows, int32_t dim, int64_t n, float scale) {
     check_dtype(dtype);
     RVX_REQUIRE(rows >= 1 && rows < MAX_INDEX, RVX_ERR_INVALID_PARAMETER, "rows must be in [1, 2^31 - 1)");
     RVX_REQUIRE(dim >= 1 && dim <= EMBED_MAX_DIM, RVX_ERR_INVALID_PARAMETER, "dim must be in [1, 65536]");
     RVX_REQUIRE(n >= 0 && n <= MAX_INDEX, RVX_ERR_INVALID_PARAMETER, "n must be in [0, 2^31)");
+    RVX_REQUIRE(std::isfinite(scale), RVX_ERR_INVALID_PARAMETER, "scale must be finite");
 }
 
 void check_scores(int32_t dtype, int64_t n, int64_t c, int64_t ld, float temperature) {
@@ -38,7 +39,7 @@ extern "C" {
 rvx_status rvx_embedding_forward_device(const rvx_buffer* table, int32_t dtype, int64_t rows, int32_t dim,
                                         const rvx_buffer* ids, int64_t n, float scale, rvx_buffer* out) {
     return guard([&] {
-        check_embedding(dtype, rows, dim, n);
+        check_embedding(dtype, rows, dim, n, scale);
         const int size = dtype_size(dtype);
         check_rows(table, "table", rows, dim, dim, size);
         check_rows(ids, "ids", n, 1, 1, 8);
@@ -55,7 +56,7 @@ rvx_status rvx_embedding_backward_device(const rvx_buffer* grad_out, int32_t dty
                                          int64_t rows, int32_t dim, float scale, int32_t accumulate,
                                          int32_t table_dtype, rvx_buffer* grad_table) {
     return guard([&] {
-        check_embedding(dtype, rows, dim, n);
+        check_embedding(dtype, rows, dim, n, scale);
         check_dtype(table_dtype);
         check_rows(grad_out, "grad_out", n, dim, dim, dtype_size(dtype));
         check_rows(ids, "ids", n, 1, 1, 8);

@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
 #include <cstdio>
 #include <cstdlib>
@@ -168,4 +169,5 @@ __device__ __forceinline__ float h2_scale_dev(float m) {
 
 struct rvx_buffer {
     rvx::DevMem mem;
+    std::atomic<int> holders{1};  // the handle and the tensors over it; the last to go frees it
 };

@@ -13,7 +13,7 @@ namespace {
 
 constexpr float LN2 = 0.69314718055994530942f, LOG2E = 1.44269504088896340736f;
 constexpr float FLOOR_U = -1e4f;   // 2^u is 0 long before; keeps 0 * u finite for masked scores
-constexpr float FAR_SCORE = 1e30f; // past it the one-fma form of u could overflow
+constexpr float FAR_U = 67108864.0f;  // 2^26: past it fl(m c1) may be off by more than 2^u can take
 using u64 = unsigned long long;
 
 struct Stat {
@@ -266,8 +266,8 @@ struct Step {
     }
 };
 
-// S and E by subtraction of the running maximum itself: right for scores of any size. Only for
-// rows whose largest score is past FAR_SCORE, and for temperatures outside [1e-6, 1e6].
+// S and E by subtraction of the running maximum itself: right for scores of any size. Only where a
+// row's largest |score| / T is past FAR_U.
 template <class T>
 __device__ __attribute__((noinline)) Stat far_stats(const T* x, int64_t lo, int64_t hi, float c1) {
     Stat st;
@@ -286,13 +286,14 @@ __device__ __attribute__((noinline)) Stat far_stats(const T* x, int64_t lo, int6
 // A wave goes over elements [lo, hi) of a row. Bound by reading them: per score one unpack, half a
 // max, one fma, one exp (4 cycles), two additions and one comparison.
 template <class T, bool ENT, bool RANK, bool TOP>
-__device__ __forceinline__ Stat walk(const T* __restrict__ x, int64_t lo, int64_t hi, float c1, bool near, int64_t target,
+__device__ __forceinline__ Stat walk(const T* __restrict__ x, int64_t lo, int64_t hi, float c1, int64_t target,
                                      float st_score, int& before, Best& best) {
     constexpr int N = Step<T>::N, SIZE = Step<T>::SIZE;
     const int lane = threadIdx.x & 63;
     // 2^u is taken against b = fl(m c1), the lane's largest score in log2 units: u = fma(x, c1, -b) is
     // rounded once, and what b is off from m c1 is put right at the end.
-    float m = -INFINITY, b = -FAR_SCORE * c1, s = 0.f, e = 0.f;
+    const float far = fminf(FAR_U / c1, 1e30f);
+    float m = -INFINITY, b = -far * c1, s = 0.f, e = 0.f;
     Step<T> nxt;
     if (lo < hi) nxt.load(x, lo, hi);
     for (int64_t at = lo; at < hi; at += SIZE) {
@@ -306,7 +307,7 @@ __device__ __forceinline__ Stat walk(const T* __restrict__ x, int64_t lo, int64_
             for (int j = 0; j < N; ++j) cm = fmaxf(cm, v[u][j]);
         if (__any(cm > m)) {
             m = fmaxf(m, cm);
-            const float bn = fminf(fmaxf(m, -FAR_SCORE), FAR_SCORE) * c1;
+            const float bn = fminf(fmaxf(m, -far), far) * c1;
             const float d = fmaxf(b - bn, FLOOR_U), r = __builtin_amdgcn_exp2f(d);
             if constexpr (ENT) e = r * fmaf(s, d, e);
             s *= r;
@@ -394,13 +395,12 @@ __device__ __forceinline__ Stat walk(const T* __restrict__ x, int64_t lo, int64_
         st.e = r * fmaf(s, d, e);
         st.s = s * r;
     }
-    const bool far = fabsf(m) > FAR_SCORE && m != -INFINITY;
-    if (!near || __any(far)) {
-        // lanes past FAR_SCORE count only where the row's largest score is there too
+    if (__any(fabsf(m) > far && m != -INFINITY)) {
+        // lanes past it count only where the largest score is there too
         float mw = m;
         mw = fmaxf(mw, lane_xor<32>(mw)), mw = fmaxf(mw, lane_xor<16>(mw)), mw = fmaxf(mw, lane_xor<8>(mw));
         mw = fmaxf(mw, lane_xor<4>(mw)), mw = fmaxf(mw, lane_xor<2>(mw)), mw = fmaxf(mw, lane_xor<1>(mw));
-        if (!near || (fabsf(mw) > FAR_SCORE && mw != -INFINITY)) st = far_stats(x, lo, hi, c1);
+        if (fabsf(mw) > far) st = far_stats(x, lo, hi, c1);
     }
     return join_lanes(st, c1);
 }
@@ -421,7 +421,7 @@ struct Row {  // a row's target
 // A wave a row (many rows).
 template <class T, bool ENT, bool RANK, bool TOP>
 __global__ __launch_bounds__(64 * LP_WAVES) void logprobs_wave_kernel(const T* __restrict__ scores, int64_t n, int64_t c,
-                                                                     int64_t ld, float c1, float inv_t, bool near,
+                                                                     int64_t ld, float c1, float inv_t,
                                                                      const int64_t* __restrict__ targets, int k,
                                                                      LogProbsOut out) {
     constexpr int ROOM = Best::ROOM;
@@ -433,7 +433,7 @@ __global__ __launch_bounds__(64 * LP_WAVES) void logprobs_wave_kernel(const T* _
     const Row r(x, targets, row, c);
     int before = 0;
     Best best(TOP ? pend + wave * ROOM : nullptr, k);
-    const Stat st = walk<T, ENT, RANK, TOP>(x, 0, c, c1, near, r.target, r.score, before, best);
+    const Stat st = walk<T, ENT, RANK, TOP>(x, 0, c, c1, r.target, r.score, before, best);
     if ((threadIdx.x & 63) == 0) write_row(st, before, row, r.score, r.there, inv_t, out);
     if constexpr (TOP) write_top(best.list, k, row, st, inv_t, out);
 }
@@ -442,7 +442,7 @@ __global__ __launch_bounds__(64 * LP_WAVES) void logprobs_wave_kernel(const T* _
 // parts == null: the block has the whole row.
 template <class T, bool ENT, bool RANK, bool TOP>
 __global__ __launch_bounds__(64 * LP_WAVES) void logprobs_block_kernel(const T* __restrict__ scores, int64_t c, int64_t ld,
-                                                                      float c1, float inv_t, bool near,
+                                                                      float c1, float inv_t,
                                                                       const int64_t* __restrict__ targets, int k,
                                                                       int splits, int64_t seg_len, Part* parts, u64* keys,
                                                                       LogProbsOut out) {
@@ -458,7 +458,7 @@ __global__ __launch_bounds__(64 * LP_WAVES) void logprobs_block_kernel(const T* 
     const Row r(x, targets, row, c);
     int before = 0;
     Best best(TOP ? pend + wave * ROOM : nullptr, k);
-    Stat st = walk<T, ENT, RANK, TOP>(x, lo, hi, c1, near, r.target, r.score, before, best);
+    Stat st = walk<T, ENT, RANK, TOP>(x, lo, hi, c1, r.target, r.score, before, best);
     if (lane == 0) found[wave] = Part{st.m, st.s, st.e, before};
     if constexpr (TOP) lists[wave][lane] = best.list;
     __syncthreads();
@@ -596,7 +596,6 @@ __global__ __launch_bounds__(256) void logprobs_backward_kernel(
 void log_probs(int32_t dtype, const void* scores, int64_t n, int64_t c, int64_t ld, float temperature,
                const int64_t* targets, int k, const LogProbsOut& out) {
     const float inv_t = (float)(1.0 / (double)temperature), c1 = (float)(1.44269504088896340736 / (double)temperature);
-    const bool near = temperature >= 1e-6f && temperature <= 1e6f;
     with_dtype(dtype, [&](auto zero) {
         using T = decltype(zero);
         constexpr int64_t STEP = Step<T>::SIZE;
@@ -631,10 +630,10 @@ void log_probs(int32_t dtype, const void* scores, int64_t n, int64_t c, int64_t 
                 if (by_wave)
                     RVX_LAUNCH("log_probs", (logprobs_wave_kernel<T, E, R, K>),
                                dim3((unsigned)((rows + LP_WAVES - 1) / LP_WAVES)), dim3(64 * LP_WAVES), 0, x, rows, c, ld, c1,
-                               inv_t, near, t, k, o);
+                               inv_t, t, k, o);
                 else
                     RVX_LAUNCH("log_probs", (logprobs_block_kernel<T, E, R, K>), dim3((unsigned)(rows * splits)),
-                               dim3(64 * LP_WAVES), 0, x, c, ld, c1, inv_t, near, t, k, (int)splits, seg, parts, keys, o);
+                               dim3(64 * LP_WAVES), 0, x, c, ld, c1, inv_t, t, k, (int)splits, seg, parts, keys, o);
             };
             auto flag = [](bool on, auto&& f) {
                 if (on) f(std::true_type{});

@@ -197,6 +197,33 @@ KernelTimer::~KernelTimer() {
     if (g_prof.pending.size() > 4096) g_prof.drain();
 }
 
+// DLPack's DLManagedTensor (its DLTensor first), with what it points to.
+struct ManagedTensor {
+    void* data;
+    int32_t device_type, device_id, ndim;
+    uint8_t code, bits;
+    uint16_t lanes;
+    int64_t *shape, *strides;
+    uint64_t byte_offset;
+    void* context;
+    void (*deleter)(ManagedTensor*);
+};
+struct BufferTensor {
+    ManagedTensor dl;
+    int64_t size = 0, step = 1;
+    rvx_buffer* of = nullptr;
+};
+
+void let_go(rvx_buffer* buf) {
+    if (buf && buf->holders.fetch_sub(1) == 1) delete buf;
+}
+void release_tensor(ManagedTensor* t) {
+    if (!t) return;
+    auto* b = static_cast<BufferTensor*>(t->context);
+    let_go(b->of);
+    delete b;
+}
+
 }  // namespace rvx
 
 using namespace rvx;
@@ -289,7 +316,18 @@ rvx_status rvx_buffer_alloc(int64_t bytes, rvx_buffer** out) {
     });
 }
 rvx_status rvx_buffer_free(rvx_buffer* buf) {
-    return guard([&] { delete buf; });
+    return guard([&] { let_go(buf); });
+}
+rvx_status rvx_buffer_tensor(rvx_buffer* buf, void** out) {
+    return guard([&] {
+        RVX_REQUIRE(buf && out, RVX_ERR_INVALID_PARAMETER, "null argument");
+        auto t = std::make_unique<BufferTensor>();
+        t->of = buf;
+        t->size = buf->mem.bytes;
+        t->dl = {buf->mem.p, 10 /* ROCm */, buf->mem.dev, 1, 1 /* unsigned */, 8, 1, &t->size, &t->step, 0, t.get(), release_tensor};
+        buf->holders.fetch_add(1);
+        *out = &t.release()->dl;
+    });
 }
 int64_t rvx_buffer_bytes(const rvx_buffer* buf) { return buf ? buf->mem.bytes : 0; }
 void* rvx_buffer_device_ptr(rvx_buffer* buf) { return buf ? buf->mem.p : nullptr; }

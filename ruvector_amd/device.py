@@ -56,25 +56,12 @@ def dtype_code(dtype: str) -> int:
         raise L.RvxError(2, f"unknown dtype {dtype!r}: one of {', '.join(_DTYPES)}") from None
 
 
-class _DLTensor(C.Structure):
-    _fields_ = [("data", C.c_void_p), ("device_type", C.c_int32), ("device_id", C.c_int32), ("ndim", C.c_int32),
-                ("code", C.c_uint8), ("bits", C.c_uint8), ("lanes", C.c_uint16), ("shape", C.POINTER(C.c_int64)),
-                ("strides", C.POINTER(C.c_int64)), ("byte_offset", C.c_uint64)]
-
-
-class _DLManaged(C.Structure):
-    pass
-
-
-_DLDeleter = C.CFUNCTYPE(None, C.POINTER(_DLManaged))
-_DLManaged._fields_ = [("tensor", _DLTensor), ("ctx", C.c_void_p), ("deleter", _DLDeleter)]
-_DL_ROCM = 10
-_exported = {}  # address of a _DLManaged -> what it needs alive until its consumer is done
-
-
-@_DLDeleter
-def _dl_release(managed):
-    _exported.pop(C.addressof(managed.contents), None)
+def int32(value, what: str) -> int:
+    """`value` as a C int32 argument (ctypes would cut a larger one short)."""
+    value = int(value)
+    if not -2 ** 31 <= value < 2 ** 31:
+        raise L.RvxError(2, f"{what} {value} is not a 32-bit number")
+    return value
 
 
 _capsule_new = C.PYFUNCTYPE(C.py_object, C.c_void_p, C.c_char_p, C.c_void_p)(("PyCapsule_New", C.pythonapi))
@@ -82,10 +69,20 @@ _capsule_valid = C.PYFUNCTYPE(C.c_int, C.c_void_p, C.c_char_p)(("PyCapsule_IsVal
 _capsule_pointer = C.PYFUNCTYPE(C.c_void_p, C.c_void_p, C.c_char_p)(("PyCapsule_GetPointer", C.pythonapi))
 
 
+class _DLManaged(C.Structure):
+    """DLManagedTensor, as far as its deleter."""
+    _fields_ = [("tensor", C.c_byte * 48), ("context", C.c_void_p), ("deleter", C.CFUNCTYPE(None, C.c_void_p))]
+
+
 @C.CFUNCTYPE(None, C.c_void_p)
-def _dl_dropped(capsule):
-    if _capsule_valid(capsule, b"dltensor"):  # no consumer took it
-        _exported.pop(_capsule_pointer(capsule, b"dltensor"), None)
+def _capsule_dropped(capsule, valid=_capsule_valid, pointer=_capsule_pointer, managed=_DLManaged):
+    if valid(capsule, b"dltensor"):  # no consumer took it
+        p = pointer(capsule, b"dltensor")
+        managed.from_address(p).deleter(p)
+
+
+# A capsule can be dropped while the interpreter ends, after this module's names are gone.
+C.pythonapi.Py_IncRef(C.py_object(_capsule_dropped))
 
 
 class Buffer:
@@ -105,21 +102,27 @@ class Buffer:
         return self._h
 
     def __dlpack_device__(self):
-        return (_DL_ROCM, self._device)
+        return (10, self._device)  # ROCm
 
     def __dlpack__(self, stream=None, **_):
         """The allocation as a flat uint8 tensor of another library (DLPack, no copy): what that
         library queues on `stream` waits for the library's work so far. What it writes is ordered
-        before later rvx calls by stream_wait(stream). The tensor keeps this Buffer alive."""
+        before later rvx calls by stream_wait(stream). The memory lives until both the Buffer and the
+        tensor are gone. torch has to be imported before this library is first used: the two then
+        share one HIP runtime."""
         if not self._h:
             raise L.RvxError(2, "the buffer is freed")
         if stream != -1:
-            stream_signal(0 if stream in (None, 1) else stream)
-        shape, strides = (C.c_int64 * 1)(self.nbytes), (C.c_int64 * 1)(1)
-        m = _DLManaged(_DLTensor(L.load().rvx_buffer_device_ptr(self._h), _DL_ROCM, self._device, 1, 1, 8, 1, shape,
-                                 strides, 0), None, _dl_release)
-        _exported[C.addressof(m)] = (m, self, shape, strides)
-        return _capsule_new(C.addressof(m), b"dltensor", C.cast(_dl_dropped, C.c_void_p))
+            dev = C.c_int32(0)
+            L.call("rvx_get_device", C.byref(dev))
+            set_device(self._device)
+            try:
+                stream_signal(0 if stream in (None, 1) else stream)
+            finally:
+                set_device(dev.value)
+        p = C.c_void_p()
+        L.call("rvx_buffer_tensor", self._h, C.byref(p))
+        return _capsule_new(p.value, b"dltensor", C.cast(_capsule_dropped, C.c_void_p))
 
     @classmethod
     def from_numpy(cls, a: np.ndarray) -> "Buffer":

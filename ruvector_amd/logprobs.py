@@ -10,7 +10,7 @@ from __future__ import annotations
 from typing import Optional
 
 from . import _lib as L
-from .device import Buffer, dtype_code
+from .device import Buffer, dtype_code, int32
 
 
 class LogProbsError(L.RvxError):
@@ -39,7 +39,7 @@ def log_probs_device(scores: Buffer, n: int, c: int, temperature: float = 1.0, t
     log_probs_backward_device, and the k <= 64 best ids top_ids [n][k] int64 with top_logp [n][k]
     f32 (lowest id first among equals; -1 / -inf past the scores above -inf)."""
     _check("rvx_log_probs_device", scores.handle, dtype_code(dtype), n, c, c if ld is None else ld, temperature,
-           _h(targets), k, _h(logp), _h(rank), _h(entropy), _h(stats), _h(top_ids), _h(top_logp))
+           _h(targets), int32(k, "k"), _h(logp), _h(rank), _h(entropy), _h(stats), _h(top_ids), _h(top_logp))
 
 
 def log_probs_backward_device(scores: Buffer, n: int, c: int, temperature: float, stats: Buffer, grad: Buffer,

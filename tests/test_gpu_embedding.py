@@ -142,21 +142,107 @@ def test_gradient_is_the_forward_pass_differentiated():
 def test_refusals():
     t, ids, out = rv.Buffer(64 * 4), rv.Buffer(8 * 8), rv.Buffer(8 * 8 * 4)
     rv.embedding_forward_device(t, 8, 8, ids, 8, out)
-    for bad in (dict(rows=9), dict(dim=9), dict(n=9), dict(dtype="f64"), dict(dim=0), dict(rows=0), dict(n=-1),
+    for bad in (dict(scale=math.inf), dict(scale=math.nan), dict(dim=2 ** 32 + 8), dict(rows=9), dict(dim=9), dict(n=9), dict(dtype="f64"), dict(dim=0), dict(rows=0), dict(n=-1),
                 dict(out=t), dict(out=ids)):
-        a = dict(dict(rows=8, dim=8, n=8, out=out, dtype="f32"), **bad)
+        a = dict(dict(rows=8, dim=8, n=8, out=out, dtype="f32", scale=1.0), **bad)
         with pytest.raises(rv.RvxError):
-            rv.embedding_forward_device(t, a["rows"], a["dim"], ids, a["n"], a["out"], dtype=a["dtype"])
+            rv.embedding_forward_device(t, a["rows"], a["dim"], ids, a["n"], a["out"], dtype=a["dtype"], scale=a["scale"])
         with pytest.raises(rv.RvxError):
-            rv.embedding_backward_device(t, ids, a["n"], a["rows"], a["dim"], t if a["out"] is t else a["out"], dtype=a["dtype"])
+            rv.embedding_backward_device(t, ids, a["n"], a["rows"], a["dim"], t if a["out"] is t else a["out"], dtype=a["dtype"],
+                                         scale=a["scale"])
 
 
-def test_dlpack_views_share_the_buffer():
-    b = rv.Buffer.from_numpy(torch.arange(12, dtype=torch.float32).numpy())
-    v = torch.from_dlpack(b).view(torch.float32)
-    assert v.is_cuda and torch.equal(v.cpu(), torch.arange(12, dtype=torch.float32))
-    v.mul_(2)
-    rv.stream_wait(torch.cuda.current_stream().cuda_stream)
-    assert torch.equal(from_buffer(b, (12,), torch.float32), 2 * torch.arange(12, dtype=torch.float32))
-    del b
-    assert v.cpu()[3] == 6
+# torch brings its own HIP runtime: it has to be loaded before librvx for the two to share the GPU
+INTEROP = """
+import gc
+import torch
+import ruvector_amd as rv
+b = rv.Buffer.from_numpy(torch.arange(12, dtype=torch.float32).numpy())
+assert b.__dlpack_device__()[0] == 10
+v = torch.from_dlpack(b).view(torch.float32)
+assert v.is_cuda and v.data_ptr() % 256 == 0 and torch.equal(v.cpu(), torch.arange(12, dtype=torch.float32))
+side = torch.cuda.Stream()
+rows, dim, n = 5000, 256, 20000
+table, ids, out = rv.Buffer(rows * dim * 4), rv.Buffer(n * 8), rv.Buffer(n * dim * 4)
+t = torch.from_dlpack(table).view(torch.float32).view(rows, dim)
+i = torch.from_dlpack(ids).view(torch.int64)
+o = torch.from_dlpack(out).view(torch.float32).view(n, dim)
+torch.cuda.synchronize()
+for step in range(3):
+    # written on another stream, used by the library, read on that stream: ordered on the GPU alone
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+        t.copy_(torch.randn(rows, dim, device="cuda"))
+        i.copy_(torch.randint(0, rows, (n,), device="cuda"))
+        rv.stream_wait(side.cuda_stream)
+        rv.embedding_forward_device(table, rows, dim, ids, n, out, scale=2.0)
+        rv.stream_signal(side.cuda_stream)
+        assert torch.equal(o, t[i] * 2), step
+b.free()
+del b
+gc.collect()
+assert v.cpu()[3] == 3                      # the view keeps the memory
+big = rv.Buffer(1 << 30)
+w = torch.from_dlpack(big)
+taken = torch.cuda.mem_get_info()[0]
+del w                                       # the Buffer keeps it
+assert torch.cuda.mem_get_info()[0] < taken + (1 << 29)
+c = big.__dlpack__(stream=-1)               # a capsule nobody takes
+big.free()
+assert torch.cuda.mem_get_info()[0] < taken + (1 << 29)
+del c
+assert torch.cuda.mem_get_info()[0] >= taken + (1 << 29)
+late = table.__dlpack__(stream=-1)          # this, and the views above, go with the interpreter
+print("interop ok", flush=True)
+"""
+
+
+def test_dlpack_views_and_stream_order():
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-u", "-c", INTEROP], cwd=root, capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and "interop ok" in r.stdout, r.stdout + r.stderr
+
+
+def test_offsets_past_32_bits():
+    """A table of more than 2^31 elements: rows at its end, forward, and their gradient."""
+    rows, dim = 2 ** 21 + 5, 1024
+    table = rv.Buffer(rows * dim * 4)
+    table.fill_uniform(rows * dim, 3)
+    ids = torch.tensor([rows - 1, 0, rows - 2, rows, rows - 1, 2 ** 21], dtype=torch.int64)
+    out = out_buffer((6, dim), torch.float32)
+    rv.embedding_forward_device(table, rows, dim, to_buffer(ids), 6, out)
+    want = torch.from_numpy(table.gather_rows(rows, dim, ids.clamp(0, rows - 1).numpy())).clone()
+    want[3] = 0
+    assert torch.equal(from_buffer(out, (6, dim), torch.float32), want)
+    for n in (6, 1500):  # both ways of grouping
+        many = ids.repeat(n // 6)
+        g = torch.randint(-3, 4, (n, dim)).float()
+        before = torch.from_numpy(table.gather_rows(rows, dim, [rows - 1, 2 ** 21, rows - 3]))
+        rv.embedding_backward_device(to_buffer(g), to_buffer(many), n, rows, dim, table, accumulate=True)
+        after = torch.from_numpy(table.gather_rows(rows, dim, [rows - 1, 2 ** 21, rows - 3]))
+        assert_within(after[0], before[0].double() + g[many == rows - 1].double().sum(0), (after[0].abs() + 1).double() * F32)
+        assert_within(after[1], before[1].double() + g[many == 2 ** 21].double().sum(0), (after[1].abs() + 1).double() * F32)
+        assert torch.equal(after[2], before[2])
+
+
+def test_calls_from_several_threads():
+    import threading
+    cases = [_grad_case("f32", "f32", 200 + t, 64, 3000 + 500 * t, "zipf", False, seed=t) for t in range(4)]
+    fails = []
+
+    def work(case):
+        dy, ids, start, want, tol = case
+        try:
+            for _ in range(5):
+                assert_within(_grad(dy, ids, start, "f32", "f32", False), want, tol)
+        except Exception as e:  # noqa: BLE001
+            fails.append(e)
+    threads = [threading.Thread(target=work, args=(c,)) for c in cases]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not fails, fails

@@ -136,6 +136,48 @@ def test_ties_and_orders(dtype, shape, n, c, k):
     check(scores, targets, 1.0, k, dtype)
 
 
+@pytest.mark.parametrize("scale,temperature", [(1e5, 1.0), (1e8, 1.0), (1e20, 1e18), (1e30, 1.0), (3e38, 1e37), (1.0, 1e-7), (1e-30, 1e-31),
+                                               (1e3, 1e7), (10.0, 3e38)])
+@pytest.mark.parametrize("c", [70, 9000])
+def test_scores_and_temperatures_of_any_size(scale, temperature, c):
+    scores, targets = make(5, c, "f32", spread=1.0)
+    scores = (scores.clamp(-1, 1) * scale).float()
+    scores[0] += scale * 0.0 if scale > 1e37 else scale  # all positive
+    scores[1, ::2] = -math.inf
+    targets[:3] = scores[:3].argmax(1)
+    got = forward(scores, targets, temperature, 3, "f32")
+    want, _ = reference(scores, targets, temperature, 3)
+    # u is off by 3 roundings of itself; what is over 40 below the best adds nothing, so log p is off by
+    # that of the scores within 40 and by its own size's roundings, E (|u| e^u) as in check()
+    _, s_err = tolerances(scores, 1.0)
+    row = s_err + 3 * F32 * 40
+    assert_within(got["stats"][:, 1], want["stats"][:, 1], row)
+    assert_within(got["logp"], want["logp"], row + 4 * F32 * want["logp"].abs().nan_to_num(0, 0, 0))
+    assert_within(got["entropy"], want["entropy"], 4 * (1 + 2 * math.log(c)) * s_err + 8 * F32 * 40)
+    assert torch.equal(got["top_ids"], want["top_ids"]) and torch.equal(got["rank"], want["rank"])
+
+
+def test_offsets_past_32_bits():
+    """Rows more than 2^31 elements apart, of which 500 are used."""
+    ld, c = 2 ** 31 + 64, 500
+    big = rv.Buffer((ld + c) * 2)
+    scores, targets = make(2, c, "bf16")
+    for r in range(2):
+        big.upload(scores[r].view(torch.uint8).numpy(), offset=r * ld * 2)
+    outs = dict(logp=rv.Buffer(8), rank=rv.Buffer(16), stats=rv.Buffer(16), entropy=rv.Buffer(8))
+    rv.log_probs_device(big, 2, c, 1.0, targets=to_buffer(targets), ld=ld, dtype="bf16", **outs)
+    small = forward(scores, targets, 1.0, 0, "bf16")
+    assert torch.equal(from_buffer(outs["logp"], (2,), torch.float32), small["logp"])
+    assert torch.equal(from_buffer(outs["rank"], (2,), torch.int64), small["rank"])
+    rv.log_probs_backward_device(big, 2, c, 1.0, outs["stats"], big, targets=to_buffer(targets), grad_logp=to_buffer(torch.ones(2)),
+                                 ld=ld, dtype="bf16")
+    import numpy as np
+    want = backward(scores, targets, 1.0, torch.ones(2), None, "bf16")
+    for r in range(2):
+        got = torch.from_numpy(big.download(np.uint8, (c * 2,), offset=r * ld * 2)).view(torch.bfloat16)
+        assert torch.equal(got, want[r])
+
+
 def test_nan_and_inf():
     scores, targets = make(4, 3000, "f32")
     scores[0, 17] = math.nan
@@ -255,7 +297,7 @@ def test_refusals():
     s, t, f = rv.Buffer(4 * 16 * 4), rv.Buffer(4 * 8), rv.Buffer(4 * 4)
     rv.log_probs_device(s, 4, 16, targets=t, logp=f)
     for bad in (dict(n=5), dict(c=17), dict(c=0), dict(ld=15), dict(temperature=0.0), dict(temperature=-1.0),
-                dict(temperature=math.nan), dict(temperature=math.inf), dict(k=65), dict(k=-1), dict(dtype="int8"),
+                dict(temperature=math.nan), dict(temperature=math.inf), dict(k=65), dict(k=-1), dict(k=2 ** 32), dict(dtype="int8"),
                 dict(targets=None), dict(logp=s), dict(logp=t), dict(logp=f, entropy=f), dict(top_ids=f), dict(k=2, top_ids=f),
                 dict(n=-1), dict(stats=f)):
         a = dict(dict(n=4, c=16, temperature=1.0, targets=t, logp=f), **bad)

@@ -22,6 +22,20 @@ def test_embedding(dtype, rows, dim, n, word):
     assert st == 2 and word in msg
 
 
+@pytest.mark.parametrize("scale", [float("inf"), float("nan")])
+def test_embedding_scale(scale):
+    assert _status("rvx_embedding_forward_device", None, 0, 8, 8, None, 8, scale, None)[0] == 2
+    assert _status("rvx_embedding_backward_device", None, 0, None, 8, 8, 8, scale, 0, 0, None)[0] == 2
+
+
+def test_numbers_past_32_bits():
+    from ruvector_amd.device import int32
+    assert int32(-2 ** 31, "k") == -2 ** 31
+    for bad in (2 ** 31, -2 ** 31 - 1, 2 ** 32 + 8):
+        with pytest.raises(rv.RvxError):
+            int32(bad, "k")
+
+
 def test_embedding_table_dtype():
     st, msg = _status("rvx_embedding_backward_device", None, 0, None, 8, 8, 8, 1.0, 0, 9, None)
     assert st == 2 and "dtype" in msg
