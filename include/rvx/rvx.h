@@ -385,7 +385,7 @@ enum { RVX_DTYPE_F32 = 0, RVX_DTYPE_F16 = 1, RVX_DTYPE_BF16 = 2 };
 
 /* Rows of a learned table by id: out[i] = scale * table[ids[i]] for i < n, table [rows][dim] and
  * out [n][dim] of `dtype`, ids int64. An id outside [0, rows) is absent: its row of out is zeros.
- * rows < 2^31 - 1, n < 2^31, 1 <= dim <= 65536; out must not be the table. */
+ * rows < 2^31 - 1, n < 2^31, 1 <= dim <= 65536, scale finite; out must not be the table. */
 rvx_status rvx_embedding_forward_device(const rvx_buffer* table, int32_t dtype, int64_t rows, int32_t dim,
                                         const rvx_buffer* ids_i64, int64_t n, float scale, rvx_buffer* out);
 /* Its gradient: g[v] = scale * sum of grad_out[i] over the i with ids[i] = v, each sum in 32 bits
@@ -398,7 +398,8 @@ rvx_status rvx_embedding_backward_device(const rvx_buffer* grad_out, int32_t dty
                                          int32_t table_dtype, rvx_buffer* grad_table);
 
 /* Log probabilities of given ids over rows of scores, with entropy and the best alternatives:
- * scores [n][c] of `dtype`, row i at element i * ld (ld >= c), p = softmax(scores / temperature).
+ * scores [n][c] of `dtype`, row i at element i * ld (ld >= c), p = softmax(scores / temperature),
+ * temperature in [2^-100, 2^100].
  * Every output is nullable (= not wanted):
  *   logp    [n] f32    log p[targets[i]]; 0 where the target is outside [0, c) (no target)
  *   rank    [n] int64  how many ids are ranked before the target (higher score, or the same score
@@ -432,7 +433,10 @@ rvx_status rvx_log_probs_backward_device(const rvx_buffer* scores, int32_t dtype
  * W [out][in], bias [out], A_r [rank_r][in], B_r [out][rank_r], x [n][in], y [n][out], all row-major
  * of the layer's dtype; A_r x is kept in 32 bits. The layer copies weights and adapters into its
  * own layout, so their buffers may be freed after the call. A row whose id is outside
- * [0, max_adapters), or names a slot never set or set with rank 0, has no adapter. */
+ * [0, max_adapters), or names a slot never set or set with rank 0, has no adapter. An f32 layer
+ * takes more than 64 rows as pairs of f16 values, each row of x and W scaled by a power of two: a
+ * product x_j W_oj is then off by at most 3 2^-22 max|x| max|W_o|, and an infinity in x or W can
+ * make outputs NaN that are infinite otherwise. */
 typedef struct rvx_adapter_linear rvx_adapter_linear;
 typedef struct {
     int32_t in_features, out_features;  /* 1 .. 65536 */

@@ -290,7 +290,7 @@ __global__ __launch_bounds__(64 * WAVES) void shrink_kernel(const T* __restrict_
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
                                 hi[j] = (T)(v[r][j] * up);
-                                lo[j] = (T)(v[r][j] * up - (float)hi[j]);
+                                lo[j] = fabsf((float)hi[j]) < INFINITY ? (T)(v[r][j] * up - (float)hi[j]) : (T)0.0f;
                             }
                             const int64_t o = at * t.ld + r * 16 + (lane >> 4) * 4;
                             __builtin_memcpy(t.hi + o, hi, sizeof(hi));
@@ -480,7 +480,6 @@ __device__ __forceinline__ void wait_and_meet() {
 // none of the three units waits for the others' turns.
 template <int READS, int COPIES, int PRODUCTS>
 __device__ __forceinline__ void spread() {
-#ifndef NO_SPREAD
     constexpr int EACH = PRODUCTS / (READS + COPIES) > 0 ? PRODUCTS / (READS + COPIES) : 1;
 #pragma unroll
     for (int i = 0; i < COPIES; ++i) {
@@ -493,7 +492,6 @@ __device__ __forceinline__ void spread() {
         __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
     }
     __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS, 0);
-#endif
 }
 
 // P: the products' type; _Float16 with T = float: hi and lo fragments in turn, KF = 2.
@@ -664,7 +662,9 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const P* __restrict_
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int col = col0 + (j >> 1) * 32 + (j & 1) * 4 + r;
-                    acc[i][j][r] *= xi * (col < out ? w_inv[col] : 0.0f);
+                    // (the scales' product can be past the largest float where a sum is 0)
+                    const float wi = col < out ? w_inv[col] : 0.0f, s = xi * wi;
+                    acc[i][j][r] = s < INFINITY ? acc[i][j][r] * s : acc[i][j][r] * xi * wi;
                 }
         }
     }

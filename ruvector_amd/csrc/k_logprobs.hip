@@ -204,12 +204,16 @@ struct Part {  // what one block found of one row
     int before;
 };
 
+// (score - m) / T; halves, as the difference itself may be past the largest float
+__device__ __forceinline__ float gap(float score, float m, float inv_t) {
+    return 2.0f * ((0.5f * score - 0.5f * m) * inv_t);
+}
 __device__ __forceinline__ void write_row(const Stat& st, int before, int64_t row, float st_score, bool has_target,
                                           float inv_t, const LogProbsOut& out) {
     const bool empty = st.s == 0.0f;
     const float m = empty ? -INFINITY : st.m;
     const float log_sum = empty ? -INFINITY : logf(st.s);
-    if (out.logp) out.logp[row] = !has_target ? 0.0f : empty ? -INFINITY : (st_score - m) * inv_t - log_sum;
+    if (out.logp) out.logp[row] = !has_target ? 0.0f : empty ? -INFINITY : gap(st_score, m, inv_t) - log_sum;
     if (out.rank) out.rank[row] = has_target ? before : -1;
     if (out.entropy) out.entropy[row] = empty ? 0.0f : log_sum - LN2 * (st.e / st.s);
     if (out.stats) {
@@ -224,7 +228,7 @@ __device__ __forceinline__ void write_top(u64 list, int k, int64_t row, const St
     const bool none = list == 0;
     if (out.top_ids) out.top_ids[row * k + lane] = none ? -1 : (int64_t)(0xffffffffu - (uint32_t)list);
     if (out.top_logp)
-        out.top_logp[row * k + lane] = none ? -INFINITY : (key_score(list) - st.m) * inv_t - logf(st.s);
+        out.top_logp[row * k + lane] = none ? -INFINITY : gap(key_score(list), st.m, inv_t) - logf(st.s);
 }
 
 // ---------------------------------------------------------------- one pass
@@ -389,8 +393,8 @@ __device__ __forceinline__ Stat walk(const T* __restrict__ x, int64_t lo, int64_
     if constexpr (TOP)
         if (best.waiting) best.flush();
     Stat st;
-    if (s != 0.f) {  // to the reference m itself
-        const float d = fmaf(-m, c1, b), r = __builtin_amdgcn_exp2f(d);
+    if (s != 0.f) {  // to the reference m itself; d is large only below -far, where the lane adds nothing
+        const float d = fminf(fmaf(-m, c1, b), 100.0f), r = __builtin_amdgcn_exp2f(d);
         st.m = m;
         st.e = r * fmaf(s, d, e);
         st.s = s * r;

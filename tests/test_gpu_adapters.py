@@ -126,6 +126,38 @@ def test_f16_intermediate_past_the_type(n):
     assert_within(run(layer_of(m, 4, "f16"), x, ids), want, tol)
 
 
+@pytest.mark.parametrize("n", [7, 200])
+@pytest.mark.parametrize("size", [1e-30, 1e-18, 1e18, 1e30])
+def test_f32_of_any_size(n, size):
+    """Rows and weights of one size whose products stay in range; elsewhere exact zeros."""
+    inp, out = 80, 50
+    m = make(inp, out, n, [], "f32")
+    m["x"][:, 40:] = 0
+    m["x"] = m["x"].clamp(-1, 1) * size
+    m["w"] = m["w"].clamp(-1, 1) / size
+    m["w"][::2, :40] = 0                       # these outputs are 0: what they weigh is 0 in x
+    m["w"][::2, 40:] = torch.tensor(size).clamp(max=1e30)
+    got = run(layer_of(m, 8, "f32"), m["x"], None)
+    want, tol = reference(m, None, "f32")
+    assert (got[:, ::2] == 0).all()
+    # as halves: a product is off by 3 2^-22 of the two rows' largest values, 40 of them
+    most = m["x"].double().abs().amax(1)[:, None] * m["w"].double().abs().amax(1)
+    assert_within(got[:, 1::2], want[:, 1::2], (tol + 40 * 3 * 2.0 ** -22 * most)[:, 1::2])
+
+
+@pytest.mark.parametrize("n", [7, 200])
+def test_bf16_intermediate_infinite(n):
+    """A x past the largest float is infinite, and so is y, with B's sign."""
+    m = make(64, 40, n, [1], "bf16")
+    a, b, scale = m["adapters"][0]
+    m["adapters"] = [((a.abs() + 0.1) * 1e30, b.sign() + 0.5, scale)]
+    m["x"] = (m["x"].abs() + 0.1) * 1e30
+    m["w"] *= 0
+    m["ids"][:] = 0
+    got = run(layer_of(m, 1, "bf16"), m["x"], m["ids"]).float()
+    assert torch.equal(got, (math.inf * m["adapters"][0][1].float().T).expand(n, -1))
+
+
 def test_adapters_replaced_and_cleared():
     m = make(96, 80, 70, [8, 8], "f32")
     layer = layer_of(m, 8, "f32")

@@ -136,8 +136,8 @@ def test_ties_and_orders(dtype, shape, n, c, k):
     check(scores, targets, 1.0, k, dtype)
 
 
-@pytest.mark.parametrize("scale,temperature", [(1e5, 1.0), (1e8, 1.0), (1e20, 1e18), (1e30, 1.0), (3e38, 1e37), (1.0, 1e-7), (1e-30, 1e-31),
-                                               (1e3, 1e7), (10.0, 3e38)])
+@pytest.mark.parametrize("scale,temperature", [(1e5, 1.0), (1e8, 1.0), (1e20, 1e18), (1e30, 1.0), (3e38, 1.0), (3e38, 1e30), (1.0, 1e-7), (1e-28, 1e-29),
+                                               (1e3, 1e7), (10.0, 1e30), (1.0, 2.0 ** -100)])
 @pytest.mark.parametrize("c", [70, 9000])
 def test_scores_and_temperatures_of_any_size(scale, temperature, c):
     scores, targets = make(5, c, "f32", spread=1.0)
