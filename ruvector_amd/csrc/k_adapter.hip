@@ -799,6 +799,7 @@ void adapter_forward(const AdapterArgs& g) {
         }
         constexpr bool F32 = __is_same(T, float);
         auto tiles = [&](int64_t bm, int64_t bn) { return (n + bm - 1) / bm * ((s.out + bn - 1) / bn); };
+        auto rounds = [&](int64_t bm, int64_t bn) { return (tiles(bm, bn) + cus - 1) / cus; };
         const int64_t row_tiles = (n + 15) / 16;
         // without adapters one row tile is read as it is: its 16-row loads cost less than another launch
         T* packed = (F32 && !few) || (n <= 16 && !g.ids) ? nullptr : (T*)scratch_bytes("adapter_x", row_tiles * s.kt * 1024);
@@ -850,7 +851,9 @@ void adapter_forward(const AdapterArgs& g) {
                        dim3(64 * WM * WN), 0, (const P*)xp, x_inv, n, (const P*)wp, g.w_inv, frags, s.nt, bias, b, s.b_slot,
                        s.rk, g.ids, (const int32_t*)perm, g.slot, s.slots, t, s.out, tm, tn, y);
         };
+        constexpr integral_constant<int, 1> I1{};
         constexpr integral_constant<int, 2> I2{};
+        constexpr integral_constant<int, 3> I3{};
         constexpr integral_constant<int, 4> I4{};
         constexpr integral_constant<int, 64> I64{};
         constexpr integral_constant<int, 128> I128{};
@@ -862,13 +865,15 @@ void adapter_forward(const AdapterArgs& g) {
             auto* x_inv = (float*)(halves + bytes);
             RVX_LAUNCH("adapter_split", split_kernel<false>, dim3((unsigned)row_tiles), dim3(1024), 0, x, s.in, n,
                        (const int32_t*)perm, ktq, (_Float16*)halves, x_inv);
-            if (tiles(128, 128) >= cus) go(_Float16{}, halves, x_inv, g.w_split, 2 * ktq, I128, I128, I2, I2, I4, I2);
-            else go(_Float16{}, halves, x_inv, g.w_split, 2 * ktq, I64, I64, I2, I2, I4, I2);
+            if (tiles(128, 128) < cus) go(_Float16{}, halves, x_inv, g.w_split, 2 * ktq, I64, I64, I2, I2, I4, I2);
+            else if (7 * rounds(256, 128) <= 4 * rounds(128, 128))
+                go(_Float16{}, halves, x_inv, g.w_split, 2 * ktq, I256, I128, I4, I2, I3, I2);
+            else go(_Float16{}, halves, x_inv, g.w_split, 2 * ktq, I128, I128, I4, I2, I4, I2);
         } else {
-            if (tiles(256, 256) >= cus)
-                go(T{}, packed, nullptr, w, s.kt, I256, I256, I2, I4, I4, integral_constant<int, 1>{});
-            else if (tiles(128, 128) >= cus) go(T{}, packed, nullptr, w, s.kt, I128, I128, I2, I2, I4, I2);
-            else go(T{}, packed, nullptr, w, s.kt, I64, I64, I2, I2, I4, I2);
+            if (tiles(128, 128) < cus) go(T{}, packed, nullptr, w, s.kt, I64, I64, I2, I2, I4, I2);
+            else if (8 * tiles(256, 128) <= 5 * cus) go(T{}, packed, nullptr, w, s.kt, I128, I128, I4, I2, I4, I1);
+            else if (7 * rounds(256, 256) <= 4 * rounds(256, 128)) go(T{}, packed, nullptr, w, s.kt, I256, I256, I2, I4, I4, I1);
+            else go(T{}, packed, nullptr, w, s.kt, I256, I128, I4, I2, I4, I1);
         }
     });
 }

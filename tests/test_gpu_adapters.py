@@ -96,6 +96,17 @@ def test_large_tiles(dtype):
     assert_within(got, want, tol)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,out", [(4000, 4090), (1800, 4001), (1001, 4000), (3000, 2100)])
+@pytest.mark.parametrize("inp", [40, 200, 300])
+def test_every_tile(dtype, n, out, inp):
+    """Row and output counts of each of the tiles' sizes; sums of fewer stages than are in flight, and more."""
+    m = make(inp, out, n, [16, 40], dtype, bias=True)
+    got = run(layer_of(m, 40, dtype), m["x"], m["ids"])
+    want, tol = reference(m, m["ids"], dtype)
+    assert_within(got, want, tol)
+
+
 @pytest.mark.parametrize("n", [5, 300])
 def test_rows_do_not_depend_on_each_other(n):
     """An adapter, or a row, with infinities and NaN changes its own rows alone."""
