@@ -234,7 +234,7 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_move_kernel(const int64_t* 
 
 // Up to SMALL_SORT positions: one block sorts them in LDS, in one launch; the other blocks meanwhile
 // set `clear` (nullable) to zeros.
-constexpr int SMALL_SORT = 8192, SMALL_BITS = 9, SMALL_THREADS = 1024, SMALL_WAVES = SMALL_THREADS / 64;
+constexpr int SMALL_SORT = 6144, SMALL_BITS = 9, SMALL_THREADS = 1024, SMALL_WAVES = SMALL_THREADS / 64;
 
 __global__ __launch_bounds__(SMALL_THREADS) void sort_small_kernel(const int64_t* __restrict__ ids, int n, uint32_t rows,
                                                                   int passes, int bits, uint32_t* __restrict__ key_out,
@@ -394,25 +394,22 @@ struct Group {
     __device__ __forceinline__ bool long_last(uint32_t rows) const { return last < rows && trail > 0 && trail + goes >= LONG; }
 };
 
-// A 1 for every row that is looked up, from the first entry of each id's run.
-__global__ __launch_bounds__(256) void embed_mark_kernel(const uint32_t* __restrict__ key, int64_t n, uint32_t rows,
-                                                        unsigned char* __restrict__ present) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const uint32_t k = key[i];
-        if (k < rows && (i == 0 || key[i - 1] != k)) present[k] = 1;
-    }
-}
-
-// One wave per (group, slab): the group's parts of long runs.
+// One wave per (group, slab): the group's parts of long runs. present (nullable): a 1 for every row that is
+// looked up, from the first entry of its run.
 template <class T>
 __global__ __launch_bounds__(64) void embed_groups_kernel(const T* __restrict__ grad_out, int dim,
                                                          const uint32_t* __restrict__ key,
                                                          const uint32_t* __restrict__ pos, int64_t n, uint32_t rows,
-                                                         float* __restrict__ heads, float* __restrict__ tails) {
+                                                         float* __restrict__ heads, float* __restrict__ tails,
+                                                         unsigned char* __restrict__ present) {
     constexpr int N = Vec16<T>::N;
     const int64_t g = blockIdx.x;
     const int lane = threadIdx.x;
     const Group at(key, pos, n, g);
+    if (present && blockIdx.y == 0) {
+        const uint32_t left = __shfl_up(at.key, 1);
+        if (at.key < rows && (lane ? left != at.key : at.came == 0)) present[at.key] = 1;
+    }
     const int col = blockIdx.y * 64 * N + lane * N;
     auto sum = [&](int from, int count, float* out) {
         PackOf<float, N> acc[1] = {};
@@ -494,17 +491,43 @@ __global__ __launch_bounds__(64) void embed_long_kernel(int dim, const uint32_t*
     if (here.long_last(rows)) run(here.last, heads, here.goes > 0);
 }
 
+// The block-th of `blocks` blocks' share of the rows that are not marked: zeros.
+__device__ __forceinline__ void zero_rows(unsigned char* table, int64_t rows, int64_t row_bytes,
+                                          const unsigned char* __restrict__ present, int block, int blocks) {
+    const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+    const int64_t step = (int64_t)blocks * waves;
+    const uint4 z = {0, 0, 0, 0};
+    for (int64_t w = (int64_t)block * waves + (threadIdx.x >> 6); w * 64 < rows; w += step) {  // 64 rows a turn
+        unsigned long long absent = __ballot(w * 64 + lane < rows && !present[w * 64 + lane]);
+        while (absent) {
+            unsigned char* p = table + (w * 64 + __ffsll(absent) - 1) * row_bytes;
+            absent &= absent - 1;
+            int64_t b = (int64_t)lane * 16;
+            for (; b + 16 <= row_bytes; b += 64 * 16) __builtin_memcpy(p + b, &z, 16);
+            if (b < row_bytes)
+                for (; b < row_bytes; b += 2) *(uint16_t*)(p + b) = 0;
+        }
+    }
+}
+
 // One wave per (sorted entry, slab): the first entry of an id sums the id's run into its row. Bound
 // by HBM: a wave takes up to 4 vectors a lane, so that a row's bytes are all in flight at once.
-// UP: 4 times as many rows of a run in flight; costs occupancy.
+// UP: 4 times as many rows of a run in flight; costs occupancy. The first zero_blocks blocks set the
+// rows without an entry to zeros meanwhile.
 template <class T, class S, int V, bool UP>
 __global__ __launch_bounds__(256) void embed_rows_kernel(const T* __restrict__ grad_out, int dim, int64_t begin,
                                                         const uint32_t* __restrict__ key,
                                                         const uint32_t* __restrict__ pos, int64_t n, uint32_t rows,
-                                                        float scale, bool add, S* grad_table) {
+                                                        float scale, bool add, S* grad_table, int zero_blocks,
+                                                        const unsigned char* __restrict__ present) {
     constexpr int N = Vec16<T>::N;
     const int lane = threadIdx.x & 63;
-    const int64_t i0 = begin + (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if ((int)blockIdx.x < zero_blocks) {
+        if (blockIdx.y == 0)
+            zero_rows((unsigned char*)grad_table, rows, (int64_t)dim * (int64_t)sizeof(S), present, blockIdx.x, zero_blocks);
+        return;
+    }
+    const int64_t i0 = begin + (int64_t)(blockIdx.x - zero_blocks) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (i0 >= n) return;
     // one load gives the entry before, this one and the 62 after it
     const int64_t near_i = i0 + lane - 1;
@@ -526,62 +549,61 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const T* __restrict__ g
     finish_row<S, N, V>(row, acc, old, col, dim, scale);
 }
 
-// Few positions: no sort. The wave of position i looks for its id among the positions before it
-// (then another wave has the row) and adds the rows of the positions after it, in order.
-constexpr int SCAN_MAX = 1024;
+// Few positions: no sort. The block of position i and a slab of columns looks for its id among all
+// positions, 64 a wave and turn: before i (then another block has the row), and from i on, whose rows
+// each wave adds in order; the waves' sums are added in theirs.
+constexpr int SCAN_MAX = 1024, SCAN_WAVES = 4;
 
 template <class T, class S>
-__global__ __launch_bounds__(256) void embed_scan_kernel(const T* __restrict__ grad_out, int dim,
-                                                        const int64_t* __restrict__ ids, int n, int64_t rows,
-                                                        float scale, bool add, S* grad_table) {
+__global__ __launch_bounds__(64 * SCAN_WAVES) void embed_scan_kernel(const T* __restrict__ grad_out, int dim,
+                                                                    const int64_t* __restrict__ ids, int n, int64_t rows,
+                                                                    float scale, bool add, S* grad_table) {
     constexpr int N = Vec16<T>::N;
-    const int lane = threadIdx.x & 63;
-    const int i0 = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (i0 >= n) return;
+    __shared__ float sums[SCAN_WAVES][64 * N];
+    __shared__ int counts[SCAN_WAVES];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int i0 = blockIdx.x;
     const int64_t id = ids[i0];
     if (id < 0 || id >= rows) return;
-    for (int j = 0; j < i0; j += 64)
-        if (__any(j + lane < i0 && ids[j + lane] == id)) return;
-    const int col = blockIdx.y * 64 * N + lane * N;
-    S* const row = grad_table + id * dim;
-    PackOf<S, N> v[1] = {};
-    if (add) get_cols<S, N, 1>(row, v, col, dim);
-    PackOf<float, N> acc[1] = {};
-    for (int j = i0; j < n; j += 64) {
-        unsigned long long m = __ballot(j + lane < n && ids[j + lane] == id);
-        const int count = __popcll(m);
-        int mine = 0;  // lane r: the r-th position of the 64 with the id
-        for (int r = 0; r < count; ++r) {
-            const int b = __ffsll(m) - 1;
-            m &= m - 1;
-            if (lane == r) mine = j + b;
-        }
-        add_rows<4, T, N, 1>(acc, count, col, dim,
-                       [&](int r) { return grad_out + (int64_t)__builtin_amdgcn_readlane(mine, r) * dim; });
-    }
+    bool before = false;
+    for (int p = wave * 64 + lane; p < i0; p += 64 * SCAN_WAVES) before |= ids[p] == id;
+    if (__syncthreads_or(before)) return;
+    // a thread's columns of the sums (of the rows': lane * N ..)
+    constexpr int THREADS = 64 * SCAN_WAVES, OWN = (64 * N + THREADS - 1) / THREADS;
+    const int col0 = blockIdx.y * 64 * N;
+    S* const row = grad_table + id * dim + col0;
+    auto mine = [&](int q) { return (int)threadIdx.x + q * THREADS; };
+    auto there = [&](int q) { return mine(q) < 64 * N && col0 + mine(q) < dim; };
+    float old[OWN];  // does not wait for the sum
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[0][i] = (S)fmaf(acc[0][i], scale, (float)v[0][i]);
-    put_cols<S, N, 1>(row, v, col, dim);
+    for (int q = 0; q < OWN; ++q) old[q] = add && there(q) ? (float)row[mine(q)] : 0.0f;
+    PackOf<float, N> acc[1] = {};
+    int found = 0;
+    for (int j = wave * 64; j < n; j += 64 * SCAN_WAVES) {
+        const int p = j + lane;
+        const unsigned long long m = __ballot(p >= i0 && p < n && ids[p] == id);
+        const int count = __popcll(m);
+        if (!count) continue;
+        // lane r: the r-th of these positions
+        const int below = __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+        const int place = __builtin_amdgcn_ds_permute((m >> lane & 1 ? below : count + lane - below) * 4, p);
+        add_rows<16, T, N, 1>(acc, count, col0 + lane * N, dim,
+                              [&](int r) { return grad_out + (int64_t)__builtin_amdgcn_readlane(place, r) * dim; });
+        found += count;
+    }
+    if (found) __builtin_memcpy(&sums[wave][lane * N], &acc[0], sizeof(acc[0]));
+    if (lane == 0) counts[wave] = found;
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < OWN; ++q) {
+        if (!there(q)) continue;
+        float sum = 0.0f;
+        for (int w = 0; w < SCAN_WAVES; ++w)
+            if (counts[w]) sum += sums[w][mine(q)];
+        row[mine(q)] = (S)fmaf(sum, scale, old[q]);
+    }
 }
 
-// Every row that is not marked: zeros.
-__global__ __launch_bounds__(256) void embed_zero_rows_kernel(unsigned char* table, int64_t rows, int64_t row_bytes,
-                                                             const unsigned char* __restrict__ present) {
-    const int lane = threadIdx.x & 63;
-    const int64_t waves = (int64_t)gridDim.x * 4;
-    const uint4 z = {0, 0, 0, 0};
-    for (int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); w * 64 < rows; w += waves) {  // 64 rows a turn
-        unsigned long long absent = __ballot(w * 64 + lane < rows && !present[w * 64 + lane]);
-        while (absent) {
-            unsigned char* p = table + (w * 64 + __ffsll(absent) - 1) * row_bytes;
-            absent &= absent - 1;
-            int64_t b = (int64_t)lane * 16;
-            for (; b + 16 <= row_bytes; b += 64 * 16) __builtin_memcpy(p + b, &z, 16);
-            if (b < row_bytes)
-                for (; b < row_bytes; b += 2) *(uint16_t*)(p + b) = 0;
-        }
-    }
-}
 // The whole table: zeros.
 __global__ __launch_bounds__(256) void embed_zero_kernel(unsigned char* table, int64_t bytes) {
     zero_bytes(table, bytes, blockIdx.x, gridDim.x);
@@ -589,8 +611,6 @@ __global__ __launch_bounds__(256) void embed_zero_kernel(unsigned char* table, i
 
 }  // namespace
 
-constexpr int64_t ZERO_BESIDE_BYTES = (int64_t)32 << 20;
-constexpr int ZERO_BESIDE_BLOCKS = 2;
 
 void embedding_forward(int32_t dtype, const void* table, int64_t rows, int dim, const int64_t* ids, int64_t n,
                        float scale, void* out) {
@@ -628,7 +648,7 @@ void embedding_backward(int32_t dtype, const void* grad_out, const int64_t* ids,
             using S = decltype(s);
             const int slabs = (dim + 64 * Vec16<T>::N - 1) / (64 * Vec16<T>::N);
             RVX_LAUNCH("embedding_backward", (embed_scan_kernel<T, S>),
-                       dim3((unsigned)((n + 3) / 4), slabs), dim3(256), 0, (const T*)grad_out, dim, ids, (int)n,
+                       dim3((unsigned)n, slabs), dim3(64 * SCAN_WAVES), 0, (const T*)grad_out, dim, ids, (int)n,
                        rows, scale, accumulate, (S*)grad_table);
         });
         return;
@@ -642,15 +662,15 @@ void embedding_backward(int32_t dtype, const void* grad_out, const int64_t* ids,
     const int64_t groups = (n + GROUP - 1) / GROUP, span_count = n / (GROUP * GROUP);
     float* heads = scratch_f32("embed_partial", (2 * groups + span_count) * dim);
     float *tails = heads + groups * dim, *spans = tails + groups * dim;
-    // A small table's dense gradient is set to zeros before the sums; of a large one only the rows
-    // without an id, beside the sums.
-    const bool beside = !accumulate && table_bytes >= ZERO_BESIDE_BYTES;
+    // A dense gradient's other rows become zeros beside other work: of few positions the whole table
+    // beside the sort, by blocks that it leaves idle; of many, the rows without an id beside the sums.
+    const bool beside = !accumulate && n > SMALL_SORT;
     const int64_t words = (rows + 3) / 4;
     auto* present = beside ? (uint32_t*)scratch_bytes("embed_present", words * 4) : nullptr;  // a byte a row
     if (n <= SMALL_SORT) {
         const int passes = (key_bits + SMALL_BITS - 1) / SMALL_BITS, bits = (key_bits + passes - 1) / passes;
-        unsigned char* clear = beside ? (unsigned char*)present : accumulate ? nullptr : (unsigned char*)grad_table;
-        const int64_t bytes = beside ? words * 4 : accumulate ? 0 : table_bytes;
+        unsigned char* clear = accumulate ? nullptr : (unsigned char*)grad_table;
+        const int64_t bytes = accumulate ? 0 : table_bytes;
         const int64_t blocks = std::min<int64_t>((bytes + 16383) / 16384, 2LL * device().num_cus);
         RVX_LAUNCH("embedding_sort", sort_small_kernel, dim3((unsigned)(1 + blocks)), dim3(SMALL_THREADS), 0, ids, (int)n,
                    (uint32_t)rows, passes, bits, key[0], pos[0], clear, bytes);
@@ -680,30 +700,15 @@ void embedding_backward(int32_t dtype, const void* grad_out, const int64_t* ids,
             }
         }
         sk = key[(passes + 1) & 1], sp = pos[(passes + 1) & 1];
-        if (!accumulate && !beside) zero_table();
     }
-    hipEvent_t zeroed = nullptr;
-    if (beside) {  // on a second stream: the two write different rows
-        RVX_LAUNCH("embedding_mark", embed_mark_kernel,
-                   dim3((unsigned)std::min<int64_t>((n + 255) / 256, 4LL * device().num_cus)), dim3(256), 0, sk, n,
-                   (uint32_t)rows, (unsigned char*)present);
-        hipEvent_t* ev = pipeline_events(2);
-        RVX_HIP(hipEventRecord(ev[0], stream()));
-        RVX_HIP(hipStreamWaitEvent(device().aux, ev[0], 0));
-        StreamScope on(device().aux);
-        const int64_t blocks = std::min<int64_t>((rows + 255) / 256, (int64_t)ZERO_BESIDE_BLOCKS * device().num_cus);
-        RVX_LAUNCH("embedding_zero", embed_zero_rows_kernel, dim3((unsigned)blocks), dim3(256), 0, (unsigned char*)grad_table,
-                   rows, table_bytes / rows, (const unsigned char*)present);
-        zeroed = ev[1];
-        RVX_HIP(hipEventRecord(zeroed, device().aux));
-    }
+    const int zero_blocks = beside ? (int)std::min<int64_t>((rows + 255) / 256, (int64_t)device().num_cus) : 0;
     typed([&](auto t, auto s) {
         using T = decltype(t);
         using S = decltype(s);
         constexpr int N = Vec16<T>::N;
         const int vecs = (dim + 64 * N - 1) / (64 * N);  // vectors a lane for a whole row
         RVX_LAUNCH("embedding_groups", embed_groups_kernel<T>, dim3((unsigned)groups, vecs), dim3(64), 0, (const T*)grad_out,
-                   dim, sk, sp, n, (uint32_t)rows, heads, tails);
+                   dim, sk, sp, n, (uint32_t)rows, heads, tails, (unsigned char*)present);
         if (span_count > 1)
             RVX_LAUNCH("embedding_long", embed_spans_kernel, dim3((unsigned)((span_count + 3) / 4), (dim + 255) / 256),
                        dim3(256), 0, (const float*)tails, dim, sk, span_count, (uint32_t)rows, spans);
@@ -713,10 +718,13 @@ void embedding_backward(int32_t dtype, const void* grad_out, const int64_t* ids,
         const int slabs = (vecs + 3) / 4, per = (vecs + slabs - 1) / slabs;
         auto go = [&](auto v, auto up) {
             constexpr int64_t SLICE = (int64_t)1 << 24;  // entries of one launch: at most 2^30 threads
-            for (int64_t i = 0; i < n; i += SLICE)
+            for (int64_t i = 0; i < n; i += SLICE) {
+                const int zeros = i ? 0 : zero_blocks;
                 RVX_LAUNCH("embedding_backward", (embed_rows_kernel<T, S, decltype(v)::value, decltype(up)::value>),
-                           dim3((unsigned)((std::min(SLICE, n - i) + 3) / 4), slabs), dim3(256), 0, (const T*)grad_out, dim, i,
-                           sk, sp, n, (uint32_t)rows, scale, accumulate, (S*)grad_table);
+                           dim3((unsigned)((std::min(SLICE, n - i) + 3) / 4 + zeros), slabs), dim3(256), 0, (const T*)grad_out,
+                           dim, i, sk, sp, n, (uint32_t)rows, scale, accumulate, (S*)grad_table, zeros,
+                           (const unsigned char*)present);
+            }
         };
         auto by_width = [&](auto up) {
         if (per == 1) go(std::integral_constant<int, 1>{}, up);
@@ -728,7 +736,6 @@ void embedding_backward(int32_t dtype, const void* grad_out, const int64_t* ids,
         if (n * slabs <= 32LL * device().num_cus) by_width(std::true_type{});
         else by_width(std::false_type{});
     });
-    if (zeroed) RVX_HIP(hipStreamWaitEvent(stream(), zeroed, 0));
 }
 
 }  // namespace rvx

@@ -608,7 +608,7 @@ void log_probs(int32_t dtype, const void* scores, int64_t n, int64_t c, int64_t 
         const int cus = device().num_cus;
         const int64_t steps = (c + STEP - 1) / STEP;
         const bool by_wave = n >= 8LL * cus || steps == 1;
-        int64_t splits = std::max<int64_t>(1, std::min<int64_t>((4LL * cus + n - 1) / n, (steps + LP_WAVES - 1) / LP_WAVES));
+        int64_t splits = n >= cus ? 1 : std::min<int64_t>((2LL * cus + n - 1) / n, (steps + LP_WAVES - 1) / LP_WAVES);
         const int64_t seg = (steps + splits * LP_WAVES - 1) / (splits * LP_WAVES) * STEP;
         splits = by_wave ? 1 : (c + seg * LP_WAVES - 1) / (seg * LP_WAVES);
         Part* parts = nullptr;
