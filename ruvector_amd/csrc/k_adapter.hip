@@ -10,7 +10,8 @@
 // wave loads a fragment with one coalesced instruction, copies it to LDS as it is, and reads it
 // back without bank conflicts. Weights are laid out when they are set, x by the launch that computes
 // t, which reads it anyway: a CU takes 75 to 110 bytes a ns from L2 in whole KiB, but only 35 where
-// each load gathers 16 rows, and the projection reads x many times. W and B are the first operand, x and t the second, so that a lane
+// each load gathers 16 rows, and the projection reads x many times (bf16 4096 x 4096, 8192 rows: 299 us
+// with x read as it lies, 256 so). W and B are the first operand, x and t the second, so that a lane
 // holds 4 outputs of one row; the 32 outputs of two neighbouring fragments are interleaved by 4
 // (`out_of`), so that the two give it 8 neighbouring outputs. Along `in`, two neighbouring fragments
 // are interleaved by pieces (`in_of`): a row's two pieces of one lane are neighbours, and the loads of
@@ -97,7 +98,8 @@ __device__ __forceinline__ int adapter_of(const int32_t* ids, const AdapterSlot*
 
 // ---------------------------------------------------------------- grouping rows
 // perm: GROUP_ROWS rows at a time, a block each, in the order of their adapters (adapters that agree
-// modulo GROUP_BINS - 1 may mix: the order is for speed alone).
+// modulo GROUP_BINS - 1 may mix: the order is for speed alone). f16 2048 x 2048, rank 64, 2000 rows of 32
+// adapters in turn: 517 us without, 67 with it at the time.
 constexpr int GROUP_THREADS = 1024, GROUP_ROWS = 2 * GROUP_THREADS, GROUP_BITS = 9, GROUP_BINS = 1 << GROUP_BITS;
 
 __global__ __launch_bounds__(GROUP_THREADS) void group_rows_kernel(const int32_t* __restrict__ ids, int64_t n,
@@ -180,17 +182,20 @@ __device__ __forceinline__ typename Mma<T>::V row_piece(const T* row, int c, int
     return v;
 }
 
+// Bound by the latency of its loads where rows are few: bf16 4096 x 4096, 64 rows: 26.5 us for the layer
+// with one block a row tile, 22.8 with the sum in FEW_PARTS parts; by HBM where they are many.
 // A block: 16 rows (of the permutation), the waves split the sum over `in`. Lays the rows out in
 // fragment order (PACK) and computes t for them: the block's y-th, (y + gridDim.y)-th .. different
 // adapter is its work; RT == 0: no adapters.
-template <class T, int RT, int WAVES, bool SPLIT, bool PACK>
-__global__ __launch_bounds__(64 * WAVES) void shrink_kernel(const T* __restrict__ x, int in, int64_t n,
+constexpr int SHRINK_WAVES = 8;
+template <class T, int RT, bool SPLIT, bool PACK>
+__global__ __launch_bounds__(64 * SHRINK_WAVES) void shrink_kernel(const T* __restrict__ x, int in, int64_t n,
                                                            const int32_t* __restrict__ perm, const T* __restrict__ a,
                                                            int64_t a_slot, int kt, const int32_t* __restrict__ ids,
                                                            const AdapterSlot* __restrict__ slot, int slots, Mid<T> t,
                                                            T* __restrict__ packed) {
     using V = typename Mma<T>::V;
-    constexpr int N = PIECE<T>, R = RT ? RT : 1;
+    constexpr int N = PIECE<T>, R = RT ? RT : 1, WAVES = SHRINK_WAVES;
     __shared__ f32x4 red[RT ? WAVES : 1][R][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t row0 = (int64_t)blockIdx.x * 16;
@@ -315,7 +320,7 @@ __global__ __launch_bounds__(64 * WAVES) void shrink_kernel(const T* __restrict_
 // of x and of W is scaled by a power of two to a largest value in [2^14, 2^15) and split into hi + lo,
 // 22 bits of the row's largest values and 2^-39 of them at least of the others, and three products
 // hi hi + hi lo + lo hi give x w within about 2^-22. Fragment q of hi lies beside that of lo. inv: 1 /
-// scale. One wave a row.
+// scale. One wave a row. 4096 x 4096, 2048 rows: 588 us with the f32 instructions, 206 so.
 template <bool WEIGHT>
 __global__ __launch_bounds__(1024) void split_kernel(const float* __restrict__ x, int in, int64_t rows,
                                                     const int32_t* __restrict__ perm, int ktq,
@@ -364,7 +369,9 @@ __global__ __launch_bounds__(1024) void split_kernel(const float* __restrict__ x
 
 // ---------------------------------------------------------------- few rows
 // A block: a fragment tile's 16 outputs for all (<= 16 MT) rows; its waves split the sum and join in
-// LDS. Bound by reading W once.
+// LDS. Bound by reading W once: bf16 4096 x 4096 10 us for 1 row, 14 for 16, 20.6 for 64, with t.
+// As tiles (below): 33 rows 37 us to 19 here, 64 rows 36 to 21; f32 73 to 37; bf16 768 x
+// 768, 64 rows 17 to 11.5.
 constexpr int FEW_WAVES = 16;
 
 // MT == 0: one row tile, x row-major.
@@ -453,8 +460,12 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_rows_kernel(const T* __res
 // KF == 1, large tiles: while a stage is multiplied from registers, the next one is read into others.
 // Behind a stage's one barrier everybody has read it, so its place is free for stage s + NS, and has
 // the next: the copies of NS - 2 stages more may still be on their way, which hides their latency.
-// KF > 1, small tiles: a fragment is a few products only, so a barrier serves KF of them; behind it
+// KF > 1, small tiles and halves: a fragment is a few products only, so a barrier serves KF of them; behind it
 // stage s has arrived and s - 1 is read, whose place the copies of s + NS - 1 take.
+// Bound by LDS, which takes the copies and gives each fragment to WN or WM waves: about 200 bytes a ns
+// of both whatever the tile; larger tiles need fewer for a product. Waves count too: a wave's copies
+// go out about 100 ns apart, so the tiles of four waves of 64 x 64 and 128 x 64 were half as fast as of eight
+// (bf16 4096 x 4096, 2048 rows: 110 and 107 us, 82 and 80 with eight).
 template <int BM, int BN, int WM, int WN, int NS, int KF>
 struct TileCfg {
     static constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
@@ -777,7 +788,7 @@ void adapter_forward(const AdapterArgs& g) {
         T* y = (T*)g.y;
         const int64_t n = g.n;
         const int cus = device().num_cus;
-        const bool few = n <= 64;
+        const bool few = n <= 64;  // (as far as the registers of one block's rows go; figures at the kernel)
         Mid<T> t{};
         int32_t* perm = nullptr;
         if (g.ids) {
@@ -806,28 +817,24 @@ void adapter_forward(const AdapterArgs& g) {
         // few row tiles: several blocks each, for the turns of different adapters and parts of the sum
         const unsigned spare = (unsigned)std::max<int64_t>(1, std::min<int64_t>(16, 2 * cus / row_tiles));
         const unsigned turns = g.ids ? few ? 16 : spare : 1, sums = few ? FEW_PARTS : g.ids ? 1 : std::min(spare, 4u);
-        auto shrink = [&](auto rt, auto waves, auto split, auto pack) {
-            constexpr int RT = decltype(rt)::value, W = decltype(waves)::value;
-            RVX_LAUNCH("adapter_shrink", (shrink_kernel<T, RT, W, decltype(split)::value, decltype(pack)::value>),
-                       dim3((unsigned)row_tiles, turns, sums), dim3(64 * W), 0, x, s.in, n, (const int32_t*)perm,
+        auto shrink = [&](auto rt, auto split, auto pack) {
+            constexpr int RT = decltype(rt)::value;
+            RVX_LAUNCH("adapter_shrink", (shrink_kernel<T, RT, decltype(split)::value, decltype(pack)::value>),
+                       dim3((unsigned)row_tiles, turns, sums), dim3(64 * SHRINK_WAVES), 0, x, s.in, n, (const int32_t*)perm,
                        (const T*)g.a, s.a_slot, s.kt, g.ids, g.slot, s.slots, t, packed);
         };
-        auto by_rank = [&](auto waves, auto split, auto pack) {
-            if (!g.ids) shrink(integral_constant<int, 0>{}, waves, split, std::true_type{});
-            else if (s.rt == 1) shrink(integral_constant<int, 1>{}, waves, split, pack);
-            else if (s.rt == 2) shrink(integral_constant<int, 2>{}, waves, split, pack);
-            else if (s.rt == 4) shrink(integral_constant<int, 4>{}, waves, split, pack);
-            else shrink(integral_constant<int, 8>{}, integral_constant<int, 8>{}, split, pack);
+        auto by_rank = [&](auto split, auto pack) {
+            if (!g.ids) shrink(integral_constant<int, 0>{}, split, std::true_type{});
+            else if (s.rt == 1) shrink(integral_constant<int, 1>{}, split, pack);
+            else if (s.rt == 2) shrink(integral_constant<int, 2>{}, split, pack);
+            else if (s.rt == 4) shrink(integral_constant<int, 4>{}, split, pack);
+            else shrink(integral_constant<int, 8>{}, split, pack);
         };
         if (few) {
-            if (packed) by_rank(integral_constant<int, 8>{}, std::false_type{}, std::true_type{});
+            if (packed) by_rank(std::false_type{}, std::true_type{});
         } else {
-            auto many = [&](auto waves) {
-                if (packed) by_rank(waves, std::true_type{}, std::true_type{});
-                else if (g.ids) by_rank(waves, std::true_type{}, std::false_type{});
-            };
-            if (row_tiles < cus) many(integral_constant<int, 16>{});
-            else many(integral_constant<int, 8>{});
+            if (packed) by_rank(std::true_type{}, std::true_type{});
+            else if (g.ids) by_rank(std::true_type{}, std::false_type{});
         }
         if (few) {
             auto go = [&](auto mt) {
@@ -865,11 +872,18 @@ void adapter_forward(const AdapterArgs& g) {
             auto* x_inv = (float*)(halves + bytes);
             RVX_LAUNCH("adapter_split", split_kernel<false>, dim3((unsigned)row_tiles), dim3(1024), 0, x, s.in, n,
                        (const int32_t*)perm, ktq, (_Float16*)halves, x_inv);
+            // whole layer, 4096 x 4096: 512 rows 91 us by 64 x 64, 115 by 128 x 128; 1024: 149, 131 and 174 by
+            // 256 x 128; 2048: 263, 228, 206; 4096: 525, 433, 390. A round of the larger tiles takes 7 / 4 of one of the
+            // smaller.
             if (tiles(128, 128) < cus) go(_Float16{}, halves, x_inv, g.w_split, 2 * ktq, I64, I64, I2, I2, I4, I2);
             else if (7 * rounds(256, 128) <= 4 * rounds(128, 128))
                 go(_Float16{}, halves, x_inv, g.w_split, 2 * ktq, I256, I128, I4, I2, I3, I2);
             else go(_Float16{}, halves, x_inv, g.w_split, 2 * ktq, I128, I128, I4, I2, I4, I2);
         } else {
+            // whole layer, bf16 4096 x 4096: 512 rows 43 us by 64 x 64, 48 by 128 x 128, 66 by 256 x 128, 106 by 256
+            // x 256; 1024: 69, 53, 67, 106; 2048: 120, 83, 79, 109; 4096: 227, 152, 149, 135; 8192: 432, 286, 280, 253.
+            // A round of the largest takes 7 / 4 of one of 256 x 128; two tiles of 128 x 128 on a CU as long as one
+            // of these.
             if (tiles(128, 128) < cus) go(T{}, packed, nullptr, w, s.kt, I64, I64, I2, I2, I4, I2);
             else if (8 * tiles(256, 128) <= 5 * cus) go(T{}, packed, nullptr, w, s.kt, I128, I128, I4, I2, I4, I1);
             else if (7 * rounds(256, 256) <= 4 * rounds(256, 128)) go(T{}, packed, nullptr, w, s.kt, I256, I256, I2, I4, I4, I1);

@@ -2,8 +2,10 @@
 //
 // Forward: out[i] = scale * table[id_i]; one read and one write of each row, bound by HBM.
 // Backward: g[v] = scale * sum_{i: id_i = v} dy[i]. The positions are grouped by id with a stable
-// radix sort of (id, i), so a row's sum runs over i in ascending order whatever ran when: no
-// floating-point atomics, the same bits every call.
+// radix sort of (id, i) and summed in an order that depends on the ids alone: no floating-point
+// atomics, the same bits every call. Sums in 32 bits, rounded once to the table's type. It cannot do
+// without reading dy and writing the rows; the sort (key and position, 8 bytes, a pass) and its
+// launches are what comes on top.
 #include "heads.hpp"
 
 namespace rvx {
@@ -40,7 +42,10 @@ __device__ __forceinline__ PackOf<S, N> get_vec(const S* row, int c, int dim) {
 }
 
 // ---------------------------------------------------------------- forward
-constexpr int EF_U = 4;  // 16-byte chunks per lane
+// A lane: EF_U 16-byte chunks of the output as one array, 256 chunks apart, so that short rows fill
+// waves too and all loads go out before the first is used. bf16 1000000 x 768, 131072 ids: 78 to 81 us, 5
+// TB/s read and written (a large copy: 4.7); 64 f32 rows of 128: 4.3 us, a launch.
+constexpr int EF_U = 4;
 
 template <class T>
 __global__ __launch_bounds__(256) void embed_forward_kernel(const T* __restrict__ table, int64_t rows, int dim, int cpr,
@@ -87,7 +92,10 @@ __global__ __launch_bounds__(256) void embed_forward_kernel(const T* __restrict_
 // Stable LSD radix sort of (key, position), key = id, or `rows` for an absent id. The n positions
 // are cut into at most SORT_TILES tiles, one block each. A pass is two launches: every tile counts
 // its digits in LDS, then moves its elements; for that each block sums the counts of the tiles
-// before it by itself, which costs less than a launch for a scan.
+// before it by itself, which costs less than a launch for a scan. Bound by the latency of 64 blocks'
+// steps: 100003 positions of 500009 rows, two passes of 10 bits, 31 us (counting by atomics in memory
+// instead of LDS: three times that where ids are as frequent as words). Digits of at most 11 bits:
+// 8 waves' counters of 2^11 fit LDS.
 constexpr int SORT_TILES = 64, SORT_THREADS = 512, SORT_WAVES = SORT_THREADS / 64, SORT_STEP = SORT_THREADS * 4;
 constexpr int SORT_MAX_BITS = 11, SORT_BINS = 1 << SORT_MAX_BITS;
 
@@ -233,7 +241,8 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_move_kernel(const int64_t* 
 }
 
 // Up to SMALL_SORT positions: one block sorts them in LDS, in one launch; the other blocks meanwhile
-// set `clear` (nullable) to zeros.
+// set `clear` (nullable) to zeros. Against the passes over tiles, whole gradient f32 of 100000 x 128: 17
+// us to 23 at 2000 positions, 25.4 to 26.6 at 6144, 32 to 30 at 8192.
 constexpr int SMALL_SORT = 6144, SMALL_BITS = 9, SMALL_THREADS = 1024, SMALL_WAVES = SMALL_THREADS / 64;
 
 __global__ __launch_bounds__(SMALL_THREADS) void sort_small_kernel(const int64_t* __restrict__ ids, int n, uint32_t rows,
@@ -322,7 +331,8 @@ __global__ __launch_bounds__(SMALL_THREADS) void sort_small_kernel(const int64_t
 // entries: a group's part of its first key's run (`tails`) and of its last key's (`heads`, where
 // that is another key) are summed by a wave of their own, GROUP whole tails of one run once more
 // (`spans`), and the wave of the run's first group adds these. (A run of LONG entries touches an end
-// of its group.) Groups and order depend on the sorted ids alone.
+// of its group.) Groups and order depend on the sorted ids alone. Ids as frequent as words, bf16 65536
+// x 1024: the rows kernel alone, one wave for the most frequent id, took 311 us of a gradient that takes 183.
 constexpr int GROUP = 64, LONG = 63;
 
 // A wave's columns of a row: V vectors of N columns a lane, vector q at (q * 64 + lane) * N.
@@ -511,10 +521,12 @@ __device__ __forceinline__ void zero_rows(unsigned char* table, int64_t rows, in
 }
 
 // One wave per (sorted entry, slab): the first entry of an id sums the id's run into its row. Bound
-// by HBM: a wave takes up to 4 vectors a lane, so that a row's bytes are all in flight at once.
-// UP: 4 times as many rows of a run in flight; costs occupancy. The first zero_blocks blocks set the
-// rows without an entry to zeros meanwhile.
-template <class T, class S, int V, bool UP>
+// by HBM: a wave takes up to 4 vectors a lane, so that a row's bytes are all in flight at once; f32
+// 500009 x 768, 100003 ids, added to the table: 4.9 TB/s. The first zero_blocks blocks set the
+// rows without an entry to zeros meanwhile: bf16 262144 x 1024, 65536 ids: 167 us, 181 with these in a
+// launch on a second stream; bf16 512 columns, 20000 ids, a table of 512 MB: 129 us, 148 and, with the whole
+// table cleared before, 154; of 64 MB: 41, 63 and 49.
+template <class T, class S, int V>
 __global__ __launch_bounds__(256) void embed_rows_kernel(const T* __restrict__ grad_out, int dim, int64_t begin,
                                                         const uint32_t* __restrict__ key,
                                                         const uint32_t* __restrict__ pos, int64_t n, uint32_t rows,
@@ -543,7 +555,7 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const T* __restrict__ g
     PackOf<S, N> old[V] = {};
     if (add) get_cols<S, N, V>(row, old, col, dim);  // does not wait for the sum
     PackOf<float, N> acc[V] = {};
-    add_rows<(V == 1 ? 8 : V == 2 ? 4 : 2) * (UP ? 4 : 1), T, N, V>(acc, run, col, dim, [&](int j) {
+    add_rows<(V == 1 ? 8 : V == 2 ? 4 : 2), T, N, V>(acc, run, col, dim, [&](int j) {
         return grad_out + (int64_t)(uint32_t)__builtin_amdgcn_readlane(near_pos, j + 1) * dim;
     });
     finish_row<S, N, V>(row, acc, old, col, dim, scale);
@@ -551,7 +563,9 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const T* __restrict__ g
 
 // Few positions: no sort. The block of position i and a slab of columns looks for its id among all
 // positions, 64 a wave and turn: before i (then another block has the row), and from i on, whose rows
-// each wave adds in order; the waves' sums are added in theirs.
+// each wave adds in order; the waves' sums are added in theirs. Against the sort: bf16 of 1024 columns,
+// 1000 positions: 7.7 us to 13.6 (20000 ids), 6.3 to 15.6 (40 ids), 28 to 18 (one id); 2000: 16.3 to
+// 15.4. Eight waves a block: 11.3, 6.1 and 20.7 us at 1000; one: 6.4, 11.7 and 137.
 constexpr int SCAN_MAX = 1024, SCAN_WAVES = 4;
 
 template <class T, class S>
@@ -716,25 +730,20 @@ void embedding_backward(int32_t dtype, const void* grad_out, const int64_t* ids,
                    (uint32_t)rows, (const float*)heads, (const float*)tails, (const float*)spans, scale, accumulate,
                    (S*)grad_table);
         const int slabs = (vecs + 3) / 4, per = (vecs + slabs - 1) / slabs;
-        auto go = [&](auto v, auto up) {
+        auto go = [&](auto v) {
             constexpr int64_t SLICE = (int64_t)1 << 24;  // entries of one launch: at most 2^30 threads
             for (int64_t i = 0; i < n; i += SLICE) {
                 const int zeros = i ? 0 : zero_blocks;
-                RVX_LAUNCH("embedding_backward", (embed_rows_kernel<T, S, decltype(v)::value, decltype(up)::value>),
+                RVX_LAUNCH("embedding_backward", (embed_rows_kernel<T, S, decltype(v)::value>),
                            dim3((unsigned)((std::min(SLICE, n - i) + 3) / 4 + zeros), slabs), dim3(256), 0, (const T*)grad_out,
                            dim, i, sk, sp, n, (uint32_t)rows, scale, accumulate, (S*)grad_table, zeros,
                            (const unsigned char*)present);
             }
         };
-        auto by_width = [&](auto up) {
-        if (per == 1) go(std::integral_constant<int, 1>{}, up);
-        else if (per == 2) go(std::integral_constant<int, 2>{}, up);
-        else if (per == 3) go(std::integral_constant<int, 3>{}, up);
-        else go(std::integral_constant<int, 4>{}, up);
-        };
-        // few waves: the latency of long runs counts, else the waves that hide it do
-        if (n * slabs <= 32LL * device().num_cus) by_width(std::true_type{});
-        else by_width(std::false_type{});
+        if (per == 1) go(std::integral_constant<int, 1>{});
+        else if (per == 2) go(std::integral_constant<int, 2>{});
+        else if (per == 3) go(std::integral_constant<int, 3>{});
+        else go(std::integral_constant<int, 4>{});
     });
 }
 
