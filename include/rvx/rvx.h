@@ -71,7 +71,8 @@ rvx_status rvx_synchronize(void);
 /* Order the library's work on the current device against another stream's (a hipStream_t of the
  * same device; NULL = the default stream), without waiting on the host: after
  * rvx_stream_wait(s) the library's later work waits for what is queued on s; after
- * rvx_stream_signal(s) later work on s waits for what the library has queued. */
+ * rvx_stream_signal(s) later work on s waits for what the library has queued. Refused for a stream
+ * that is being captured into a graph: the library's work is not recorded there. */
 rvx_status rvx_stream_wait(void* stream);
 rvx_status rvx_stream_signal(void* stream);
 /* Free the per-device scratch pool (pipeline chunk buffers, scan images, ...) that compute

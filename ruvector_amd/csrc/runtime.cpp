@@ -281,15 +281,23 @@ static void stream_order(hipStream_t first, hipStream_t then) {
     hipEventDestroy(e);  // the queued wait keeps what it needs
     RVX_HIP(st);
 }
+static void check_not_captured(hipStream_t s) {
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    RVX_HIP(hipStreamIsCapturing(s, &st));
+    RVX_REQUIRE(st == hipStreamCaptureStatusNone, RVX_ERR_INVALID_PARAMETER,
+                "the stream is being captured into a graph: the library's work is not recorded there");
+}
 rvx_status rvx_stream_wait(void* s) {
     return guard([&] {
         const hipStream_t mine = stream();
+        check_not_captured((hipStream_t)s);
         stream_order((hipStream_t)s, mine);
     });
 }
 rvx_status rvx_stream_signal(void* s) {
     return guard([&] {
         const hipStream_t mine = stream();
+        check_not_captured((hipStream_t)s);
         stream_order(mine, (hipStream_t)s);
     });
 }

@@ -178,6 +178,18 @@ for step in range(3):
         rv.embedding_forward_device(table, rows, dim, ids, n, out, scale=2.0)
         rv.stream_signal(side.cuda_stream)
         assert torch.equal(o, t[i] * 2), step
+graph, seven = torch.cuda.CUDAGraph(), torch.zeros(4, device="cuda")
+with torch.cuda.graph(graph):
+    seven += 7
+    for order in (rv.stream_wait, rv.stream_signal):
+        try:
+            order(torch.cuda.current_stream().cuda_stream)
+            raise SystemExit("a stream being captured was taken")
+        except rv.RvxError as e:
+            assert "captured" in str(e), e
+graph.replay()                              # the capture went on undisturbed
+graph.replay()
+assert seven.tolist() == [14.0] * 4
 b.free()
 del b
 gc.collect()
