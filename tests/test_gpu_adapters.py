@@ -87,7 +87,7 @@ def test_forward(dtype, inp, out, n, ranks, max_rank):
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_large_tiles(dtype):
-    """The largest tile: 16 x 17 tiles of 256 rows and columns, with edges."""
+    """Rounds of large tiles with edges, requests of many rows."""
     m = make(64, 4200, 4200, [16, 4, 9], dtype)
     layer = layer_of(m, 16, dtype)
     ids = torch.repeat_interleave(torch.tensor([0, -1, 2, 1, 3, 0, 2]), 600).to(torch.int32)  # requests of 600 rows
