@@ -673,9 +673,12 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const P* __restrict_
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int col = col0 + (j >> 1) * 32 + (j & 1) * 4 + r;
-                    // (the scales' product can be past the largest float where a sum is 0)
+                    // The scales' product can be past the largest float or below the smallest normal one where
+                    // the result is neither: then one after the other, the larger first (a sum is 0 or in
+                    // [2^-48, 2^46], so the first product is in range unless the result is past it too).
                     const float wi = col < out ? w_inv[col] : 0.0f, s = xi * wi;
-                    acc[i][j][r] = s < INFINITY ? acc[i][j][r] * s : acc[i][j][r] * xi * wi;
+                    const bool normal = s >= 0x1p-126f && s < INFINITY;
+                    acc[i][j][r] = normal ? acc[i][j][r] * s : acc[i][j][r] * fmaxf(xi, wi) * fminf(xi, wi);
                 }
         }
     }
