@@ -90,6 +90,9 @@ rvx_status rvx_buffer_free(rvx_buffer* buf);
 /* A DLManagedTensor (DLPack) over the whole buffer: one dimension of bytes, no copy. The memory
  * lives until both the handle is freed and the tensor's deleter has run. */
 rvx_status rvx_buffer_tensor(rvx_buffer* buf, void** out);
+/* The same over a copy of the buffer (on the current device), which the library's later work and
+ * streams ordered behind it by rvx_stream_signal may read; the tensor alone holds the copy. */
+rvx_status rvx_buffer_copy_tensor(const rvx_buffer* buf, void** out);
 int64_t    rvx_buffer_bytes(const rvx_buffer* buf);
 void*      rvx_buffer_device_ptr(rvx_buffer* buf);
 rvx_status rvx_buffer_upload(rvx_buffer* buf, const void* src, int64_t bytes, int64_t offset);

@@ -104,6 +104,7 @@ SIGNATURES = {
     "rvx_buffer_alloc": (None, [I64, PP]),
     "rvx_buffer_free": (None, [P]),
     "rvx_buffer_tensor": (None, [P, PP]),
+    "rvx_buffer_copy_tensor": (None, [P, PP]),
     "rvx_buffer_bytes": (I64, [P]),
     "rvx_buffer_device_ptr": (P, [P]),
     "rvx_buffer_upload": (None, [P, P, I64, I64]),

@@ -223,6 +223,13 @@ void release_tensor(ManagedTensor* t) {
     let_go(b->of);
     delete b;
 }
+ManagedTensor* tensor_of(rvx_buffer* buf) {  // a holder of buf, not counted here
+    auto t = std::make_unique<BufferTensor>();
+    t->of = buf;
+    t->size = buf->mem.bytes;
+    t->dl = {buf->mem.p, 10 /* ROCm */, buf->mem.dev, 1, 1 /* unsigned */, 8, 1, &t->size, &t->step, 0, t.get(), release_tensor};
+    return &t.release()->dl;
+}
 
 }  // namespace rvx
 
@@ -329,12 +336,21 @@ rvx_status rvx_buffer_free(rvx_buffer* buf) {
 rvx_status rvx_buffer_tensor(rvx_buffer* buf, void** out) {
     return guard([&] {
         RVX_REQUIRE(buf && out, RVX_ERR_INVALID_PARAMETER, "null argument");
-        auto t = std::make_unique<BufferTensor>();
-        t->of = buf;
-        t->size = buf->mem.bytes;
-        t->dl = {buf->mem.p, 10 /* ROCm */, buf->mem.dev, 1, 1 /* unsigned */, 8, 1, &t->size, &t->step, 0, t.get(), release_tensor};
+        *out = tensor_of(buf);
         buf->holders.fetch_add(1);
-        *out = &t.release()->dl;
+    });
+}
+rvx_status rvx_buffer_copy_tensor(const rvx_buffer* buf, void** out) {
+    return guard([&] {
+        RVX_REQUIRE(buf && out, RVX_ERR_INVALID_PARAMETER, "null argument");
+        RVX_REQUIRE(buf->mem.dev == device().id, RVX_ERR_INVALID_PARAMETER,
+                    "the buffer is on device " + std::to_string(buf->mem.dev) + ", not the current one");
+        auto copy = std::make_unique<rvx_buffer>();
+        copy->mem.reset(buf->mem.bytes);
+        if (buf->mem.bytes)
+            RVX_HIP(hipMemcpyAsync(copy->mem.p, buf->mem.p, (size_t)buf->mem.bytes, hipMemcpyDeviceToDevice, stream()));
+        *out = tensor_of(copy.get());  // (the tensor is its one holder)
+        copy.release();
     });
 }
 int64_t rvx_buffer_bytes(const rvx_buffer* buf) { return buf ? buf->mem.bytes : 0; }

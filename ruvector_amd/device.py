@@ -104,25 +104,35 @@ class Buffer:
     def __dlpack_device__(self):
         return (10, self._device)  # ROCm
 
-    def __dlpack__(self, stream=None, **_):
+    def __dlpack__(self, stream=None, max_version=None, dl_device=None, copy=None):
         """The allocation as a flat uint8 tensor of another library (DLPack, no copy): what that
         library queues on `stream` waits for the library's work so far. What it writes is ordered
         before later rvx calls by stream_wait(stream). The memory lives until both the Buffer and the
-        tensor are gone. torch has to be imported before this library is first used: the two then
-        share one HIP runtime."""
+        tensor are gone. copy=True: over a copy, made behind what is queued on `stream` and here, that
+        lives as long as the tensor. torch has to be imported before this library is first used: the
+        two then share one HIP runtime."""
+        if dl_device is not None and tuple(int(d) for d in dl_device) != self.__dlpack_device__():
+            raise BufferError(f"the buffer is on device {self.__dlpack_device__()}, not {tuple(dl_device)}")
         if not self._h:
             raise L.RvxError(2, "the buffer is freed")
-        if stream != -1:
-            dev = C.c_int32(0)
-            L.call("rvx_get_device", C.byref(dev))
-            set_device(self._device)
-            try:
-                stream_signal(0 if stream in (None, 1) else stream)
-            finally:
-                set_device(dev.value)
-        p = C.c_void_p()
-        L.call("rvx_buffer_tensor", self._h, C.byref(p))
-        return _capsule_new(p.value, b"dltensor", C.cast(_capsule_dropped, C.c_void_p))
+        dev, p = C.c_int32(0), C.c_void_p()
+        consumer = 0 if stream in (None, 1) else stream
+        L.call("rvx_get_device", C.byref(dev))
+        set_device(self._device)
+        try:
+            if copy and consumer != -1:
+                stream_wait(consumer)
+            if not copy and consumer != -1:
+                stream_signal(consumer)  # (refuses a stream that is being captured, before anything is held)
+            L.call("rvx_buffer_copy_tensor" if copy else "rvx_buffer_tensor", self._h, C.byref(p))
+            capsule = _capsule_new(p.value, b"dltensor", C.cast(_capsule_dropped, C.c_void_p))
+            if copy and consumer != -1:
+                stream_signal(consumer)
+            elif copy:
+                synchronize()
+        finally:
+            set_device(dev.value)
+        return capsule
 
     @classmethod
     def from_numpy(cls, a: np.ndarray) -> "Buffer":
