@@ -26,14 +26,14 @@ AdapterShape adapter_shape(int32_t dtype, int32_t in, int32_t out, int32_t max_r
 
 // src [rows][cols] row-major to fragments [tiles][frags][64 lanes][16 bytes], zero padded; what: 0 W, 1 A, 2 B
 void adapter_pack(int32_t dtype, const void* src, int rows, int cols, int tiles, int frags, int what, void* dst);
-// f32 layers: W once more, as two f16 halves in fragment order and 1 / the scale of each output
+// f32 layers: W once more, as three bf16 a value in fragment order and 1 / the scale of each output
 int64_t adapter_split_bytes(const AdapterShape& s);
-void adapter_split(const AdapterShape& s, const float* w, void* halves, float* inv);
+void adapter_split(const AdapterShape& s, const float* w, void* parts, float* inv);
 
 struct AdapterArgs {
     AdapterShape s;
     const void *w, *bias, *a, *b;  // bias nullable
-    const void* w_split;           // f32: W as two f16 halves, and 1 / their scales
+    const void* w_split;           // f32: W as three bf16 a value, and 1 / the scales
     const float* w_inv;
     const AdapterSlot* slot;
     const void* x;

@@ -315,16 +315,34 @@ __global__ __launch_bounds__(64 * SHRINK_WAVES) void shrink_kernel(const T* __re
     }
 }
 
-// ---------------------------------------------------------------- f32 as two halves
-// f32 products of many rows run on the f16 matrix instructions, 16 times the f32 ones' rate: each row
-// of x and of W is scaled by a power of two to a largest value in [2^14, 2^15) and split into hi + lo,
-// 22 bits of the row's largest values and 2^-39 of them at least of the others, and three products
-// hi hi + hi lo + lo hi give x w within about 2^-22. Fragment q of hi lies beside that of lo. inv: 1 /
-// scale. One wave a row. 4096 x 4096, 2048 rows: 588 us with the f32 instructions, 206 so.
+// ---------------------------------------------------------------- f32 as three bf16
+// f32 products of many rows run on the bf16 matrix instructions, 16 times the f32 ones' rate: a value is
+// exactly the sum of three bf16, h + m + l, each rounded to nearest from what the ones before leave:
+// 8 bits each, |m| <= 2^-8 |h|, |l| <= 2^-17 |h|. Of the nine products the six largest are taken, h h, h m,
+// m h, m m, h l and l h; the others are below 2^-24 |x w| together, half a step of an f32 product.
+// bf16 has f32's range but for its smallest values, so each row of x and of W is scaled by a power of
+// two to a largest value in [2^54, 2^55): a value down to 2^-165 of it is held exactly, smaller ones within
+// 2^-189 of it, and the sum of 2^16 products stays in range. inv: 1 / scale. The three fragments of a depth are
+// neighbours. One wave a row. 4096 x 4096, 2048 rows: 588 us with the f32 instructions, 337 so.
+// (Two f16 values a number, three products: twice as fast, but 22 bits of a row's largest values and fewer
+// of its others, which an f32 layer cannot do with: x = (1, 1.23 2^-26 ..), W = (2^-40, 1.1 ..) was off by 2e-5.)
+constexpr int SPLIT_PARTS = 3;
+constexpr int SPLIT_EXP = 54;
+
+// v as a sum of N values of T, rounded to nearest; all of an infinity or a NaN is in the first
+template <class T, int N>
+__device__ __forceinline__ void pieces_of(float v, T (&p)[N]) {
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+        p[q] = (T)v;
+        v = fabsf((float)p[q]) < INFINITY ? v - (float)p[q] : 0.0f;
+    }
+}
+
 template <bool WEIGHT>
 __global__ __launch_bounds__(1024) void split_kernel(const float* __restrict__ x, int in, int64_t rows,
                                                     const int32_t* __restrict__ perm, int ktq,
-                                                    _Float16* __restrict__ out, float* __restrict__ inv) {
+                                                    __bf16* __restrict__ out, float* __restrict__ inv) {
     const int lane = threadIdx.x & 63, m = threadIdx.x >> 6;
     const int64_t place = WEIGHT ? out_of(blockIdx.x, m) : (int64_t)blockIdx.x * 16 + m;
     const bool there = place < rows;
@@ -342,28 +360,30 @@ __global__ __launch_bounds__(1024) void split_kernel(const float* __restrict__ x
         float v[8];
         piece(p * 8, v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(v[j]));
+        for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(v[j]) < INFINITY ? fabsf(v[j]) : 0.0f);
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
-    const float scale = h2_scale_dev(most);
-    if (there && lane == 0) inv[place] = 1.0f / scale;
+    const int e = most > 0.0f ? min(126, SPLIT_EXP - ilogbf(most)) : 0;
+    const float scale = ldexpf(1.0f, e);
+    if (there && lane == 0) inv[place] = ldexpf(1.0f, -e);
 #pragma unroll 2
     for (int p = lane; p < pieces; p += 64) {
         float v[8];
         piece(p * 8, v);
-        f16x8 hi, lo;
+        bf16x8 part[SPLIT_PARTS];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float s = v[j] * scale;
-            hi[j] = (_Float16)s;
-            lo[j] = (_Float16)(s - (float)hi[j]);
+            __bf16 b[SPLIT_PARTS];
+            pieces_of(v[j] * scale, b);
+#pragma unroll
+            for (int h = 0; h < SPLIT_PARTS; ++h) part[h][j] = b[h];
         }
         // the inverse of in_of: 8 pieces a pair of fragments, two by two of a lane
         const int q = (p >> 3) * 2 + (p & 1), to = ((p & 7) >> 1) * 16 + m;
-        _Float16* o = out + (((int64_t)blockIdx.x * ktq + q) * 2) * 512 + to * 8;
-        __builtin_memcpy(o, &hi, 16);
-        __builtin_memcpy(o + 512, &lo, 16);
+        __bf16* o = out + ((int64_t)blockIdx.x * ktq + q) * SPLIT_PARTS * 512 + to * 8;
+#pragma unroll
+        for (int h = 0; h < SPLIT_PARTS; ++h) __builtin_memcpy(o + h * 512, &part[h], 16);
     }
 }
 
@@ -460,7 +480,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_rows_kernel(const T* __res
 // KF == 1, large tiles: while a stage is multiplied from registers, the next one is read into others.
 // Behind a stage's one barrier everybody has read it, so its place is free for stage s + NS, and has
 // the next: the copies of NS - 2 stages more may still be on their way, which hides their latency.
-// KF > 1, small tiles and halves: a fragment is a few products only, so a barrier serves KF of them; behind it
+// KF > 1, small tiles and split f32: a fragment is a few products only, so a barrier serves KF of them; behind it
 // stage s has arrived and s - 1 is read, whose place the copies of s + NS - 1 take.
 // Bound by LDS, which takes the copies and gives each fragment to WN or WM waves: about 200 bytes a ns
 // of both whatever the tile; larger tiles need fewer for a product. Waves count too: a wave's copies
@@ -505,7 +525,7 @@ __device__ __forceinline__ void spread() {
     __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS, 0);
 }
 
-// P: the products' type; _Float16 with T = float: hi and lo fragments in turn, KF = 2.
+// P: the products' type; __bf16 with T = float: a value's three fragments in turn, KF = 3.
 template <class T, class P, int BM, int BN, int WM, int WN, int NS, int KF>
 __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const P* __restrict__ x, const float* __restrict__ x_inv,
                                                            int64_t n, const P* __restrict__ w,
@@ -518,8 +538,8 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const P* __restrict_
     using Cf = TileCfg<BM, BN, WM, WN, NS, KF>;
     using V = typename Mma<T>::V;
     using PV = typename Mma<P>::V;
-    constexpr bool HALVES = !__is_same(T, P);
-    static_assert(!HALVES || KF == 2);
+    constexpr bool SPLIT = !__is_same(T, P);
+    static_assert(!SPLIT || KF == SPLIT_PARTS);
     constexpr int N = PIECE<T>, TM = Cf::TM, TN = Cf::TN;
     __shared__ __align__(16) unsigned char lds[NS * Cf::STAGE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -573,7 +593,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const P* __restrict_
 #pragma unroll
             for (int f = 0; f < KF; ++f) copy(min(s * KF + f, kt - 1), buf, f);
         };
-        PV xv[2][TM], wv[2][TN];
+        PV xv[SPLIT ? 3 : 2][TM], wv[SPLIT ? 3 : 2][TN];
         auto read = [&](auto to, int buf, int f) {
             constexpr int h = decltype(to)::value;
             const unsigned char* base = lds + buf * Cf::STAGE + f * (Cf::XF + Cf::WF) * 1024 + lane * 16;
@@ -599,19 +619,28 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const P* __restrict_
             for (int s = 0; s < stages; ++s) {
                 wait_and_meet<(NS - 2) * COPIES * KF>();
                 fill(s + NS - 1, last);
-                const int depth = min(KF, kt - s * KF);  // even
-                read(integral_constant<int, 0>{}, buf, 0);
+                constexpr integral_constant<int, 0> I0{};
+                constexpr integral_constant<int, 1> I1{};
+                constexpr integral_constant<int, 2> I2{};
+                read(I0, buf, 0);
+                if constexpr (SPLIT) {
+                    read(I1, buf, 1);
+                    multiply(I0, I0);
+                    read(I2, buf, 2);
+                    multiply(I0, I1);
+                    multiply(I1, I0);
+                    multiply(I1, I1);
+                    multiply(I0, I2);
+                    multiply(I2, I0);
+                } else {
+                    const int depth = min(KF, kt - s * KF);  // even
 #pragma unroll
-                for (int f = 0; f < KF; f += 2) {
-                    if (f >= depth) break;
-                    read(integral_constant<int, 1>{}, buf, f + 1);
-                    multiply(integral_constant<int, 0>{}, integral_constant<int, 0>{});
-                    if (f + 2 < depth) read(integral_constant<int, 0>{}, buf, f + 2);
-                    if constexpr (HALVES) {
-                        multiply(integral_constant<int, 0>{}, integral_constant<int, 1>{});
-                        multiply(integral_constant<int, 1>{}, integral_constant<int, 0>{});
-                    } else {
-                        multiply(integral_constant<int, 1>{}, integral_constant<int, 1>{});
+                    for (int f = 0; f < KF; f += 2) {
+                        if (f >= depth) break;
+                        read(I1, buf, f + 1);
+                        multiply(I0, I0);
+                        if (f + 2 < depth) read(I0, buf, f + 2);
+                        multiply(I1, I1);
                     }
                 }
                 last = buf;
@@ -664,7 +693,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const P* __restrict_
         if (place >= n) row[i] = -1;
     }
     const int col0 = ntw * 16 + (lane >> 4) * 8;  // of the pair j, j + 1: col0 + j * 16 ..
-    if constexpr (HALVES) {
+    if constexpr (SPLIT) {
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
             const float xi = row[i] >= 0 ? x_inv[row0 + (wm * TM + i) * 16 + (lane & 15)] : 0.0f;
@@ -674,8 +703,9 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const P* __restrict_
                 for (int r = 0; r < 4; ++r) {
                     const int col = col0 + (j >> 1) * 32 + (j & 1) * 4 + r;
                     // The scales' product can be past the largest float or below the smallest normal one where
-                    // the result is neither: then one after the other, the larger first (a sum is 0 or in
-                    // [2^-48, 2^46], so the first product is in range unless the result is past it too).
+                    // the result is neither: then one after the other, the larger first. (It is at least 1
+                    // where the product is too large, at most 1 where it is too small, and a sum below
+                    // 2^127: the first step ends in range unless the result does not.)
                     const float wi = col < out ? w_inv[col] : 0.0f, s = xi * wi;
                     const bool normal = s >= 0x1p-126f && s < INFINITY;
                     acc[i][j][r] = normal ? acc[i][j][r] * s : acc[i][j][r] * fmaxf(xi, wi) * fminf(xi, wi);
@@ -775,11 +805,11 @@ void adapter_pack(int32_t dtype, const void* src, int rows, int cols, int tiles,
 }
 
 int64_t adapter_split_bytes(const AdapterShape& s) {
-    return s.dtype == RVX_DTYPE_F32 ? (int64_t)s.nt * split_frags(s.in) * 2048 : 0;
+    return s.dtype == RVX_DTYPE_F32 ? (int64_t)s.nt * split_frags(s.in) * SPLIT_PARTS * 1024 : 0;
 }
-void adapter_split(const AdapterShape& s, const float* w, void* halves, float* inv) {
+void adapter_split(const AdapterShape& s, const float* w, void* parts, float* inv) {
     RVX_LAUNCH("adapter_split", split_kernel<true>, dim3((unsigned)s.nt), dim3(1024), 0, w, s.in, (int64_t)s.out,
-               (const int32_t*)nullptr, split_frags(s.in), (_Float16*)halves, inv);
+               (const int32_t*)nullptr, split_frags(s.in), (__bf16*)parts, inv);
 }
 
 void adapter_forward(const AdapterArgs& g) {
@@ -870,18 +900,18 @@ void adapter_forward(const AdapterArgs& g) {
         constexpr integral_constant<int, 256> I256{};
         if constexpr (F32) {
             const int ktq = split_frags(s.in);
-            const int64_t bytes = row_tiles * ktq * 2048;
-            auto* halves = (char*)scratch_bytes("adapter_x", bytes + n * 4);
-            auto* x_inv = (float*)(halves + bytes);
+            const int64_t bytes = row_tiles * ktq * SPLIT_PARTS * 1024;
+            auto* parts = (char*)scratch_bytes("adapter_x", bytes + n * 4);
+            auto* x_inv = (float*)(parts + bytes);
             RVX_LAUNCH("adapter_split", split_kernel<false>, dim3((unsigned)row_tiles), dim3(1024), 0, x, s.in, n,
-                       (const int32_t*)perm, ktq, (_Float16*)halves, x_inv);
-            // whole layer, 4096 x 4096: 512 rows 91 us by 64 x 64, 115 by 128 x 128; 1024: 149, 131 and 174 by
-            // 256 x 128; 2048: 263, 228, 206; 4096: 525, 433, 390. A round of the larger tiles takes 7 / 4 of one of the
+                       (const int32_t*)perm, ktq, (__bf16*)parts, x_inv);
+            // whole layer, 4096 x 4096: 512 rows 141 us by 64 x 64, 178 by 128 x 128; 1024: 242, 208 and 288 by
+            // 256 x 128; 2048: 428, 365, 337; 4096: 847, 707, 654. A round of the larger tiles takes 7 / 4 of one of the
             // smaller.
-            if (tiles(128, 128) < cus) go(_Float16{}, halves, x_inv, g.w_split, 2 * ktq, I64, I64, I2, I2, I4, I2);
+            if (tiles(128, 128) < cus) go(__bf16{}, parts, x_inv, g.w_split, SPLIT_PARTS * ktq, I64, I64, I2, I2, I3, I3);
             else if (7 * rounds(256, 128) <= 4 * rounds(128, 128))
-                go(_Float16{}, halves, x_inv, g.w_split, 2 * ktq, I256, I128, I4, I2, I3, I2);
-            else go(_Float16{}, halves, x_inv, g.w_split, 2 * ktq, I128, I128, I4, I2, I4, I2);
+                go(__bf16{}, parts, x_inv, g.w_split, SPLIT_PARTS * ktq, I256, I128, I4, I2, I2, I3);
+            else go(__bf16{}, parts, x_inv, g.w_split, SPLIT_PARTS * ktq, I128, I128, I4, I2, I3, I3);
         } else {
             // whole layer, bf16 4096 x 4096: 512 rows 43 us by 64 x 64, 48 by 128 x 128, 66 by 256 x 128, 106 by 256
             // x 256; 1024: 69, 53, 67, 106; 2048: 120, 83, 79, 109; 4096: 227, 152, 149, 135; 8192: 432, 286, 280, 253.

@@ -32,3 +32,62 @@ def test_f32_products_near_the_ends(n, xe, we, inp, out):
     # product within 3 2^-22 of the two rows' largest values
     most = x.abs().amax(1)[:, None] * w.abs().amax(1)
     assert_within(got, want, size * F32 * (inp + 4) + inp * (3 * 2.0 ** -22 * most + TINY["f32"]))
+
+
+def f32_forward(x, w):
+    return run(rv.AdapterLinear(w.shape[1], w.shape[0], to_buffer(w), max_adapters=0), x, None)
+
+
+def assert_f32(got, x, w):
+    """Within what sums of `in` products in 32 bits may be off, whatever the values' sizes beside each other:
+    in - 1 roundings of partial sums, 2^-24 of each product, and the last steps of the smallest numbers."""
+    x, w = x.double(), w.double()
+    inp = x.shape[1]
+    assert_within(got, x @ w.T, (x.abs() @ w.abs().T) * F32 * (inp + 4) + inp * TINY["f32"])
+
+
+@pytest.mark.parametrize("n", [1, 64, 65, 200, 700])
+@pytest.mark.parametrize("inp,out", [(65, 64), (1000, 70)])
+def test_f32_large_values_in_different_columns(n, inp, out):
+    """What is large in x meets what is small in W: the small values of a row count in full."""
+    x, w = torch.full((n, inp), 1.23 * 2.0 ** -26), torch.full((out, inp), 1.1)
+    x[:, 0], w[:, 0] = 1, 2.0 ** -40
+    assert_f32(f32_forward(x, w), x, w)
+
+
+@pytest.mark.parametrize("n", [64, 65, 300])
+@pytest.mark.parametrize("low,high", [(-5, 5), (-30, 30), (-62, 52), (-120, 0)])
+def test_f32_rows_of_any_spread(n, low, high):
+    """Magnitudes spread evenly over many powers of two, within a row and between rows."""
+    g = torch.Generator().manual_seed(n + high)
+    inp, out = 333, 90
+    power = lambda *s: torch.randint(low, high + 1, s, generator=g).double()  # noqa: E731
+    x = (spread(g, n, inp).double() * 2.0 ** power(n, inp)).float()
+    w = (spread(g, out, inp).double() * 2.0 ** power(out, inp)).float()
+    if high == 0:  # the small values of x beside the large ones of W
+        x[:, ::2] = 0
+        x[:, 0] = 1
+        w[:, 0] = 2.0 ** -126
+        w[:, 1:] = spread(g, out, inp - 1) * 2.0 ** 100
+    assert_f32(f32_forward(x, w), x, w)
+
+
+@pytest.mark.parametrize("n", [64, 65, 200])
+@pytest.mark.parametrize("xe,we", [(-61, -61), (-20, -102), (60, 60), (100, -126), (-126, 100), (0, 0)])
+def test_f32_as_exact_as_32_bits(n, xe, we):
+    g = torch.Generator().manual_seed(n - xe)
+    x, w = spread(g, n, 100) * 2.0 ** xe, spread(g, 70, 100) * 2.0 ** we
+    assert_f32(f32_forward(x, w), x, w)
+
+
+@pytest.mark.parametrize("n", [5, 100])
+def test_f32_infinities_stay_in_their_rows(n):
+    """A row with an infinity or a NaN is not finite; the others, and its own scale, are as without."""
+    g = torch.Generator().manual_seed(n)
+    x, w = spread(g, n, 80), spread(g, 50, 80) * 1e-20
+    clean = f32_forward(x, w)
+    x[2, 7], x[4, 9] = torch.inf, torch.nan
+    got = f32_forward(x, w)
+    keep = torch.ones(n, dtype=torch.bool)
+    keep[[2, 4]] = False
+    assert torch.equal(got[keep], clean[keep]) and not torch.isfinite(got[[2, 4]]).any() and got[4].isnan().all()
