@@ -435,7 +435,8 @@ rvx_status rvx_log_probs_backward_device(const rvx_buffer* scores, int32_t dtype
  * belong to different tenants or requests:
  *   y[i] = W x[i] + bias + scale_r B_r (A_r x[i]),  r = adapter_ids[i],
  * W [out][in], bias [out], A_r [rank_r][in], B_r [out][rank_r], x [n][in], y [n][out], all row-major
- * of the layer's dtype; A_r x is kept in 32 bits. The layer copies weights and adapters into its
+ * of the layer's dtype; A_r x is kept in 32 bits (f16, more than 64
+ * rows: within 2^-39 of a row's largest value of it). The layer copies weights and adapters into its
  * own layout, so their buffers may be freed after the call. A row whose id is outside
  * [0, max_adapters), or names a slot never set or set with rank 0, has no adapter. An f32 layer
  * takes more than 64 rows as three bf16 values a number, each row of x and W scaled by a power of two:

@@ -159,14 +159,29 @@ __global__ __launch_bounds__(GROUP_THREADS) void group_rows_kernel(const int32_t
 }
 
 // ---------------------------------------------------------------- t = s A x
-// What the projection reads of t. Few rows: f32, `f`, as FEW_PARTS parts to be added up. Tiles: pieces of T, hi + lo, 16 (bf16) or 22
-// (f16) bits of each value, so that t's rounding is far below y's (f32: hi alone); f16: a row whose
-// largest value is not in [2^-3, 2^15) is scaled by a power of two to [2^14, 2^15), undone by `back`.
+// v as a sum of N values of T, rounded to nearest; all of an infinity or a NaN is in the first
+template <class T, int N>
+__device__ __forceinline__ void pieces_of(float v, T (&p)[N]) {
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+        p[q] = (T)v;
+        v = fabsf((float)p[q]) < INFINITY ? v - (float)p[q] : 0.0f;
+    }
+}
+
+// What the projection reads of t. Few rows: f32, `f`, as FEW_PARTS parts to be added up. Tiles: as
+// pieces of T for its matrix instructions, `plane` elements apart, whose sum is t: one in f32, three in bf16 (all
+// 24 bits) and f16. f16: each row is scaled by a power of two to a largest value in [2^14, 2^15), undone by
+// `back`; the sum of three is then t within half of f16's smallest step, 2^-25, which is 2^-39 of the largest.
+// (Two pieces held 16 bits in bf16 and took within 1% of the time.)
 constexpr int FEW_PARTS = 4;
+template <class T>
+constexpr int MID_PIECES = sizeof(T) == 2 ? 3 : 1;
 template <class T>
 struct Mid {
     float* f;
-    T *hi, *lo;
+    T* piece;
+    int64_t plane;
     float* back;
     int32_t* eff;  // few rows: a row's adapter and its rank, id * 256 + rank, -1 = none
     int ld;
@@ -260,54 +275,62 @@ __global__ __launch_bounds__(64 * SHRINK_WAVES) void shrink_kernel(const T* __re
             if (wave == 0) {
                 // lane l has ranks r * 16 + (l / 16) * 4 .. of row l % 16
                 const AdapterSlot info = slot[id];
-                float v[RT][4], most = 0.0f;
-#pragma unroll
-                for (int r = 0; r < RT; ++r) {
+                auto value = [&](int r, float (&v)[4]) {
                     f32x4 sum = red[0][r][lane];
 #pragma unroll
                     for (int w = 1; w < WAVES; ++w) sum += red[w][r][lane];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        // past the adapter's rank: zeros, whatever x holds
-                        v[r][j] = r * 16 + (lane >> 4) * 4 + j < info.rank ? sum[j] * info.scale : 0.0f;
-                        most = fmaxf(most, fabsf(v[r][j]));
+                    for (int j = 0; j < 4; ++j)  // past the adapter's rank: zeros, whatever x holds
+                        v[j] = r * 16 + (lane >> 4) * 4 + j < info.rank ? sum[j] * info.scale : 0.0f;
+                };
+                const int64_t at = row0 + (lane & 15);  // the place in the permutation
+                const bool own = __shfl(mine, lane & 15) == id;
+                auto write = [&](int r, const float (&v)[4], float up) {
+                    const int64_t o = at * t.ld + r * 16 + (lane >> 4) * 4;
+                    if (!own) return;
+                    if constexpr (!SPLIT) {
+                        __builtin_memcpy(t.f + (int64_t)blockIdx.z * n * t.ld + o, v, 16);
+                    } else {
+                        T p[4][MID_PIECES<T>];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) pieces_of(v[j] * up, p[j]);
+#pragma unroll
+                        for (int q = 0; q < MID_PIECES<T>; ++q) {
+                            const T four[4] = {p[0][q], p[1][q], p[2][q], p[3][q]};
+                            __builtin_memcpy(t.piece + q * t.plane + o, four, sizeof(four));
+                        }
                     }
-                }
-                float up = 1.0f, down = 1.0f;
+                };
                 if constexpr (SPLIT && __is_same(T, _Float16)) {
+                    float v[RT][4], most = 0.0f;
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) {
+                        value(r, v[r]);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(v[r][j]));
+                    }
                     most = fmaxf(most, __shfl_xor(most, 16));
                     most = fmaxf(most, __shfl_xor(most, 32));
-                    if (most > 0.0f && most < INFINITY && !(most >= 0.125f && most < 32768.0f)) {
+                    float up = 1.0f, down = 1.0f;
+                    if (most > 0.0f && most < INFINITY) {
                         const int e = min(126, max(-126, 14 - ilogbf(most)));
                         up = ldexpf(1.0f, e), down = ldexpf(1.0f, -e);
                     }
-                }
-                const int64_t at = row0 + (lane & 15);  // the place in the permutation
-                if (__shfl(mine, lane & 15) == id) {
-                    if constexpr (!SPLIT) {
+                    if (own && lane < 16) t.back[at] = down;
 #pragma unroll
-                        for (int r = 0; r < RT; ++r) __builtin_memcpy(t.f + (blockIdx.z * n + at) * t.ld + r * 16 + (lane >> 4) * 4, v[r], 16);
-                    } else {
-                        if (t.back && lane < 16) t.back[at] = down;
-#pragma unroll
-                        for (int r = 0; r < RT; ++r) {
-                            T hi[4], lo[4];
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                hi[j] = (T)(v[r][j] * up);
-                                lo[j] = fabsf((float)hi[j]) < INFINITY ? (T)(v[r][j] * up - (float)hi[j]) : (T)0.0f;
-                            }
-                            const int64_t o = at * t.ld + r * 16 + (lane >> 4) * 4;
-                            __builtin_memcpy(t.hi + o, hi, sizeof(hi));
-                            if (sizeof(T) == 2) __builtin_memcpy(t.lo + o, lo, sizeof(lo));
-                        }
-                        if (RT == 1 && t.ld > 16) {  // a fragment is 32 ranks deep
-                            const int64_t o = at * t.ld + 16 + (lane >> 4) * 4;
-                            const T zero[4] = {};
-                            __builtin_memcpy(t.hi + o, zero, sizeof(zero));
-                            __builtin_memcpy(t.lo + o, zero, sizeof(zero));
-                        }
+                    for (int r = 0; r < RT; ++r) write(r, v[r], up);
+                } else {
+                    constexpr int TURNS = SPLIT && RT == 8 ? 1 : RT;  // (8 at once would spill)
+#pragma unroll TURNS
+                    for (int r = 0; r < RT; ++r) {
+                        float v[4];
+                        value(r, v);
+                        write(r, v, 1.0f);
                     }
+                }
+                if (SPLIT && RT == 1 && t.ld > 16) {  // a fragment is 32 ranks deep
+                    const float zero[4] = {};
+                    write(1, zero, 1.0f);
                 }
             }
             __syncthreads();
@@ -324,20 +347,10 @@ __global__ __launch_bounds__(64 * SHRINK_WAVES) void shrink_kernel(const T* __re
 // two to a largest value in [2^54, 2^55): a value down to 2^-165 of it is held exactly, smaller ones within
 // 2^-189 of it, and the sum of 2^16 products stays in range. inv: 1 / scale. The three fragments of a depth are
 // neighbours. One wave a row. 4096 x 4096, 2048 rows: 588 us with the f32 instructions, 337 so.
-// (Two f16 values a number, three products: twice as fast, but 22 bits of a row's largest values and fewer
+// (Two f16 values a number, three products: 206 us, but 22 bits of a row's largest values and fewer
 // of its others, which an f32 layer cannot do with: x = (1, 1.23 2^-26 ..), W = (2^-40, 1.1 ..) was off by 2e-5.)
 constexpr int SPLIT_PARTS = 3;
 constexpr int SPLIT_EXP = 54;
-
-// v as a sum of N values of T, rounded to nearest; all of an infinity or a NaN is in the first
-template <class T, int N>
-__device__ __forceinline__ void pieces_of(float v, T (&p)[N]) {
-#pragma unroll
-    for (int q = 0; q < N; ++q) {
-        p[q] = (T)v;
-        v = fabsf((float)p[q]) < INFINITY ? v - (float)p[q] : 0.0f;
-    }
-}
 
 template <bool WEIGHT>
 __global__ __launch_bounds__(1024) void split_kernel(const float* __restrict__ x, int in, int64_t rows,
@@ -721,18 +734,16 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const P* __restrict_
             for (int i = 0; i < TM; ++i)
                 if (who[i] >= 0) back[i] = t.back[row0 + (wm * TM + i) * 16 + (lane & 15)];
         for (int k = 0; k < rk; ++k) {
-            V hi[TM], lo[TM];  // rows without an adapter hold anything: their products are dropped
-#pragma unroll
-            for (int i = 0; i < TM; ++i) {
-                const int64_t place = min(row0 + (wm * TM + i) * 16 + (lane & 15), n - 1);
-                const int64_t at = place * t.ld + k * DEPTH<T> + (lane >> 4) * N;
-                hi[i] = load_piece(t.hi + at);
-                if constexpr (sizeof(T) == 2) lo[i] = load_piece(t.lo + at);
-            }
             int held = -1;
             V bv[TN];
 #pragma unroll
             for (int i = 0; i < TM; ++i) {
+                // rows without an adapter hold anything: their products are dropped
+                const int64_t place = min(row0 + (wm * TM + i) * 16 + (lane & 15), n - 1);
+                const T* at = t.piece + place * t.ld + k * DEPTH<T> + (lane >> 4) * N;
+                V tv[MID_PIECES<T>];
+#pragma unroll
+                for (int q = 0; q < MID_PIECES<T>; ++q) tv[q] = load_piece(at + q * t.plane);
                 unsigned long long todo = __ballot(who[i] >= 0);
                 while (todo) {
                     const int id = __builtin_amdgcn_readlane(who[i], __ffsll(todo) - 1);
@@ -746,8 +757,9 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const P* __restrict_
                     }
 #pragma unroll
                     for (int j = 0; j < TN; ++j) {
-                        f32x4 add = Mma<T>::run(bv[j], hi[i], f32x4{0, 0, 0, 0});
-                        if constexpr (sizeof(T) == 2) add = Mma<T>::run(bv[j], lo[i], add);
+                        f32x4 add{0, 0, 0, 0};
+#pragma unroll
+                        for (int q = 0; q < MID_PIECES<T>; ++q) add = Mma<T>::run(bv[j], tv[q], add);
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
                             acc[i][j][r] = who[i] == id ? fmaf(add[r], back[i], acc[i][j][r]) : acc[i][j][r];
@@ -835,10 +847,9 @@ void adapter_forward(const AdapterArgs& g) {
                 while (bits < GROUP_BITS && (1 << bits) <= s.slots) ++bits;
                 RVX_LAUNCH("adapter_group", group_rows_kernel, dim3((unsigned)((n + GROUP_ROWS - 1) / GROUP_ROWS)),
                            dim3(GROUP_THREADS), 0, g.ids, n, s.slots, bits, perm);
-                const int64_t plane = n * t.ld;
-                t.hi = (T*)scratch_bytes("adapter_t", 2 * plane * (int64_t)sizeof(T) + n * 4);
-                t.lo = t.hi + plane;
-                t.back = __is_same(T, _Float16) ? (float*)(t.lo + plane) : nullptr;
+                t.plane = n * t.ld;
+                t.piece = (T*)scratch_bytes("adapter_t", MID_PIECES<T> * t.plane * (int64_t)sizeof(T) + n * 4);
+                t.back = __is_same(T, _Float16) ? (float*)(t.piece + MID_PIECES<T> * t.plane) : nullptr;
             }
         }
         constexpr bool F32 = __is_same(T, float);

@@ -4,9 +4,8 @@ import pytest
 import torch
 
 rv = pytest.importorskip("ruvector_amd")
-from heads_ref import F32, TINY, assert_within  # noqa: E402
+from heads_ref import DTYPES, F32, HALF, TINY, assert_within, to_buffer  # noqa: E402
 from test_gpu_adapters import run  # noqa: E402
-from heads_ref import to_buffer  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -91,3 +90,39 @@ def test_f32_infinities_stay_in_their_rows(n):
     keep = torch.ones(n, dtype=torch.bool)
     keep[[2, 4]] = False
     assert torch.equal(got[keep], clean[keep]) and not torch.isfinite(got[[2, 4]]).any() and got[4].isnan().all()
+
+
+def adapted(x, a, b, dtype):
+    """b (a x) alone: a layer with weights of zero and one adapter."""
+    n, inp = x.shape
+    layer = rv.AdapterLinear(inp, b.shape[0], to_buffer(torch.zeros(b.shape[0], inp, dtype=DTYPES[dtype])), max_rank=a.shape[0],
+                             max_adapters=1, dtype=dtype)
+    layer.set_adapter(0, a.shape[0], to_buffer(a), to_buffer(b))
+    return run(layer, x, torch.zeros(n, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", [1, 64, 65, 300])
+@pytest.mark.parametrize("rank", [2, 40, 100])
+@pytest.mark.parametrize("size", [1.0, 2.0 ** -9, 2.0 ** 8])
+def test_a_x_in_32_bits(dtype, n, rank, size):
+    """Pairs of nearly equal A x whose difference is y: what A x loses shows."""
+    g = torch.Generator().manual_seed(n + rank)
+    inp, out, T = 8, 20, DTYPES[dtype]
+    x = (spread(g, n, inp) * size).to(T)
+    a = spread(g, rank, inp).to(T)
+    a[1::2] = a[0::2]
+    a[1::2, 0] += a[0::2, 0] * 2.0 ** -6
+    b = spread(g, out, rank).to(T)
+    b[:, 1::2] = -b[:, 0::2]
+    got = adapted(x, a, b, dtype)
+    x, a, b = x.double(), a.double(), b.double()
+    t, ts = x @ a.T, x.abs() @ a.abs().T
+    # t: a sum of `in` products, and a step of 32 bits (f16: 2^-39 of the row's largest); then the sum of the
+    # products with B, each of up to three pieces, and y's rounding
+    off = ts * F32 * (inp + 1)
+    if dtype == "f16":
+        off = off + t.abs().amax(1, keepdim=True) * 2.0 ** -39
+    want = t @ b.T
+    tol = off @ b.abs().T + (t.abs() @ b.abs().T) * F32 * (3 * rank + 1)
+    assert_within(got, want, tol * 1.01 + want.abs() * HALF[dtype] * 1.01 + TINY[dtype])
