@@ -307,12 +307,13 @@ __global__ __launch_bounds__(64 * SHRINK_WAVES) void shrink_kernel(const T* __re
                     for (int r = 0; r < RT; ++r) {
                         value(r, v[r]);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(v[r][j]));
+                        for (int j = 0; j < 4; ++j)  // an infinity stays one, the others still have to fit
+                            most = fmaxf(most, fabsf(v[r][j]) < INFINITY ? fabsf(v[r][j]) : 0.0f);
                     }
                     most = fmaxf(most, __shfl_xor(most, 16));
                     most = fmaxf(most, __shfl_xor(most, 32));
                     float up = 1.0f, down = 1.0f;
-                    if (most > 0.0f && most < INFINITY) {
+                    if (most > 0.0f) {
                         const int e = min(126, max(-126, 14 - ilogbf(most)));
                         up = ldexpf(1.0f, e), down = ldexpf(1.0f, -e);
                     }

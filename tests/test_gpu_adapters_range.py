@@ -126,3 +126,16 @@ def test_a_x_in_32_bits(dtype, n, rank, size):
     want = t @ b.T
     tol = off @ b.abs().T + (t.abs() @ b.abs().T) * F32 * (3 * rank + 1)
     assert_within(got, want, tol * 1.01 + want.abs() * HALF[dtype] * 1.01 + TINY[dtype])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", [3, 64, 65, 200])
+@pytest.mark.parametrize("first,want", [((1, -1), torch.inf), ((-1, -1), -torch.inf), ((1, 0), torch.inf), ((0, 1), torch.nan)])
+def test_an_infinite_a_x_beside_a_large_one(dtype, n, first, want):
+    """A x = (inf, 384000): the second is past f16, yet no infinity."""
+    T = DTYPES[dtype]
+    a = torch.zeros(2, 64, dtype=T)
+    a[0, 0], a[1] = torch.inf, 60
+    got = adapted(torch.full((n, 64), 100.0, dtype=T), a, torch.tensor([first] * 20, dtype=T), dtype)
+    assert torch.equal(got.float().nan_to_num(nan=1.0, posinf=2.0, neginf=-2.0),
+                       torch.full((n, 20), want).nan_to_num(nan=1.0, posinf=2.0, neginf=-2.0))
