@@ -159,12 +159,14 @@ __global__ __launch_bounds__(GROUP_THREADS) void group_rows_kernel(const int32_t
 }
 
 // ---------------------------------------------------------------- t = s A x
-// v as a sum of N values of T, rounded to nearest; all of an infinity or a NaN is in the first
+// v as a sum of N values of T, rounded to nearest; all of an infinity or a NaN is in the first. (A finite v
+// that would be rounded to infinity, next to the largest float: bf16's largest value first.)
 template <class T, int N>
 __device__ __forceinline__ void pieces_of(float v, T (&p)[N]) {
 #pragma unroll
     for (int q = 0; q < N; ++q) {
         p[q] = (T)v;
+        if (__is_same(T, __bf16) && fabsf((float)p[q]) == INFINITY && fabsf(v) < INFINITY) p[q] = (T)copysignf(0x1.fep127f, v);
         v = fabsf((float)p[q]) < INFINITY ? v - (float)p[q] : 0.0f;
     }
 }

@@ -139,3 +139,13 @@ def test_an_infinite_a_x_beside_a_large_one(dtype, n, first, want):
     got = adapted(torch.full((n, 64), 100.0, dtype=T), a, torch.tensor([first] * 20, dtype=T), dtype)
     assert torch.equal(got.float().nan_to_num(nan=1.0, posinf=2.0, neginf=-2.0),
                        torch.full((n, 20), want).nan_to_num(nan=1.0, posinf=2.0, neginf=-2.0))
+
+
+@pytest.mark.parametrize("n", [3, 64, 65, 200])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_bf16_a_x_next_to_the_largest_float(n, sign):
+    """A x = 2^128 - 2^119, a float that is rounded to an infinite bf16."""
+    a = torch.zeros(1, 64).bfloat16()
+    a[0, 3], a[0, 40] = sign * 2.0 ** 127, sign * (2.0 ** 127 - 2.0 ** 119)
+    got = adapted(torch.ones(n, 64).bfloat16(), a, torch.full((20, 1), 2.0 ** -100).bfloat16(), "bf16")
+    assert torch.equal(got, torch.full((n, 20), sign * 2.0 ** 28).bfloat16())  # 2^28 - 2^19 in 8 bits
