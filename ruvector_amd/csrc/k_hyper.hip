@@ -27,7 +27,60 @@ __global__ void k_project_rows(float* x, int64_t n, int d, float c) {
     pdev::project_inplace(x + r * d, d, c, pdev::EPS);
 }
 
+// pdev::log_map_negp for d a multiple of 4 and aligned rows: the same operations on every value in the same
+// order, four values a load, with -p (+) y computed again where it is needed instead of stored and read back.
+// 100000 x 1024: 0.84 ms; a value a load 6.7 ms (5.1 with packed f32 instructions, for which the compiler joins
+// loads by itself). Bound by reading x three times, a row a lane.
+__device__ __forceinline__ float chunk_sq(float4 v) { return ((v.x * v.x + v.y * v.y) + v.z * v.z) + v.w * v.w; }
+__device__ void log_map_negp4(const float4* y, const float4* negp, float np_sq, int d4, float c, float4* out) {
+    c = fmaxf(fabsf(c), pdev::EPS);
+    const float sqrt_c = sqrtf(c);
+    float nx = 0.0f, ny = 0.0f, dxy = 0.0f;
+#pragma unroll 4
+    for (int i = 0; i < d4; ++i) {
+        const float4 p = negp[i], v = y[i];
+        nx = nx + chunk_sq(p);
+        ny = ny + chunk_sq(v);
+        dxy = dxy + (((p.x * v.x + p.y * v.y) + p.z * v.z) + p.w * v.w);
+    }
+    const float coef_x = (1.0f + 2.0f * c * dxy) + c * ny;
+    const float coef_y = 1.0f - c * nx;
+    const float inv = 1.0f / fmaxf((1.0f + 2.0f * c * dxy) + c * c * nx * ny, pdev::EPS);
+    auto diff = [&](int i) {
+        const float4 p = negp[i], v = y[i];
+        return float4{(coef_x * p.x + coef_y * v.x) * inv, (coef_x * p.y + coef_y * v.y) * inv,
+                      (coef_x * p.z + coef_y * v.z) * inv, (coef_x * p.w + coef_y * v.w) * inv};
+    };
+    auto times = [](float4 v, float f) { return float4{v.x * f, v.y * f, v.z * f, v.w * f}; };
+    float ns = 0.0f;
+#pragma unroll 4
+    for (int i = 0; i < d4; ++i) ns = ns + chunk_sq(diff(i));
+    // project_inplace
+    const float max_norm = (1.0f / sqrt_c) - pdev::EPS;
+    const bool outside = ns >= max_norm * max_norm && ns >= pdev::EPS * pdev::EPS;
+    const float scale = outside ? max_norm / sqrtf(ns) : 1.0f;  // (a product with 1 changes nothing)
+    if (outside) {
+        ns = 0.0f;
+        for (int i = 0; i < d4; ++i) ns = ns + chunk_sq(times(diff(i), scale));
+    }
+    const float norm_diff = sqrtf(ns);
+    if (norm_diff < pdev::EPS) {
+        for (int i = 0; i < d4; ++i) out[i] = float4{0.0f, 0.0f, 0.0f, 0.0f};
+        return;
+    }
+    const float lambda_p = 2.0f / fmaxf(1.0f - c * np_sq, pdev::EPS);
+    const float arg = fminf(sqrt_c * norm_diff, 1.0f - pdev::EPS);
+    const float coef = (2.0f / (sqrt_c * lambda_p)) * glibc::rust_atanhf(arg) / norm_diff;
+#pragma unroll 4
+    for (int i = 0; i < d4; ++i) out[i] = times(times(diff(i), scale), coef);
+}
+
 // out[r] = log_centroid(x[r]) with -centroid and |centroid|^2 precomputed.
+__global__ void k_log_map_rows4(const float* x, int64_t n, int d, const float* negp, float np_sq, float c, float* out) {
+    const int64_t r = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (r >= n) return;
+    log_map_negp4((const float4*)(x + r * d), (const float4*)negp, np_sq, d / 4, c, (float4*)(out + r * d));
+}
 __global__ void k_log_map_rows(const float* x, int64_t n, int d, const float* negp, float np_sq, float c, float* out) {
     const int64_t r = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (r >= n) return;
@@ -194,8 +247,9 @@ void poincare_topk(const float* q, int64_t nq, const float* x, int64_t n, int d,
 
 void log_map_rows(const float* x, int64_t n, int d, const float* negp_dev, float np_sq, float c, float* out) {
     if (n <= 0) return;
-    RVX_LAUNCH("hyp_log_map", k_log_map_rows, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, x, n, d, negp_dev, np_sq,
-               c, out);
+    const bool vec = d % 4 == 0 && (((uintptr_t)x | (uintptr_t)negp_dev | (uintptr_t)out) & 15) == 0;
+    RVX_LAUNCH("hyp_log_map", vec ? k_log_map_rows4 : k_log_map_rows, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, x,
+               n, d, negp_dev, np_sq, c, out);
 }
 
 void col_chain(const float* rows, int64_t n, int d, float w, float* acc) {
