@@ -1155,6 +1155,9 @@ __global__ __launch_bounds__(256) void k_scan_rerank(RerankArgs a) {
         if (r[j] == INT32_MAX || !(v[j] <= D)) continue;
         const float* xr = a.x + (int64_t)r[j] * a.d;
         float acc = 0.0f;
+        // (eight loads of a row on their way, which single-value arithmetic needs more than packed did: cosine
+        // 400000 x 768, 256 queries 0.88 ms packed, 0.95 without, 0.53 so; the sum's order stays)
+#pragma unroll 8
         for (int kk = 0; kk < a.d; kk += 4) {
             const float4 qv = *reinterpret_cast<const float4*>(qrow + kk);
             const float4 xv = *reinterpret_cast<const float4*>(xr + kk);
