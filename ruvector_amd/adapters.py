@@ -9,7 +9,7 @@ import ctypes as C
 from typing import Optional
 
 from . import _lib as L
-from .device import Buffer, dtype_code, int32
+from .device import Buffer, dtype_code, int32, int64
 
 
 class AdapterError(L.RvxError):
@@ -48,7 +48,7 @@ class AdapterLinear:
 
     def forward_device(self, x: Buffer, n: int, y: Buffer, adapter_ids: Optional[Buffer] = None) -> None:
         """x [n][in] -> y [n][out]; adapter_ids int32 [n], ids without an adapter (-1) get none."""
-        _check("rvx_adapter_linear_forward_device", self._h, x.handle, n, None if adapter_ids is None else adapter_ids.handle,
+        _check("rvx_adapter_linear_forward_device", self._h, x.handle, int64(n, "n"), None if adapter_ids is None else adapter_ids.handle,
                y.handle)
 
     def __del__(self):

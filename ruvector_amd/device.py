@@ -56,12 +56,21 @@ def dtype_code(dtype: str) -> int:
         raise L.RvxError(2, f"unknown dtype {dtype!r}: one of {', '.join(_DTYPES)}") from None
 
 
+def _whole(value, what: str, bits: int) -> int:
+    n = int(value)
+    if n != value or not -2 ** (bits - 1) <= n < 2 ** (bits - 1):
+        raise L.RvxError(2, f"{what} {value} is not a {bits}-bit whole number")
+    return n
+
+
 def int32(value, what: str) -> int:
     """`value` as a C int32 argument (ctypes would cut a larger one short)."""
-    value = int(value)
-    if not -2 ** 31 <= value < 2 ** 31:
-        raise L.RvxError(2, f"{what} {value} is not a 32-bit number")
-    return value
+    return _whole(value, what, 32)
+
+
+def int64(value, what: str) -> int:
+    """`value` as a C int64 argument."""
+    return _whole(value, what, 64)
 
 
 _capsule_new = C.PYFUNCTYPE(C.py_object, C.c_void_p, C.c_char_p, C.c_void_p)(("PyCapsule_New", C.pythonapi))

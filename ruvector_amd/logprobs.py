@@ -10,7 +10,7 @@ from __future__ import annotations
 from typing import Optional
 
 from . import _lib as L
-from .device import Buffer, dtype_code, int32
+from .device import Buffer, dtype_code, int32, int64
 
 
 class LogProbsError(L.RvxError):
@@ -38,7 +38,8 @@ def log_probs_device(scores: Buffer, n: int, c: int, temperature: float = 1.0, t
     int64 of the target (-1 without one), entropy [n] f32, stats [n][2] f32 for
     log_probs_backward_device, and the k <= 64 best ids top_ids [n][k] int64 with top_logp [n][k]
     f32 (lowest id first among equals; -1 / -inf past the scores above -inf)."""
-    _check("rvx_log_probs_device", scores.handle, dtype_code(dtype), n, c, c if ld is None else ld, temperature,
+    _check("rvx_log_probs_device", scores.handle, dtype_code(dtype), int64(n, "n"), int64(c, "c"),
+           int64(c if ld is None else ld, "ld"), temperature,
            _h(targets), int32(k, "k"), _h(logp), _h(rank), _h(entropy), _h(stats), _h(top_ids), _h(top_logp))
 
 
@@ -50,6 +51,7 @@ def log_probs_backward_device(scores: Buffer, n: int, c: int, temperature: float
     gradients by logp and by entropy (f32 [n]; None = zeros), with stats and entropy as
     log_probs_device wrote them. grad may be the scores buffer."""
     ld = c if ld is None else ld
-    _check("rvx_log_probs_backward_device", scores.handle, dtype_code(dtype), n, c, ld, temperature, _h(targets),
+    _check("rvx_log_probs_backward_device", scores.handle, dtype_code(dtype), int64(n, "n"), int64(c, "c"), int64(ld, "ld"),
+           temperature, _h(targets),
            stats.handle, _h(grad_logp), _h(entropy), _h(grad_entropy), grad.handle,
-           (ld if grad is scores else c) if ld_grad is None else ld_grad)
+           int64((ld if grad is scores else c) if ld_grad is None else ld_grad, "ld_grad"))
