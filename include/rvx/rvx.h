@@ -441,7 +441,7 @@ rvx_status rvx_log_probs_backward_device(const rvx_buffer* scores, int32_t dtype
  * [0, max_adapters), or names a slot never set or set with rank 0, has no adapter. An f32 layer
  * takes more than 64 rows as three bf16 values a number, each row of x and W scaled by a power of two:
  * a product x_j W_oj is then off by at most 2^-24 of itself (and 2^-188 max|x| max|W_o|), as an f32
- * product is, but an infinity in x or W can make outputs NaN that are infinite otherwise. */
+ * product is. */
 typedef struct rvx_adapter_linear rvx_adapter_linear;
 typedef struct {
     int32_t in_features, out_features;  /* 1 .. 65536 */

@@ -349,7 +349,8 @@ __global__ __launch_bounds__(64 * SHRINK_WAVES) void shrink_kernel(const T* __re
 // bf16 has f32's range but for its smallest values, so each row of x and of W is scaled by a power of
 // two to a largest value in [2^54, 2^55): a value down to 2^-165 of it is held exactly, smaller ones within
 // 2^-189 of it, and the sum of 2^16 products stays in range. inv: 1 / scale. The three fragments of a depth are
-// neighbours. One wave a row. 4096 x 4096, 2048 rows: 588 us with the f32 instructions, 337 so.
+// neighbours. inv is negative for a row with an infinity and no NaN: the product of an infinity and a part that
+// is 0 would be a NaN, so its outputs are added up once more from the values themselves. One wave a row. 4096 x 4096, 2048 rows: 588 us with the f32 instructions, 337 so.
 // (Two f16 values a number, three products: 206 us, but 22 bits of a row's largest values and fewer
 // of its others, which an f32 layer cannot do with: x = (1, 1.23 2^-26 ..), W = (2^-40, 1.1 ..) was off by 2e-5.)
 constexpr int SPLIT_PARTS = 3;
@@ -370,19 +371,24 @@ __global__ __launch_bounds__(1024) void split_kernel(const float* __restrict__ x
             for (int j = 0; j < 8; ++j) v[j] = there && c + j < in ? row[c + j] : 0.0f;
     };
     float most = 0.0f;
+    bool inf = false, nan = false;
     const int pieces = ktq * 4;
 #pragma unroll 4
     for (int p = lane; p < pieces; p += 64) {
         float v[8];
         piece(p * 8, v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(v[j]) < INFINITY ? fabsf(v[j]) : 0.0f);
+        for (int j = 0; j < 8; ++j) {
+            most = fmaxf(most, fabsf(v[j]) < INFINITY ? fabsf(v[j]) : 0.0f);
+            inf |= fabsf(v[j]) == INFINITY, nan |= v[j] != v[j];
+        }
     }
+    inf = __any(inf) && !__any(nan);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
     const int e = most > 0.0f ? min(126, SPLIT_EXP - ilogbf(most)) : 0;
     const float scale = ldexpf(1.0f, e);
-    if (there && lane == 0) inv[place] = ldexpf(1.0f, -e);
+    if (there && lane == 0) inv[place] = ldexpf(inf ? -1.0f : 1.0f, -e);
 #pragma unroll 2
     for (int p = lane; p < pieces; p += 64) {
         float v[8];
@@ -550,7 +556,9 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const P* __restrict_
                                                            int64_t b_slot, int rk, const int32_t* __restrict__ ids,
                                                            const int32_t* __restrict__ perm,
                                                            const AdapterSlot* __restrict__ slot, int slots, Mid<T> t,
-                                                           int out, int tiles_m, int tiles_n, T* y) {
+                                                           int out, int tiles_m, int tiles_n, T* y,
+                                                           const T* __restrict__ x_plain, const T* __restrict__ w_plain,
+                                                           int in, int kt_plain) {  // (split f32)
     using Cf = TileCfg<BM, BN, WM, WN, NS, KF>;
     using V = typename Mma<T>::V;
     using PV = typename Mma<P>::V;
@@ -710,9 +718,11 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const P* __restrict_
     }
     const int col0 = ntw * 16 + (lane >> 4) * 8;  // of the pair j, j + 1: col0 + j * 16 ..
     if constexpr (SPLIT) {
+        bool infinite = false;
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
-            const float xi = row[i] >= 0 ? x_inv[row0 + (wm * TM + i) * 16 + (lane & 15)] : 0.0f;
+            const float x_scale = row[i] >= 0 ? x_inv[row0 + (wm * TM + i) * 16 + (lane & 15)] : 0.0f, xi = fabsf(x_scale);
+            infinite |= x_scale < 0.0f;
 #pragma unroll
             for (int j = 0; j < TN; ++j)
 #pragma unroll
@@ -722,10 +732,36 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const P* __restrict_
                     // the result is neither: then one after the other, the larger first. (It is at least 1
                     // where the product is too large, at most 1 where it is too small, and a sum below
                     // 2^127: the first step ends in range unless the result does not.)
-                    const float wi = col < out ? w_inv[col] : 0.0f, s = xi * wi;
+                    const float w_scale = col < out ? w_inv[col] : 0.0f, wi = fabsf(w_scale), s = xi * wi;
+                    if (i == 0) infinite |= w_scale < 0.0f;
                     const bool normal = s >= 0x1p-126f && s < INFINITY;
                     acc[i][j][r] = normal ? acc[i][j][r] * s : acc[i][j][r] * fmaxf(xi, wi) * fminf(xi, wi);
                 }
+        }
+        if (__any(infinite)) {
+#pragma unroll 1
+            for (int e = 0; e < TM * TN * 4; ++e) {
+                const int ei = e / (TN * 4), ej = (e >> 2) % TN, er = e & 3;
+                const int64_t place = row0 + (wm * TM + ei) * 16 + (lane & 15);
+                const int col = col0 + (ej >> 1) * 32 + (ej & 1) * 4 + er;
+                if (place >= n || col >= out || !(x_inv[place] < 0.0f || w_inv[col] < 0.0f)) continue;
+                // the weights lie in fragment order: row m of tile nt
+                const int nt = (col >> 5) * 2 + (col >> 2 & 1), m = (col >> 3 & 3) * 4 + (col & 3);
+                const T* xr = x_plain + row_at(place) * in;
+                const T* wr = w_plain + ((int64_t)nt * kt_plain * 64 + m) * N;
+                float sum = 0.0f;
+#pragma unroll 1
+                for (int k = 0; k < in; ++k) {
+                    const int f = (k / (2 * DEPTH<T>)) * 2 + (k / N & 1), piece = k / (2 * N) & 3;
+                    sum = fmaf(xr[k], wr[((int64_t)f * 64 + piece * 16) * N + k % N], sum);
+                }
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int j = 0; j < TN; ++j)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) acc[i][j][r] = e == (i * TN + j) * 4 + r ? sum : acc[i][j][r];
+            }
         }
     }
     if (ids) {
@@ -903,7 +939,7 @@ void adapter_forward(const AdapterArgs& g) {
             const int tm = (int)((n + BM - 1) / BM), tn = (s.out + BN - 1) / BN;
             RVX_LAUNCH("adapter_tile", (tile_kernel<T, P, BM, BN, WM, WN, NS, decltype(kf)::value>), dim3((unsigned)(tm * tn)),
                        dim3(64 * WM * WN), 0, (const P*)xp, x_inv, n, (const P*)wp, g.w_inv, frags, s.nt, bias, b, s.b_slot,
-                       s.rk, g.ids, (const int32_t*)perm, g.slot, s.slots, t, s.out, tm, tn, y);
+                       s.rk, g.ids, (const int32_t*)perm, g.slot, s.slots, t, s.out, tm, tn, y, x, w, s.in, s.kt);
         };
         constexpr integral_constant<int, 1> I1{};
         constexpr integral_constant<int, 2> I2{};

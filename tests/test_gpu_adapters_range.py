@@ -5,6 +5,7 @@ import torch
 
 rv = pytest.importorskip("ruvector_amd")
 from heads_ref import DTYPES, F32, HALF, TINY, assert_within, to_buffer  # noqa: E402
+import test_gpu_adapters as adapters  # noqa: E402
 from test_gpu_adapters import run  # noqa: E402
 
 pytestmark = pytest.mark.gpu
@@ -149,3 +150,33 @@ def test_bf16_a_x_next_to_the_largest_float(n, sign):
     a[0, 3], a[0, 40] = sign * 2.0 ** 127, sign * (2.0 ** 127 - 2.0 ** 119)
     got = adapted(torch.ones(n, 64).bfloat16(), a, torch.full((20, 1), 2.0 ** -100).bfloat16(), "bf16")
     assert torch.equal(got, torch.full((n, 20), sign * 2.0 ** 28).bfloat16())  # 2^28 - 2^19 in 8 bits
+
+
+@pytest.mark.parametrize("n,out", [(9, 70), (64, 70), (65, 70), (200, 33), (700, 300), (1100, 4100)])
+@pytest.mark.parametrize("inp", [37, 100, 200])
+def test_f32_infinities(n, out, inp):
+    """Infinite outputs are infinite with their sign, NaN only where the formula is, in rows and outputs of
+    infinities and elsewhere, with bias and adapters."""
+    m = adapters.make(inp, out, n, [4, 9], "f32", bias=True)
+    x, w = m["x"], m["w"]
+    w[:, 5], w[::3, 7] = torch.where(torch.arange(out) % 2 == 0, 1.0, -0.5), 0.0  # few bits: parts that are 0
+    x[1, 5] = torch.inf
+    x[2, 7] = -torch.inf
+    x[n - 1, 5], x[n - 1, inp - 1] = torch.inf, -torch.inf
+    x[n // 2, 6] = torch.nan
+    x[4, 5], x[4, 6] = torch.inf, torch.nan
+    x[5, 9], x[6, 9] = 0.0, 1.0
+    w[out - 1, 9] = torch.inf
+    w[3, 10], w[3, 11] = -torch.inf, torch.nan
+    m["adapters"][1][1][7] = torch.inf
+    layer = adapters.layer_of(m, 9, "f32")
+    for ids in (None, m["ids"]):
+        got = run(layer, x, ids)
+        want = x.double() @ w.double().T + m["bias"].double()
+        if ids is not None:
+            for s, (a, b, scale) in enumerate(m["adapters"]):
+                at = torch.nonzero(ids == s)[:, 0]
+                want[at] += (scale * (x[at].double() @ a.double().T)) @ b.double().T
+        assert torch.equal(got.isnan(), want.isnan())
+        assert torch.equal(torch.where(got.isinf(), got.sign(), 0.0).double(), torch.where(want.isinf(), want.sign(), 0.0))
+        assert torch.isfinite(got).sum() > n * out // 2 - 8 * out or n < 20
