@@ -65,11 +65,15 @@ def _whole(value, what: str, bits: int) -> int:
 
 def int32(value, what: str) -> int:
     """`value` as a C int32 argument (ctypes would cut a larger one short)."""
+    if type(value) is int and -2 ** 31 <= value < 2 ** 31:
+        return value
     return _whole(value, what, 32)
 
 
 def int64(value, what: str) -> int:
     """`value` as a C int64 argument."""
+    if type(value) is int and -2 ** 63 <= value < 2 ** 63:
+        return value
     return _whole(value, what, 64)
 
 
