@@ -439,7 +439,7 @@ rvx_status rvx_log_probs_backward_device(const rvx_buffer* scores, int32_t dtype
  * rows: within 2^-39 of a row's largest value of it). The layer copies weights and adapters into its
  * own layout, so their buffers may be freed after the call. A row whose id is outside
  * [0, max_adapters), or names a slot never set or set with rank 0, has no adapter. An f32 layer
- * takes more than 64 rows as three bf16 values a number, each row of x and W scaled by a power of two:
+ * takes many rows as three bf16 values a number, each row of x and W scaled by a power of two:
  * a product x_j W_oj is then off by at most 2^-24 of itself (and 2^-188 max|x| max|W_o|), as an f32
  * product is. */
 typedef struct rvx_adapter_linear rvx_adapter_linear;

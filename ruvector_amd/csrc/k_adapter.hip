@@ -342,7 +342,7 @@ __global__ __launch_bounds__(64 * SHRINK_WAVES) void shrink_kernel(const T* __re
 }
 
 // ---------------------------------------------------------------- f32 as three bf16
-// f32 products of many rows run on the bf16 matrix instructions, 16 times the f32 ones' rate: a value is
+// f32 products of many rows, as far as they fill the card, run on the bf16 matrix instructions, 16 times the f32 ones' rate: a value is
 // exactly the sum of three bf16, h + m + l, each rounded to nearest from what the ones before leave:
 // 8 bits each, |m| <= 2^-8 |h|, |l| <= 2^-17 |h|. Of the nine products the six largest are taken, h h, h m,
 // m h, m m, h l and l h; the others are below 2^-24 |x w| together, half a step of an f32 product.
@@ -896,7 +896,12 @@ void adapter_forward(const AdapterArgs& g) {
         auto rounds = [&](int64_t bm, int64_t bn) { return (tiles(bm, bn) + cus - 1) / cus; };
         const int64_t row_tiles = (n + 15) / 16;
         // without adapters one row tile is read as it is: its 16-row loads cost less than another launch
-        T* packed = (F32 && !few) || (n <= 16 && !g.ids) ? nullptr : (T*)scratch_bytes("adapter_x", row_tiles * s.kt * 1024);
+        // f32, the smaller tiles' f32 instructions where a tile a CU is all there is, or two with short sums: the split
+        // and its launch cost more than six products at 16 times the rate save. Whole layer, f32 instructions and
+        // split: 1024 x 1024, 300 rows 36 and 40 us, 1000: 41 and 46, 1300: 58 and 52; 4096 x 4096, 250 rows 107 and
+        // 107, 320: 170 and 129; two tiles, 100 x 1000, 1500 rows 19 and 25; 768 x 768, 2048: 47 and 47.
+        const bool split = F32 && !few && tiles(64, 64) > (s.in <= 512 ? 2 : 1) * (int64_t)cus;
+        T* packed = split || (n <= 16 && !g.ids) ? nullptr : (T*)scratch_bytes("adapter_x", row_tiles * s.kt * 1024);
         // few row tiles: several blocks each, for the turns of different adapters and parts of the sum
         const unsigned spare = (unsigned)std::max<int64_t>(1, std::min<int64_t>(16, 2 * cus / row_tiles));
         const unsigned turns = g.ids ? few ? 16 : spare : 1, sums = few ? FEW_PARTS : g.ids ? 1 : std::min(spare, 4u);
@@ -948,6 +953,9 @@ void adapter_forward(const AdapterArgs& g) {
         constexpr integral_constant<int, 64> I64{};
         constexpr integral_constant<int, 128> I128{};
         constexpr integral_constant<int, 256> I256{};
+        if (!split) {
+            if constexpr (F32) return go(T{}, packed, nullptr, w, s.kt, I64, I64, I2, I2, I4, I2);
+        }
         if constexpr (F32) {
             const int ktq = split_frags(s.in);
             const int64_t bytes = row_tiles * ktq * SPLIT_PARTS * 1024;

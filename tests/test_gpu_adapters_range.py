@@ -180,3 +180,52 @@ def test_f32_infinities(n, out, inp):
         assert torch.equal(got.isnan(), want.isnan())
         assert torch.equal(torch.where(got.isinf(), got.sign(), 0.0).double(), torch.where(want.isinf(), want.sign(), 0.0))
         assert torch.isfinite(got).sum() > n * out // 2 - 8 * out or n < 20
+
+
+# Rows and outputs enough for the split into bf16 values, short sums and longer ones.
+MANY = [(1100, 1000, 600), (2200, 1000, 100)]
+
+
+@pytest.mark.parametrize("n,out,inp", MANY)
+@pytest.mark.parametrize("xe,we", [(-61, -61), (-20, -102), (-102, -20), (-58, -64), (60, 60), (100, -126), (-126, 100), (0, 0)])
+def test_f32_many_rows_near_the_ends(n, out, inp, xe, we):
+    g = torch.Generator().manual_seed(n - xe)
+    x, w = spread(g, n, inp) * 2.0 ** xe, spread(g, out, inp) * 2.0 ** we
+    assert_f32(f32_forward(x, w), x, w)
+
+
+@pytest.mark.parametrize("n,out,inp", MANY)
+@pytest.mark.parametrize("low,high", [(-5, 5), (-30, 30), (-62, 52), (-120, 0)])
+def test_f32_many_rows_of_any_spread(n, out, inp, low, high):
+    g = torch.Generator().manual_seed(n + high)
+    power = lambda *s: torch.randint(low, high + 1, s, generator=g).double()  # noqa: E731
+    x = (spread(g, n, inp).double() * 2.0 ** power(n, inp)).float()
+    w = (spread(g, out, inp).double() * 2.0 ** power(out, inp)).float()
+    if high == 0:  # the small values of x beside the large ones of W
+        x[:, ::2] = 0
+        x[:, 0] = 1
+        w[:, 0] = 2.0 ** -126
+        w[:, 1:] = spread(g, out, inp - 1) * 2.0 ** 100
+    assert_f32(f32_forward(x, w), x, w)
+
+
+@pytest.mark.parametrize("n,out,inp", MANY)
+def test_f32_many_rows_with_large_values_in_different_columns(n, out, inp):
+    x, w = torch.full((n, inp), 1.23 * 2.0 ** -26), torch.full((out, inp), 1.1)
+    x[:, 0], w[:, 0] = 1, 2.0 ** -40
+    assert_f32(f32_forward(x, w), x, w)
+
+
+@pytest.mark.parametrize("n,out,inp", MANY)
+def test_f32_many_rows_with_infinities(n, out, inp):
+    test_f32_infinities(n, out, inp)
+
+
+@pytest.mark.parametrize("n,out,inp", [(1100, 1000, 600), (2200, 1000, 100), (2100, 4090, 300)])
+def test_f32_many_rows_with_adapters(n, out, inp):
+    """The three sizes of tiles, against the tolerances of f32's own roundings."""
+    m = adapters.make(inp, out, n, [16, 0, 40], "f32", bias=True)
+    layer = adapters.layer_of(m, 40, "f32")
+    for ids in (m["ids"], torch.sort(m["ids"]).values):
+        want, tol = adapters.reference(m, ids, "f32")
+        assert_within(run(layer, m["x"], ids), want, tol)
