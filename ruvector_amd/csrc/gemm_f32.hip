@@ -797,8 +797,9 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-// packed form: v_pk_mul_f32, v_cvt_pk_f16_f32 (RNE) for the high parts, the exact residual
-// x - f32(h) (v_pk_add_f32) rounded the same way for the low parts — 6 VALU per pair
+// two values at once: their scaling, v_cvt_pk_f16_f32 (RNE) for the high parts, the exact residual
+// x - f32(h) rounded the same way for the low parts — 8 VALU per pair (packed f32 instructions, which
+// the build leaves out, would make it 6; the layers' GEMMs take the same time either way)
 __device__ __forceinline__ void split_h2_pair(float a0, float a1, float sc, unsigned& w1, unsigned& w2) {
     const f32x2 x = f32x2{a0, a1} * sc;
     const f16x2 h = __builtin_convertvector(x, f16x2);

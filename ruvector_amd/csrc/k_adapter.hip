@@ -412,8 +412,8 @@ __global__ __launch_bounds__(1024) void split_kernel(const float* __restrict__ x
 // ---------------------------------------------------------------- few rows
 // A block: a fragment tile's 16 outputs for all (<= 16 MT) rows; its waves split the sum and join in
 // LDS. Bound by reading W once: bf16 4096 x 4096 10 us for 1 row, 14 for 16, 20.6 for 64, with t.
-// As tiles (below): 33 rows 37 us to 19 here, 64 rows 36 to 21; f32 73 to 37; bf16 768 x
-// 768, 64 rows 17 to 11.5.
+// As tiles (below): 33 rows 37 us to 19 here, 64 rows 36 to 21; f32 106 to 39; bf16 768 x
+// 768, 64 rows 17 to 11.
 constexpr int FEW_WAVES = 16;
 
 // MT == 0: one row tile, x row-major.

@@ -332,7 +332,8 @@ __global__ __launch_bounds__(SMALL_THREADS) void sort_small_kernel(const int64_t
 // that is another key) are summed by a wave of their own, GROUP whole tails of one run once more
 // (`spans`), and the wave of the run's first group adds these. (A run of LONG entries touches an end
 // of its group.) Groups and order depend on the sorted ids alone. Ids as frequent as words, bf16 65536
-// x 1024: the rows kernel alone, one wave for the most frequent id, took 311 us of a gradient that takes 183.
+// x 1024: the rows kernel alone, one wave for the most frequent id, took 311 us of a gradient that takes 183
+// (167 with uniform ids).
 constexpr int GROUP = 64, LONG = 63;
 
 // A wave's columns of a row: V vectors of N columns a lane, vector q at (q * 64 + lane) * N.
@@ -523,7 +524,7 @@ __device__ __forceinline__ void zero_rows(unsigned char* table, int64_t rows, in
 // One wave per (sorted entry, slab): the first entry of an id sums the id's run into its row. Bound
 // by HBM: a wave takes up to 4 vectors a lane, so that a row's bytes are all in flight at once; f32
 // 500009 x 768, 100003 ids, added to the table: 4.9 TB/s. The first zero_blocks blocks set the
-// rows without an entry to zeros meanwhile: bf16 262144 x 1024, 65536 ids: 167 us, 181 with these in a
+// rows without an entry to zeros meanwhile: bf16 262144 x 1024, 65536 uniform ids: 167 us, 181 with these in a
 // launch on a second stream; bf16 512 columns, 20000 ids, a table of 512 MB: 129 us, 148 and, with the whole
 // table cleared before, 154; of 64 MB: 41, 63 and 49.
 template <class T, class S, int V>

@@ -7,9 +7,10 @@
 // E' = r (E + S d) + .. with d = (m - m') / T, r = e^d), so one pass suffices. All three are
 // kept in 32 bits, in units of log2, for v_exp_f32.
 //
-// The floor is one read of the scores. bf16 8192 x 32000: 97 us (5.4 TB/s) for log p and the statistics, 137
-// with rank, entropy and the best 5; f32 2503 x 10007: 17 and 31 us (the best 10). The difference is
-// instructions: rank, entropy and candidates take as many again as the sum.
+// It cannot do without one read of the scores. bf16 8192 x 32000: 97 us (5.4 TB/s) for log p and the statistics,
+// 111 to 137 with rank, entropy and the best 5; f32 2503 x 10007: 17 and 31 us (the best 10). The difference
+// is instructions: rank, entropy and candidates take as many again as the sum. 35 us with a tenth of the scores
+// masked: with the entropy, a step that holds a masked score takes its products twice.
 #include "heads.hpp"
 
 namespace rvx {
