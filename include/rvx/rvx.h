@@ -415,7 +415,8 @@ rvx_status rvx_embedding_backward_device(const rvx_buffer* grad_out, int32_t dty
  *                      lowest id first among equals; -1 / -inf past the scores above -inf
  * logp and rank need targets. Scores of -inf are masked: p = 0. A row with nothing above -inf has
  * logp -inf, entropy 0, stats (-inf, -inf). A NaN or a +inf makes its row's logp, entropy and log
- * sum NaN; NaN is never ranked or listed. */
+ * sum NaN; a NaN is never counted before a target or listed, and nothing counts before a target that
+ * is NaN (rank 0, logp NaN). */
 rvx_status rvx_log_probs_device(const rvx_buffer* scores, int32_t dtype, int64_t n, int64_t c, int64_t ld,
                                 float temperature, const rvx_buffer* targets_i64, int32_t k, rvx_buffer* logp,
                                 rvx_buffer* rank_i64, rvx_buffer* entropy, rvx_buffer* stats, rvx_buffer* top_ids_i64,

@@ -229,3 +229,15 @@ def test_f32_many_rows_with_adapters(n, out, inp):
     for ids in (m["ids"], torch.sort(m["ids"]).values):
         want, tol = adapters.reference(m, ids, "f32")
         assert_within(run(layer, m["x"], ids), want, tol)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("inp", [1, 2, 7, 15, 16, 17, 31, 33, 65])
+@pytest.mark.parametrize("n,out", [(65, 1), (130, 2), (300, 33), (2100, 1030)])
+def test_short_sums(dtype, inp, n, out):
+    """Sums of one stage and less, by every form of the tiles."""
+    m = adapters.make(inp, out, n, [1, 17], dtype, bias=True)
+    layer = adapters.layer_of(m, 17, dtype)
+    for ids in (m["ids"], None):
+        want, tol = adapters.reference(m, ids, dtype)
+        assert_within(run(layer, m["x"], ids), want, tol)

@@ -159,3 +159,17 @@ def test_adapters_with_long_sums(dtype, inp, out, n, ranks, max_rank):
         want, tol = adapters.reference(m, ids, dtype)
         assert_within(got, want, tol)
         assert torch.equal(adapters.run(layer, m["x"], ids), got)
+
+
+@pytest.mark.parametrize("n,c", [(3, 40), (3, 9000), (2100, 1500)])
+def test_rank_of_a_nan(n, c):
+    """A NaN counts before no target, and no score before a target that is NaN."""
+    scores, targets = logprobs.make(n, c, "f32")
+    targets[:] = c // 2
+    clean = logprobs.forward(scores, targets, 1.0, 0, "f32")
+    scores[0, c // 2] = math.nan
+    scores[1, c - 1] = math.nan
+    before = int(clean["rank"][1]) - int((logprobs.make(n, c, "f32")[0][1, c - 1] > scores[1, c // 2]))
+    got = logprobs.forward(scores, targets, 1.0, 0, "f32")
+    assert got["rank"][0] == 0 and got["logp"][0].isnan()
+    assert got["rank"][1] == before and torch.equal(got["rank"][2:], clean["rank"][2:])
