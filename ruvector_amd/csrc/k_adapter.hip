@@ -865,6 +865,20 @@ void adapter_split(const AdapterShape& s, const float* w, void* parts, float* in
 
 void adapter_forward(const AdapterArgs& g) {
     const AdapterShape& s = g.s;
+    // f32, up to 128 rows and long sums: twice the kernels for few rows, which read W once each. Whole layer, so and by
+    // tiles: 4096 x 4096, 65 rows 58 and 106 us, 128: 74 and 105; 768 x 768 22 and 30, 28 and 30; 3000 x 100 41 and
+    // 77, 57 and 77; three times, 160 rows: 768 x 768 39 and 30; short sums, 100 x 3000, 128 rows: 22 and 16.
+    if (s.dtype == RVX_DTYPE_F32 && g.n > 64 && g.n <= 128 && s.in > 512) {
+        for (int64_t r = 0; r < g.n; r += 64) {
+            AdapterArgs part = g;
+            part.n = std::min<int64_t>(64, g.n - r);
+            part.x = (const float*)g.x + r * s.in;
+            part.y = (float*)g.y + r * s.out;
+            part.ids = g.ids ? g.ids + r : nullptr;
+            adapter_forward(part);
+        }
+        return;
+    }
     using std::integral_constant;
     with_dtype(s.dtype, [&](auto zero) {
         using T = decltype(zero);

@@ -241,3 +241,14 @@ def test_short_sums(dtype, inp, n, out):
     for ids in (m["ids"], None):
         want, tol = adapters.reference(m, ids, dtype)
         assert_within(run(layer, m["x"], ids), want, tol)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [64, 65, 66, 100, 127, 128, 129])
+@pytest.mark.parametrize("inp,out", [(512, 40), (513, 40), (700, 130)])
+def test_up_to_twice_64_rows(dtype, n, inp, out):
+    m = adapters.make(inp, out, n, [3, 20, 0], dtype, bias=True)
+    layer = adapters.layer_of(m, 20, dtype)
+    for ids in (m["ids"], None):
+        want, tol = adapters.reference(m, ids, dtype)
+        assert_within(run(layer, m["x"], ids), want, tol)
