@@ -210,15 +210,15 @@ struct Part {  // what one block found of one row
 };
 
 // (score - m) / T; halves, as the difference itself may be past the largest float
-__device__ __forceinline__ float gap(float score, float m, float inv_t) {
-    return 2.0f * ((0.5f * score - 0.5f * m) * inv_t);
+__device__ __forceinline__ float gap(float score, float m, float temp) {
+    return 2.0f * ((0.5f * score - 0.5f * m) / temp);
 }
 __device__ __forceinline__ void write_row(const Stat& st, int before, int64_t row, float st_score, bool has_target,
-                                          float inv_t, const LogProbsOut& out) {
+                                          float temp, const LogProbsOut& out) {
     const bool empty = st.s == 0.0f;
     const float m = empty ? -INFINITY : st.m;
     const float log_sum = empty ? -INFINITY : logf(st.s);
-    if (out.logp) out.logp[row] = !has_target ? 0.0f : empty ? -INFINITY : gap(st_score, m, inv_t) - log_sum;
+    if (out.logp) out.logp[row] = !has_target ? 0.0f : empty ? -INFINITY : gap(st_score, m, temp) - log_sum;
     if (out.rank) out.rank[row] = has_target ? before : -1;
     if (out.entropy) out.entropy[row] = empty ? 0.0f : log_sum - LN2 * (st.e / st.s);
     if (out.stats) {
@@ -226,14 +226,14 @@ __device__ __forceinline__ void write_row(const Stat& st, int before, int64_t ro
         out.stats[2 * row + 1] = log_sum;
     }
 }
-__device__ __forceinline__ void write_top(u64 list, int k, int64_t row, const Stat& st, float inv_t,
+__device__ __forceinline__ void write_top(u64 list, int k, int64_t row, const Stat& st, float temp,
                                           const LogProbsOut& out) {
     const int lane = threadIdx.x & 63;
     if (lane >= k) return;
     const bool none = list == 0;
     if (out.top_ids) out.top_ids[row * k + lane] = none ? -1 : (int64_t)(0xffffffffu - (uint32_t)list);
     if (out.top_logp)
-        out.top_logp[row * k + lane] = none ? -INFINITY : gap(key_score(list), st.m, inv_t) - logf(st.s);
+        out.top_logp[row * k + lane] = none ? -INFINITY : gap(key_score(list), st.m, temp) - logf(st.s);
 }
 
 // ---------------------------------------------------------------- one pass
@@ -431,7 +431,7 @@ struct Row {  // a row's target
 // A wave a row (many rows).
 template <class T, bool ENT, bool RANK, bool TOP>
 __global__ __launch_bounds__(64 * LP_WAVES) void logprobs_wave_kernel(const T* __restrict__ scores, int64_t n, int64_t c,
-                                                                     int64_t ld, float c1, float inv_t,
+                                                                     int64_t ld, float c1, float temp,
                                                                      const int64_t* __restrict__ targets, int k,
                                                                      LogProbsOut out) {
     constexpr int ROOM = Best::ROOM;
@@ -444,15 +444,15 @@ __global__ __launch_bounds__(64 * LP_WAVES) void logprobs_wave_kernel(const T* _
     int before = 0;
     Best best(TOP ? pend + wave * ROOM : nullptr, k);
     const Stat st = walk<T, ENT, RANK, TOP>(x, 0, c, c1, r.target, r.score, before, best);
-    if ((threadIdx.x & 63) == 0) write_row(st, before, row, r.score, r.there, inv_t, out);
-    if constexpr (TOP) write_top(best.list, k, row, st, inv_t, out);
+    if ((threadIdx.x & 63) == 0) write_row(st, before, row, r.score, r.there, temp, out);
+    if constexpr (TOP) write_top(best.list, k, row, st, temp, out);
 }
 
 // A block a row, or one of `splits` parts of a row: its waves take a quarter each and join in LDS.
 // parts == null: the block has the whole row.
 template <class T, bool ENT, bool RANK, bool TOP>
 __global__ __launch_bounds__(64 * LP_WAVES) void logprobs_block_kernel(const T* __restrict__ scores, int64_t c, int64_t ld,
-                                                                      float c1, float inv_t,
+                                                                      float c1, float temp,
                                                                       const int64_t* __restrict__ targets, int k,
                                                                       int splits, int64_t seg_len, Part* parts, u64* keys,
                                                                       LogProbsOut out) {
@@ -482,8 +482,8 @@ __global__ __launch_bounds__(64 * LP_WAVES) void logprobs_block_kernel(const T* 
         if constexpr (TOP) best.take(lists[w][63 - lane]);
     }
     if (!parts) {
-        if (lane == 0) write_row(st, before, row, r.score, r.there, inv_t, out);
-        if constexpr (TOP) write_top(best.list, k, row, st, inv_t, out);
+        if (lane == 0) write_row(st, before, row, r.score, r.there, temp, out);
+        if constexpr (TOP) write_top(best.list, k, row, st, temp, out);
     } else {
         if (lane == 0) parts[blockIdx.x] = Part{st.m, st.s, st.e, before};
         if constexpr (TOP)
@@ -494,7 +494,7 @@ __global__ __launch_bounds__(64 * LP_WAVES) void logprobs_block_kernel(const T* 
 // One wave a row: joins the parts of its blocks in their order.
 template <class T>
 __global__ __launch_bounds__(64) void logprobs_join_kernel(const T* __restrict__ scores, int64_t c, int64_t ld, float c1,
-                                                           float inv_t, const int64_t* __restrict__ targets, int k,
+                                                           float temp, const int64_t* __restrict__ targets, int k,
                                                            int splits, const Part* __restrict__ parts,
                                                            const u64* __restrict__ keys, LogProbsOut out) {
     __shared__ u64 pend[Best::ROOM];
@@ -513,7 +513,7 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(const T* __restrict__
     st = join_lanes(st, c1);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o);
-    if (lane == 0) write_row(st, before, row, r.score, r.there, inv_t, out);
+    if (lane == 0) write_row(st, before, row, r.score, r.there, temp, out);
     if (k) {
         Best best(pend, k);
         const u64* list = keys + row * splits * k;
@@ -533,7 +533,7 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(const T* __restrict__
                 }
         }
         if (best.waiting) best.flush();
-        write_top(best.list, k, row, st, inv_t, out);
+        write_top(best.list, k, row, st, temp, out);
     }
 }
 
@@ -608,7 +608,7 @@ __global__ __launch_bounds__(256) void logprobs_backward_kernel(
 
 void log_probs(int32_t dtype, const void* scores, int64_t n, int64_t c, int64_t ld, float temperature,
                const int64_t* targets, int k, const LogProbsOut& out) {
-    const float inv_t = (float)(1.0 / (double)temperature), c1 = (float)(1.44269504088896340736 / (double)temperature);
+    const float c1 = (float)(1.44269504088896340736 / (double)temperature);
     with_dtype(dtype, [&](auto zero) {
         using T = decltype(zero);
         constexpr int64_t STEP = Step<T>::SIZE;
@@ -646,10 +646,10 @@ void log_probs(int32_t dtype, const void* scores, int64_t n, int64_t c, int64_t 
                 if (by_wave)
                     RVX_LAUNCH("log_probs", (logprobs_wave_kernel<T, E, R, K>),
                                dim3((unsigned)((rows + LP_WAVES - 1) / LP_WAVES)), dim3(64 * LP_WAVES), 0, x, rows, c, ld, c1,
-                               inv_t, t, k, o);
+                               temperature, t, k, o);
                 else
                     RVX_LAUNCH("log_probs", (logprobs_block_kernel<T, E, R, K>), dim3((unsigned)(rows * splits)),
-                               dim3(64 * LP_WAVES), 0, x, c, ld, c1, inv_t, t, k, (int)splits, seg, parts, keys, o);
+                               dim3(64 * LP_WAVES), 0, x, c, ld, c1, temperature, t, k, (int)splits, seg, parts, keys, o);
             };
             auto flag = [](bool on, auto&& f) {
                 if (on) f(std::true_type{});
@@ -659,7 +659,7 @@ void log_probs(int32_t dtype, const void* scores, int64_t n, int64_t c, int64_t 
                 flag(out.rank != nullptr, [&](auto q) { flag(k > 0, [&](auto p) { go(e, q, p); }); });
             });
             if (splits > 1)
-                RVX_LAUNCH("log_probs_join", logprobs_join_kernel<T>, dim3((unsigned)rows), dim3(64), 0, x, c, ld, c1, inv_t, t,
+                RVX_LAUNCH("log_probs_join", logprobs_join_kernel<T>, dim3((unsigned)rows), dim3(64), 0, x, c, ld, c1, temperature, t,
                            k, (int)splits, (const Part*)parts, (const u64*)keys, o);
         }
     });
